@@ -32,6 +32,7 @@ extern "C" {
 #define MFD_DEVERR_BAD_CONTEXT 8     /* a tree context built for another request size or max_nodes */
 #define MFD_DEVERR_BAD_WINDOW 16     /* a conv window or accepted-path index outside its request / tree */
 #define MFD_DEVERR_INTERNAL 32       /* a workgroup-internal hand-over wait ran out: that workgroup's outputs are NaN */
+#define MFD_DEVERR_BAD_PAGE 64       /* a page id, table row, length or token count outside its bounds */
 
 #define MFD_GDN_HEAD_DIM 128
 #define MFD_GDN_MAX_DEPTH 16  /* nodes on a root path, root included */
@@ -383,6 +384,92 @@ int mfd_draft_prepare(const void* bonus_tokens, const void* prefix_lens, const v
  */
 int mfd_mode_mask(const int64_t* prefix_lens, const int64_t* mask_offsets, uint8_t* mask_out, int bs, int num_modes,
                   int block_size, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit draft KV cache
+ * A paged cache of e4m3 codes (OCP: 448 the largest, 0x7f / 0xff NaN) with one float32 scale per page and KV head for K
+ * and one for V; a value is code * scale. Scales are powers of two between 2^-40 and 2^40: the kernels shift exponents
+ * by them, and mfd_kv8_store writes the smallest one that puts the page's largest finite magnitude at or below 448.
+ *
+ *   k_cache/v_cache  slot s, KV head g: k_cache + s * kc_ss + g * kc_sh, 128 codes (uint8); bases and strides multiples of 16
+ *   k_scale/v_scale  [num_pages][Hkv] f32
+ *   page_table       [table_rows][table_width] int32, row stride table_stride: token t of request b lies at slot
+ *                    page_table[row][t / page_size] * page_size + t % page_size, row = req_idx ? req_idx[b] : b (device
+ *                    int64). page_size 16, 32, 64, 128 or 256
+ *   err_flag         optional; MFD_DEVERR_BAD_PAGE where a page id, row, length or count lies outside its bound. Nothing
+ *                    out of bounds is read or written: a store skips such pages, reads take page 0 for such a page id and
+ *                    no tokens for such a row, and lengths end where the table row ends.
+ *
+ * mfd_kv8_store: new tokens of a batch. Request b's tokens are rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of k / v
+ * (cu_tokens [bs + 1] int32 device, values up to N; row n, KV head g: k + n * kn_st + g * kn_sh, bf16) and go to the
+ * positions start_lens[b], start_lens[b] + 1, ... A page whose first token is among them begins anew; in a page begun
+ * earlier the scale only grows, and the page's entries before the new ones are then rounded again from their old codes
+ * (a shift, exact but for codes that become subnormal). Entries behind the new ones keep their bits. Infinities become
+ * +-448 * scale, NaN stays NaN. max_tokens: an upper bound of a request's new tokens (host; more of them are not stored
+ * and flagged). A page belongs to one request of a call: two requests storing into one page race.
+ */
+int mfd_kv8_store(const uint16_t* k, const uint16_t* v, int64_t kn_st, int64_t kn_sh, int64_t vn_st, int64_t vn_sh,
+                  uint8_t* k_cache, uint8_t* v_cache, int64_t kc_ss, int64_t kc_sh, int64_t vc_ss, int64_t vc_sh,
+                  float* k_scale, float* v_scale, int num_pages, const int32_t* page_table, int64_t table_stride,
+                  int table_rows, int table_width, int page_size, const int64_t* req_idx, const int64_t* start_lens,
+                  const int32_t* cu_tokens, int N, int bs, int max_tokens, int Hkv, int D, int32_t* err_flag,
+                  void* stream);
+
+/* mfd_mode_attn over the 8-bit cache: the same modes, GQA and block keys (bf16, own mode only).
+ *   k_new / v_new  both NULL: no block keys (queries attend to the cache alone: plain decoding, num_modes 1,
+ *                  block_size 1, after the token was stored). A row without any key gets output 0 and lse -inf
+ *   num_ctx_splits, split_keys  1: one pass. > 1: split i takes the keys i * split_keys .. of every request (the last one
+ *                  all that are left), so a request gets as many workgroups as its length asks for; split_keys a multiple
+ *                  of 64
+ *   lse            [bs K L][H] f32, natural log-sum-exp of a row's scaled scores, block keys included; or NULL
+ *   workspace      mfd_kv8_attn_workspace_bytes(...) bytes, 16-byte aligned (NULL allowed when 0); with_block: k_new given
+ */
+int64_t mfd_kv8_attn_workspace_bytes(int bs, int num_modes, int block_size, int H, int Hkv, int with_block,
+                                     int num_ctx_splits);
+int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* k_new, const uint16_t* v_new,
+                 int64_t kn_st, int64_t kn_sh, int64_t vn_st, int64_t vn_sh, const uint8_t* k_cache,
+                 const uint8_t* v_cache, int64_t kc_ss, int64_t kc_sh, int64_t vc_ss, int64_t vc_sh,
+                 const float* k_scale, const float* v_scale, int num_pages, const int32_t* page_table,
+                 int64_t table_stride, int table_rows, int table_width, int page_size, const int64_t* req_idx,
+                 const int64_t* ctx_lens, int bs, int num_modes, int block_size, int H, int Hkv, int D, float scale,
+                 int causal_in_block, int num_ctx_splits, int split_keys, uint16_t* out, int64_t o_st, int64_t o_sh,
+                 float* lse, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream);
+
+/* Attention weight that each cached token received, added to its running sum:
+ *   weights[row][h][t] = decay * weights[row][h][t] + sum over KV head h's query rows of exp(scale q.k_t - lse)
+ * for t < ctx_lens[b]; other entries keep their values. lse [bs K L][H] as mfd_kv8_attn writes it (rows of -inf add
+ * nothing). weights: [w_rows][Hkv][width] f32 with row and head strides, row = req_idx ? req_idx[b] : b; decay in [0, 1]
+ * (0: the old sums are not read). Every sum is formed in one order: results repeat bit for bit. */
+int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, const float* lse, const uint8_t* k_cache,
+                    int64_t kc_ss, int64_t kc_sh, const float* k_scale, int num_pages, const int32_t* page_table,
+                    int64_t table_stride, int table_rows, int table_width, int page_size, const int64_t* req_idx,
+                    const int64_t* ctx_lens, int bs, int num_modes, int block_size, int H, int Hkv, int D, float scale,
+                    float decay, float* weights, int64_t w_row_stride, int64_t w_head_stride, int w_rows, int width,
+                    int32_t* err_flag, void* stream);
+
+/* Tokens to keep by those sums. A token's score is the sum over KV heads of weights[row][h][t], formed in fp64 and rounded
+ * once to fp32. Of a request longer than `budget`, the first `sink` and the last `recent` tokens stay, and of the rest
+ * those with the largest scores (ties: the lowest position; NaN below everything); a shorter one keeps all.
+ *   keep      [bs][budget] int32: the kept positions, ascending, -1 behind them;  new_lens [bs] int64: how many
+ *   workspace mfd_evict_select_workspace_bytes(bs, width) bytes, 16-byte aligned
+ *   1 <= budget, sink + recent <= budget
+ */
+int64_t mfd_evict_select_workspace_bytes(int bs, int width);
+int mfd_evict_select(const float* weights, int64_t w_row_stride, int64_t w_head_stride, int w_rows, int width, int Hkv,
+                     const int64_t* req_idx, const int64_t* ctx_lens, int bs, int budget, int sink, int recent,
+                     int32_t* keep, int64_t* new_lens, void* workspace, int64_t workspace_bytes, int32_t* err_flag,
+                     void* stream);
+
+/* Kept tokens (keep, new_lens as mfd_evict_select writes them) moved from the pages of src_table to those of dst_table, in
+ * order, rounded with each destination page's own scale; destination pages must not be among the call's source pages.
+ * Entries of a destination page behind the last kept token keep their bits. weights (or NULL): the running sums move along
+ * in place (entry i <- entry keep[i]), and those from new_lens[b] to ctx_lens[b] become 0. */
+int mfd_evict_compact_kv8(const int32_t* keep, int budget, const int64_t* new_lens, const int64_t* ctx_lens,
+                          uint8_t* k_cache, uint8_t* v_cache, int64_t kc_ss, int64_t kc_sh, int64_t vc_ss,
+                          int64_t vc_sh, float* k_scale, float* v_scale, int num_pages, const int32_t* src_table,
+                          int64_t src_stride, int src_rows, int src_width, const int32_t* dst_table, int64_t dst_stride,
+                          int dst_rows, int dst_width, int page_size, const int64_t* req_idx, float* weights,
+                          int64_t w_row_stride, int64_t w_head_stride, int w_rows, int width, int bs, int Hkv, int D,
+                          int32_t* err_flag, void* stream);
 
 #ifdef __cplusplus
 }

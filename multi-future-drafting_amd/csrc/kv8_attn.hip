@@ -1,0 +1,1218 @@
+// Mode attention over the 8-bit draft KV cache (kv8_common.h) for gfx950, and the attention weight that each cached
+// token received.
+//
+//   o[row] = sum_t p[row, t] v_t,  p = softmax(scale q k_t)  over the request's cached tokens (k_t = code * k_scale,
+//   v_t = code * v_scale of the token's page) and, where they are given, the bf16 keys of the row's own mode block;
+//   lse[row] = log sum exp, natural;   w[h][t] = decay w[h][t] + sum over KV head h's query rows of
+//   exp(scale q k_t - lse[row]).
+//
+// A KV head's query rows (G query heads x K L queries, head-major) are packed into units of 32, the column count of
+// v_mfma_f32_32x32x16: only the last unit of a KV head is padded, whatever K L is. Scores are S^T = K Q^T in bf16 (a code
+// has four significant bits and the scale is a power of two, so k is exact in bf16 and every product in fp32) and
+// O^T += V^T P^T in fp16: V as bare codes (exact), P rounded to fp16 (2^-11 at most, an eighth of the bf16 output's own
+// rounding), the accumulators kept in units of the current page's v_scale and multiplied by the quotient of two scales,
+// a power of two, where the next 16 tokens have another one. Statistics are fp32.
+//
+// Two kernels, by the units of a KV head:
+//  * tile kernel: the waves of a workgroup (a unit each) share 64-key tiles. The codes come from memory to registers, two
+//    tiles ahead, and are widened on their way into LDS (K to bf16 with its scale folded in by the conversion, V to
+//    fp16), so that each code is widened once per workgroup and the products find plain MFMA operands: two buffers each
+//    of K and V, one barrier per tile. Scores of tile t + 1 and the products of tile t run interleaved in 32 slots.
+//  * stream kernel, for one unit per KV head (plain decoding): nothing is shared, so each wave walks 32-key tiles of its
+//    own through its own LDS, without barriers, and the waves' results meet at the end. Bound by the cache's way from
+//    memory.
+// Both split a context over workgroups (a fixed number of keys each, so that a batch's long contexts become more
+// workgroups, not longer ones) and merge by log-sum-exp.
+#include <algorithm>
+
+#include "kv8_common.h"
+
+namespace {
+
+using kv8::D;
+using kv8::Pages;
+using kv8::u32x4;
+
+constexpr int TK = 64;         // keys per tile of the tile kernel
+constexpr int TILE = TK * D;   // 16-bit elements of a widened tile (16 KB)
+constexpr int UROWS = 32;      // query rows per unit
+constexpr int SK = 32;         // keys per tile of the stream kernel
+constexpr int SNW = 4;         // its waves
+constexpr float LN2 = 0.6931471805599453f;
+
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct Args {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint16_t* kn;  // NULL: no block keys
+  const uint16_t* vn;
+  int64_t kn_st, kn_sh, vn_st, vn_sh;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  int64_t kc_ss, kc_sh, vc_ss, vc_sh;
+  const float* ks;  // [pages][Hkv]
+  const float* vs;
+  Pages pages;
+  const int64_t* ctx_lens;
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  float* lse;      // [bs K L][H] or NULL
+  uint16_t* ws_o;  // [S][bs][Hkv][rows][D] fp16: the partial output row divided by 2^ws_exp
+  float* ws_lse;   // [S][bs][Hkv][rows], base 2
+  float* ws_exp;   // [S][bs][Hkv][rows] the row's power-of-two scale exponent
+  int bs, K, L, H, Hkv, G, KL, rows;  // rows = G K L: query rows of a KV head
+  int SC, S, split_keys;              // context splits; partials (tile kernel: one more for the block keys)
+  int causal, ngroups;
+  float scale_log2;
+  int32_t* err_flag;
+};
+
+__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+// Workgroup barrier that is also a compiler memory barrier, with this wave's LDS operations done. Global loads in
+// flight are not waited for: the next tiles' codes stay on their way across it.
+__device__ __forceinline__ void lds_barrier() {
+  wait_lgkmcnt0();
+  asm volatile("s_barrier" ::: "memory");
+}
+
+// The value of the other 32-lane half beside the own (see v_permlane32_swap; the copy is opaque, or the compiler would
+// take the two results for equal).
+__device__ __forceinline__ int2 both_halves(float x) {
+  int y;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(y) : "v"(__builtin_bit_cast(int, x)));
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, x), y, false, false);
+  return make_int2(r[0], r[1]);
+}
+__device__ __forceinline__ float half_max(float x) {
+  const int2 r = both_halves(x);
+  return fmaxf(__builtin_bit_cast(float, r.x), __builtin_bit_cast(float, r.y));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const int2 r = both_halves(x);
+  return __builtin_bit_cast(float, r.x) + __builtin_bit_cast(float, r.y);
+}
+__device__ __forceinline__ uint32_t f2h2_bits(float x0, float x1) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x0, x1}, f16x2));
+}
+__device__ __forceinline__ uint32_t f2bf2_bits(float x0, float x1) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x0, x1}, bf16x2));
+}
+__device__ __forceinline__ f32x2 h2_to_f2(uint32_t h) {
+  return __builtin_convertvector(__builtin_bit_cast(f16x2, h), f32x2);
+}
+__device__ __forceinline__ f32x16 mfma32_f16(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// 16 codes -> 16 bf16 values times s (exact), as two 16-byte chunks; 16 codes -> 16 fp16 values (exact)
+__device__ __forceinline__ void widen_k(const u32x4& c, float s, u32x4& lo, u32x4& hi) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s, false));
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s, true));
+    if (e < 2) { lo[2 * e] = a; lo[2 * e + 1] = b; }
+    else { hi[2 * e - 4] = a; hi[2 * e - 3] = b; }
+  }
+}
+__device__ __forceinline__ void widen_v(const u32x4& c, u32x4& lo, u32x4& hi) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[e], 1.f, false));
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[e], 1.f, true));
+    if (e < 2) { lo[2 * e] = a; lo[2 * e + 1] = b; }
+    else { hi[2 * e - 4] = a; hi[2 * e - 3] = b; }
+  }
+}
+// A row's 16-byte chunks 2 part and 2 part + 1 into a widened tile ([key][d] rows of 256 bytes, chunk c of key r at
+// position c ^ swz). Parts 4 .. 7 write the upper one first: the eight lanes of a row then hit all banks at once.
+__device__ __forceinline__ void put_row(uint16_t* tile, int r, int part, int swz, const u32x4& lo, const u32x4& hi) {
+  const bool up = part >= 4;
+  const u32x4 first = up ? hi : lo, second = up ? lo : hi;
+  const int c0 = 2 * part + (up ? 1 : 0);
+  *reinterpret_cast<u32x4*>(tile + (r * 16 + (c0 ^ swz)) * 8) = first;
+  *reinterpret_cast<u32x4*>(tile + (r * 16 + ((c0 ^ 1) ^ swz)) * 8) = second;
+}
+__device__ __forceinline__ int k_swz(int r) { return r & 15; }
+__device__ __forceinline__ int v_swz(int r) { return (r & 3) << 2; }
+
+// Quotient a / b of two scales given as bits: powers of two
+__device__ __forceinline__ float scale_quotient(uint32_t a, uint32_t b) { return __uint_as_float(a - b + 0x3f800000u); }
+
+// Request of scheduling rank rho: requests by context length, longest first (ties by index), so that the longest
+// workgroups start first and short ones fill in behind them.
+__device__ __forceinline__ int request_of_rank(const int64_t* ctx_lens, int bs, int rho) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < bs; base += 64) {
+    const int b = base + lane;
+    int rank = -1;
+    if (b < bs) {
+      const int64_t cb = ctx_lens[b];
+      rank = 0;
+      for (int j = 0; j < bs; ++j) {
+        const int64_t cj = ctx_lens[j];
+        rank += (cj > cb || (cj == cb && j < b)) ? 1 : 0;
+      }
+    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(rank == rho);
+    if (hit) return base + __builtin_ctzll(hit);
+  }
+  return rho;
+}
+
+// The keys [lo, hi) of context split s
+__device__ __forceinline__ void split_range(const Args& a, int s, int ctx, int& lo, int& hi) {
+  lo = 0;
+  hi = ctx;
+  if (a.SC > 1) {
+    lo = (int)min((int64_t)s * a.split_keys, (int64_t)ctx);
+    if (s < a.SC - 1) hi = min(lo + a.split_keys, ctx);  // (the last split takes what a longer context has left)
+  }
+}
+
+// Index of a query row in the partials
+__device__ __forceinline__ int64_t partial_row(const Args& a, int s, int b, int kvh, int r) {
+  return (((int64_t)s * a.bs + b) * a.Hkv + kvh) * a.rows + r;
+}
+
+// ------------------------------------------------------------------------------------------------ tile kernel
+
+template <int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attn_tile_kernel(Args a) {
+  static_assert(NW == 4 || NW == 8, "workgroups of 4 or 8 waves");
+  constexpr int NPT = 8 / NW;   // 16-code pieces of a K or V tile per thread
+  constexpr int RSTEP = NW * 8;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds_k[2 * TILE], lds_v[2 * TILE];
+  __shared__ uint32_t lds_vs[2 * TK];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, l32 = lane & 31;
+  const int KL = a.KL, Lb = a.L, rows = a.rows;
+  const bool causal = a.causal != 0;
+  const float scale_log2 = a.scale_log2;
+
+  // workgroup -> (request by rank, KV head, split, unit group); the unit groups that read the same keys are consecutive
+  // on one XCD (workgroup id modulo 8) and share its L2
+  const int P = a.bs * a.Hkv * a.S;
+  const int jx = blockIdx.x >> 3;
+  const int ug = jx % a.ngroups;
+  const int pidx = (jx / a.ngroups) * 8 + (blockIdx.x & 7);
+  if (pidx >= P) return;
+  const int s = pidx % a.S;
+  const int kvh = (pidx / a.S) % a.Hkv;
+  const int rho = pidx / a.S / a.Hkv;
+  const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+
+  // this lane's query row; a padding row computes a copy of the last one and stores nothing
+  const int u0 = (ug * NW + w) * UROWS;
+  const bool active = u0 < rows;  // the wave has a row
+  const bool row_ok = u0 + l32 < rows;
+  const int r = min(u0 + l32, rows - 1);
+  const int head = kvh * a.G + r / KL;
+  const int qi = r % KL;
+  const int64_t token = (int64_t)b * KL + qi;
+  const int mode_lo = (qi / Lb) * Lb;  // first block key of this row's mode
+
+  bf16x8 qf[D / 16];  // Q^T: B operand, k = d = 16 c + 8 half + e
+  {
+    const uint16_t* qp = a.q + token * a.q_st + (int64_t)head * a.q_sh + half * 8;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) qf[c] = as_bf16x8(*reinterpret_cast<const u16x8*>(qp + c * 16));
+  }
+  const int32_t* trow = kv8::table_row(a.pages, b);
+  const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
+  const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0);
+  int lo, hi;
+  split_range(a, s, ctx, lo, hi);
+  bool with_block = a.kn != nullptr;
+  if (a.S > a.SC) {  // split: the block keys are a partial of their own
+    if (s == a.SC) lo = hi = ctx;
+    else with_block = false;
+  }
+  const int ntiles = (hi - lo + TK - 1) / TK;
+  const int last = ntiles - 1;
+  if (tid == 0 && s == 0 && ug == 0 && kvh == 0 && ctx != a.ctx_lens[b]) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  if (a.S > 1 && ntiles == 0 && !with_block) {  // an empty split
+    if (row_ok && half == 0) a.ws_lse[partial_row(a, s, b, kvh, r)] = -INFINITY;
+    return;
+  }
+
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16 oacc[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) oacc[db] = (f32x16){};
+  uint32_t vcur = 0x3f800000u;  // the accumulators' unit: bits of the page scale of the last 16 keys
+
+  // LDS offsets (elements) of the MFMA operands. K row 32 ks + l32, d chunk 2 c + half: (k_base ^ (c << 4)) + 4096 ks.
+  // V^T fragment of d block db and 16-key chunk c (ds_read_b64_tr_b16): (v_base ^ (db << 5)) + 2048 c, + 1024 for the
+  // chunk's second 4-key group. The k order within a chunk is the row order of S^T's accumulators, so P needs no move.
+  const int k_base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
+  int v_base;
+  {
+    const int grp = lane >> 4, sl = lane & 15, sw = sl >> 2;
+    v_base = (4 * half + sw) * 128 + (sw << 5) + (2 * (grp & 1) + ((sl & 3) >> 1)) * 8 + (sl & 1) * 4;
+  }
+  auto v_frag = [&](int off) __attribute__((always_inline)) {
+    const v4i16 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off));
+    const v4i16 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off + 1024));
+    const v4i16 v[2] = {x0, x1};
+    return __builtin_bit_cast(u32x4, v);
+  };
+  // S^T of the tile in K buffer j: keys 32 ks + 8 (x / 4) + 4 half + x % 4 (x: register), column = this lane's row
+  auto scores = [&](int j, f32x16 (&sv)[2]) __attribute__((always_inline)) {
+    const int kb = k_base + j * TILE;
+    sv[0] = sv[1] = (f32x16){};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const int off = kb ^ (c << 4);
+      const u16x8 k0f = *reinterpret_cast<const u16x8*>(lds_k + off);
+      const u16x8 k1f = *reinterpret_cast<const u16x8*>(lds_k + off + 32 * 128);
+      sv[0] = mfma32(as_bf16x8(k0f), qf[c], sv[0]);
+      sv[1] = mfma32(as_bf16x8(k1f), qf[c], sv[1]);
+    }
+  };
+  // Online softmax, first part: keys outside [klo, khi) of the tile masked, the row maximum, and the running reference
+  // moved (with a rescale) only when a score exceeds it by more than 2^8; returns the reference.
+  auto softmax_max = [&](bool masked, int klo, int khi, f32x16 (&sv)[2]) __attribute__((always_inline)) {
+    if (masked) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int key = ks * 32 + 8 * (x >> 2) + 4 * half + (x & 3);
+          sv[ks][x] = (key >= klo && key < khi) ? sv[ks][x] : -INFINITY;
+        }
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) tmax = fmaxf(tmax, sv[ks][x]);
+    const float tm = half_max(tmax) * scale_log2;
+    if (__builtin_amdgcn_ballot_w64(tm > m_run + 8.f) != 0) {
+      const float m_new = fmaxf(m_run, tm);
+      const float alpha = (m_run == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) oacc[db] *= alpha;
+      m_run = m_new;
+    }
+    return (m_run == -INFINITY) ? 0.f : m_run;
+  };
+
+  // ---- staging: thread (row tid / 8 + i RSTEP, 16 codes tid % 8) of a tile
+  const int r0 = tid >> 3, part = tid & 7;
+  const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh + part * 16;
+  const uint8_t* vc_h = a.vc + (int64_t)kvh * a.vc_sh + part * 16;
+  const float* ks_h = a.ks + kvh;
+  const float* vs_h = a.vs + kvh;
+  const int64_t kc_ss = a.kc_ss, vc_ss = a.vc_ss;
+  const int Hkv = a.Hkv;
+  int bad = 0;
+  // keys past the range repeat its last one (probability 0)
+  auto key_of = [&](int t, int i) __attribute__((always_inline)) { return min(lo + t * TK + r0 + i * RSTEP, hi - 1); };
+  auto page_of = [&](int t, int i) __attribute__((always_inline)) {
+    const int e = trow[key_of(t, i) >> shift];
+    const bool ok = (uint32_t)e < (uint32_t)num_pages;
+    bad |= ok ? 0 : 1;
+    return ok ? e : 0;
+  };
+  auto load = [&](const uint8_t* cache, int64_t ss, const float* scale, int t, int i, int e, u32x4& c, float& sc)
+                  __attribute__((always_inline)) {
+    const int64_t slot = ((int64_t)e << shift) + (key_of(t, i) & pmask);
+    c = *reinterpret_cast<const u32x4*>(cache + slot * ss);
+    sc = scale[(int64_t)e * Hkv];
+  };
+  auto put_k = [&](int j, int i, const u32x4& c, float sc) __attribute__((always_inline)) {
+    u32x4 x, y;
+    widen_k(c, sc, x, y);
+    const int rr = r0 + i * RSTEP;
+    put_row(lds_k + j * TILE, rr, part, k_swz(rr), x, y);
+  };
+  auto put_v = [&](int j, int i, const u32x4& c, float sc) __attribute__((always_inline)) {
+    u32x4 x, y;
+    widen_v(c, x, y);
+    const int rr = r0 + i * RSTEP;
+    put_row(lds_v + j * TILE, rr, part, v_swz(rr), x, y);
+    if (part == 0) lds_vs[j * TK + rr] = __float_as_uint(sc);
+  };
+
+  if (ntiles > 0) {
+    // Tile t of K and of V goes through buffer t % 2. When iteration t starts, K(t + 1) and V(t) are in LDS, K(t + 2) and
+    // V(t + 1) in (or on their way to) registers and S(t) is computed; it writes those two into the buffers that
+    // iteration t - 1 read last, asks for K(t + 3) and V(t + 2), and computes S(t + 1) and O += V(t) P(t).
+    u32x4 kr[NPT], vr[NPT];
+    float ksc[NPT], vsc[NPT];
+    int ev[NPT], ek[NPT];  // pages of tiles t + 2 and t + 3
+    {
+      u32x4 k0[NPT], v0[NPT];
+      float k0s[NPT], v0s[NPT];
+      int e0[NPT], e1[NPT];
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        e0[i] = page_of(0, i);
+        e1[i] = page_of(min(1, last), i);
+        ev[i] = page_of(min(2, last), i);
+        ek[i] = page_of(min(3, last), i);
+      }
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        load(kc_h, kc_ss, ks_h, 0, i, e0[i], k0[i], k0s[i]);
+        load(vc_h, vc_ss, vs_h, 0, i, e0[i], v0[i], v0s[i]);
+        load(kc_h, kc_ss, ks_h, min(1, last), i, e1[i], kr[i], ksc[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        put_k(0, i, k0[i], k0s[i]);
+        put_v(0, i, v0[i], v0s[i]);
+        put_k(1, i, kr[i], ksc[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        load(kc_h, kc_ss, ks_h, min(2, last), i, ev[i], kr[i], ksc[i]);
+        load(vc_h, vc_ss, vs_h, min(1, last), i, e1[i], vr[i], vsc[i]);
+      }
+    }
+    f32x16 s_a[2], s_b[2];
+    lds_barrier();
+    scores(0, s_a);
+    lds_barrier();  // every wave is done with K buffer 0
+
+    // The 32 MFMAs of an iteration as a fixed sequence of slots: s < 8 is S^T subtile 0 of tile t + 1 (d chunk s), 8 .. 15
+    // P V of key chunks 0 and 1 of tile t (d block s % 4), 16 .. 23 S^T subtile 1, 24 .. 31 P V of chunks 2 and 3. LDS
+    // operands are read FD slots ahead, a pair of probabilities is formed in each S^T slot, and a scheduling barrier
+    // closes every slot (left alone, the compiler hoists all reads and spills, or sinks them next to their products).
+    constexpr int FD = 2;
+    auto slot_is_qk = [](int sl) __attribute__((always_inline)) { return sl < 8 || (sl >= 16 && sl < 24); };
+    auto chunk_of = [](int sl) __attribute__((always_inline)) { return sl < 12 ? 0 : sl < 16 ? 1 : sl < 28 ? 2 : 3; };
+    auto fetch = [&](int sl, int kb, int vb) __attribute__((always_inline)) {
+      if (slot_is_qk(sl))
+        return *reinterpret_cast<const u32x4*>(lds_k + ((kb ^ ((sl & 7) << 4)) + (sl >= 16 ? 32 * 128 : 0)));
+      return v_frag((vb ^ ((sl & 3) << 5)) + 2048 * chunk_of(sl));
+    };
+    auto iteration = [&](int t, f32x16 (&s_cur)[2], f32x16 (&s_nxt)[2]) __attribute__((always_inline)) {
+      const int j = t & 1;
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        put_k(j, i, kr[i], ksc[i]);
+        put_v(j ^ 1, i, vr[i], vsc[i]);
+      }
+      if (t + 2 < ntiles) {
+#pragma unroll
+        for (int i = 0; i < NPT; ++i) {
+          load(vc_h, vc_ss, vs_h, t + 2, i, ev[i], vr[i], vsc[i]);
+          load(kc_h, kc_ss, ks_h, min(t + 3, last), i, ek[i], kr[i], ksc[i]);
+          ev[i] = ek[i];
+          ek[i] = page_of(min(t + 4, last), i);
+        }
+      }
+      if (active) {
+        const int khi = hi - (lo + t * TK);
+        const float msub = softmax_max(khi < TK, 0, khi, s_cur);
+        const int kb = k_base + (j ^ 1) * TILE, vb = v_base + j * TILE;
+        u32x4 opnd[32];
+#pragma unroll
+        for (int sl = 0; sl < FD; ++sl) opnd[sl] = fetch(sl, kb, vb);
+        const uint32_t vs_l = lds_vs[j * TK + 16 * (lane & 3)];  // scales of the four 16-key chunks
+        u32x4 pv[4];  // P^T B fragments (fp16 pairs) of the chunks
+        float psum = 0.f;
+        f32x16 acc0 = {}, acc1 = {};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int sl = 0; sl < 32; ++sl) {
+          if (sl == 8 || sl == 12 || sl == 24 || sl == 28) {
+            const uint32_t vsn = __builtin_amdgcn_readlane(vs_l, chunk_of(sl));
+            if (vsn != vcur) {
+              const float f = scale_quotient(vcur, vsn);
+#pragma unroll
+              for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
+              vcur = vsn;
+            }
+          }
+          if (sl + FD < 32) opnd[sl + FD] = fetch(sl + FD, kb, vb);
+          if (slot_is_qk(sl)) {
+            if (sl < 8) acc0 = mfma32(__builtin_bit_cast(bf16x8, opnd[sl]), qf[sl & 7], acc0);
+            else acc1 = mfma32(__builtin_bit_cast(bf16x8, opnd[sl]), qf[sl & 7], acc1);
+            // key pair y of chunk c: S^T registers x, x + 1 of subtile c / 2
+            const int c = (sl < 8 ? 0 : 2) + ((sl & 7) >> 2), y = sl & 3;
+            const int x = (c & 1) * 8 + 2 * y;
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[c >> 1][x], scale_log2, -msub));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[c >> 1][x + 1], scale_log2, -msub));
+            psum += p0 + p1;
+            asm volatile("" : "+v"(psum));  // keeps the add in this slot
+            pv[c][y] = f2h2_bits(p0, p1);
+          } else {
+            const int c = chunk_of(sl), db = sl & 3;
+            oacc[db] = mfma32_f16(__builtin_bit_cast(f16x8, opnd[sl]), __builtin_bit_cast(f16x8, pv[c]), oacc[db]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        l_run += psum;
+        s_nxt[0] = acc0;
+        s_nxt[1] = acc1;
+      }
+      lds_barrier();
+    };
+    for (int t = 0;;) {
+      iteration(t, s_a, s_b);
+      if (++t >= ntiles) break;
+      iteration(t, s_b, s_a);
+      if (++t >= ntiles) break;
+    }
+  }
+  if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+
+  // ---- the request's block keys in bf16: tiles through buffer 0, P split into a bf16 pair hi + lo (2^-17) against V as
+  //      it is. A workgroup whose rows lie in one query head needs only the keys of those rows' modes.
+  if (with_block) {
+    int blo = 0, bhi = KL;
+    const int g0 = ug * NW * UROWS, g1 = min(g0 + NW * UROWS, rows) - 1;  // the workgroup's rows
+    if (g0 / KL == g1 / KL) {
+      blo = (g0 % KL) / Lb * Lb;
+      bhi = ((g1 % KL) / Lb + 1) * Lb;
+    }
+    const float unit = __uint_as_float(vcur);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) oacc[db] *= unit;
+    vcur = 0x3f800000u;
+    for (int b0 = blo; b0 < bhi; b0 += TK) {
+      lds_barrier();  // every wave is done with the buffers
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        const int rr = r0 + i * RSTEP;
+        const int64_t tk = (int64_t)b * KL + min(b0 + rr, bhi - 1);
+        const u32x4* kp = reinterpret_cast<const u32x4*>(a.kn + tk * a.kn_st + (int64_t)kvh * a.kn_sh + part * 16);
+        const u32x4* vp = reinterpret_cast<const u32x4*>(a.vn + tk * a.vn_st + (int64_t)kvh * a.vn_sh + part * 16);
+        const u32x4 kx = kp[0], ky = kp[1], vx = vp[0], vy = vp[1];
+        put_row(lds_k, rr, part, k_swz(rr), kx, ky);
+        put_row(lds_v, rr, part, v_swz(rr), vx, vy);
+      }
+      lds_barrier();
+      const int klo = mode_lo - b0, khi = min(mode_lo + (causal ? qi - mode_lo + 1 : Lb), bhi) - b0;
+      if (active && __builtin_amdgcn_ballot_w64(klo < TK && khi > 0) != 0) {
+        f32x16 sv[2];
+        scores(0, sv);
+        const float msub = softmax_max(true, klo, khi, sv);
+        float psum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          u32x4 ph, pl;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int x = (c & 1) * 8 + 2 * y;
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c >> 1][x], scale_log2, -msub));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c >> 1][x + 1], scale_log2, -msub));
+            psum += p0 + p1;
+            ph[y] = f2bf2_bits(p0, p1);
+            pl[y] = f2bf2_bits(p0 - __uint_as_float(ph[y] << 16), p1 - __uint_as_float(ph[y] & 0xffff0000u));
+          }
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db) {
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, v_frag((v_base ^ (db << 5)) + 2048 * c));
+            oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, ph), oacc[db]);
+            oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, pl), oacc[db]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        l_run += psum;
+      }
+    }
+  }
+  if (!active) return;
+
+  const float l_tot = half_sum(l_run);
+  const float inv = l_tot > 0.f ? __uint_as_float(vcur) / l_tot : (l_tot == 0.f ? 0.f : l_tot);  // (NaN stays NaN)
+  const float lse2 = l_tot > 0.f ? m_run + __log2f(l_tot) : (l_tot == 0.f ? -INFINITY : l_tot);
+  if (a.S == 1) {
+    if (!row_ok) return;
+    uint16_t* op = a.out + token * a.o_st + (int64_t)head * a.o_sh;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const u16x4 vals = {f2bf_bits(oacc[db][gq * 4 + 0] * inv), f2bf_bits(oacc[db][gq * 4 + 1] * inv),
+                            f2bf_bits(oacc[db][gq * 4 + 2] * inv), f2bf_bits(oacc[db][gq * 4 + 3] * inv)};
+        *reinterpret_cast<u16x4*>(op + db * 32 + gq * 8 + half * 4) = vals;
+      }
+    if (a.lse && half == 0) a.lse[token * a.H + head] = lse2 * LN2;
+    return;
+  }
+  // partial row in fp16, scaled by a power of two into (-1, 1): half the bytes of fp32 for the merge to read back
+  float mx = 0.f;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) mx = fmaxf(mx, fabsf(oacc[db][x] * inv));
+  mx = half_max(mx);
+  const int ex = mx > 0.f ? __builtin_amdgcn_frexp_expf(mx) : 0;
+  const float down = __builtin_ldexpf(inv, -ex);
+  if (!row_ok) return;
+  const int64_t prow = partial_row(a, s, b, kvh, r);
+  uint16_t* op = a.ws_o + prow * D;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      u32x2 hv;
+      hv[0] = f2h2_bits(oacc[db][gq * 4 + 0] * down, oacc[db][gq * 4 + 1] * down);
+      hv[1] = f2h2_bits(oacc[db][gq * 4 + 2] * down, oacc[db][gq * 4 + 3] * down);
+      *reinterpret_cast<u32x2*>(op + db * 32 + gq * 8 + half * 4) = hv;
+    }
+  if (half == 0) {
+    a.ws_lse[prow] = lse2;
+    a.ws_exp[prow] = (float)ex;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- stream kernel
+
+__global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attn_stream_kernel(Args a) {
+  constexpr int STILE = SK * D;  // elements of a widened 32-key tile (8 KB)
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[SNW * 2 * STILE];
+  __shared__ float lds_m[SNW][UROWS], lds_l[SNW][UROWS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, l32 = lane & 31;
+  const int KL = a.KL, Lb = a.L, rows = a.rows;
+  const float scale_log2 = a.scale_log2;
+  const int s = blockIdx.x % a.S;
+  const int kvh = (blockIdx.x / a.S) % a.Hkv;
+  const int rho = blockIdx.x / a.S / a.Hkv;
+  const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+  const int32_t* trow = kv8::table_row(a.pages, b);
+  const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
+  const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0);
+  int lo, hi;
+  split_range(a, s, ctx, lo, hi);
+  const bool with_block = a.kn != nullptr && s == 0;
+  if (tid == 0 && s == 0 && kvh == 0 && ctx != a.ctx_lens[b]) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  if (lo >= hi && !with_block && a.S > 1) {  // an empty split
+    if (tid < rows) a.ws_lse[partial_row(a, s, b, kvh, tid)] = -INFINITY;
+    return;
+  }
+  const int r = min(l32, rows - 1);
+  const int qi = r % KL;
+  const int mode_lo = (qi / Lb) * Lb;
+  bf16x8 qf[D / 16];
+  {
+    const uint16_t* qp =
+        a.q + ((int64_t)b * KL + qi) * a.q_st + (int64_t)(kvh * a.G + r / KL) * a.q_sh + half * 8;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) qf[c] = as_bf16x8(*reinterpret_cast<const u16x8*>(qp + c * 16));
+  }
+  uint16_t* const lds_k = lds + w * 2 * STILE;
+  uint16_t* const lds_v = lds_k + STILE;
+  const int k_base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
+  int v_base;
+  {
+    const int grp = lane >> 4, sl = lane & 15, sw = sl >> 2;
+    v_base = (4 * half + sw) * 128 + (sw << 5) + (2 * (grp & 1) + ((sl & 3) >> 1)) * 8 + (sl & 1) * 4;
+  }
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16 oacc[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) oacc[db] = (f32x16){};
+  uint32_t vcur = 0x3f800000u;
+
+  auto scores = [&]() __attribute__((always_inline)) {
+    f32x16 acc = {};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      acc = mfma32(as_bf16x8(*reinterpret_cast<const u16x8*>(lds_k + (k_base ^ (c << 4)))), qf[c], acc);
+    return acc;
+  };
+  auto v_frag = [&](int off) __attribute__((always_inline)) {
+    const v4i16 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off));
+    const v4i16 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off + 1024));
+    const v4i16 v[2] = {x0, x1};
+    return __builtin_bit_cast(u32x4, v);
+  };
+  // register x of a 32-key score tile is key 8 (x / 4) + 4 half + x % 4
+  auto softmax_max = [&](bool masked, int klo, int khi, f32x16& sv) __attribute__((always_inline)) {
+    if (masked) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int key = 8 * (x >> 2) + 4 * half + (x & 3);
+        sv[x] = (key >= klo && key < khi) ? sv[x] : -INFINITY;
+      }
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) tmax = fmaxf(tmax, sv[x]);
+    const float tm = half_max(tmax) * scale_log2;
+    if (__builtin_amdgcn_ballot_w64(tm > m_run + 8.f) != 0) {
+      const float m_new = fmaxf(m_run, tm);
+      const float alpha = (m_run == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) oacc[db] *= alpha;
+      m_run = m_new;
+    }
+    return (m_run == -INFINITY) ? 0.f : m_run;
+  };
+
+  // ---- this wave's tiles: w, w + SNW, ..; a lane holds 16 codes (lane % 8) of rows lane / 8 + 8 i
+  const int r0 = lane >> 3, part = lane & 7;
+  const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh + part * 16;
+  const uint8_t* vc_h = a.vc + (int64_t)kvh * a.vc_sh + part * 16;
+  const int Hkv = a.Hkv;
+  const float* ks_h = a.ks + kvh;
+  const float* vs_h = a.vs + kvh;
+  const int64_t kc_ss = a.kc_ss, vc_ss = a.vc_ss;
+  const int ntiles = (hi - lo + SK - 1) / SK;
+  int bad = 0;
+  auto key_of = [&](int t, int i) __attribute__((always_inline)) { return min(lo + t * SK + r0 + 8 * i, hi - 1); };
+  auto page_of = [&](int t, int i) __attribute__((always_inline)) {
+    const int e = trow[key_of(t, i) >> shift];
+    const bool ok = (uint32_t)e < (uint32_t)num_pages;
+    bad |= ok ? 0 : 1;
+    return ok ? e : 0;
+  };
+  if (w < ntiles) {
+    u32x4 kr[4], vr[4];
+    float ksc[4], vsc[4];
+    int en[4];
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t slot = ((int64_t)en[i] << shift) + (key_of(t, i) & pmask);
+        kr[i] = *reinterpret_cast<const u32x4*>(kc_h + slot * kc_ss);
+        vr[i] = *reinterpret_cast<const u32x4*>(vc_h + slot * vc_ss);
+        ksc[i] = ks_h[(int64_t)en[i] * Hkv];
+        vsc[i] = vs_h[(int64_t)en[i] * Hkv];
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) en[i] = page_of(w, i);
+    load(w);
+    if (w + SNW < ntiles) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) en[i] = page_of(w + SNW, i);
+    }
+    for (int t = w; t < ntiles; t += SNW) {
+      // (a wave's LDS operations complete in order: nothing of the last tile is still to be read)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x4 x, y;
+        const int rr = r0 + 8 * i;
+        widen_k(kr[i], ksc[i], x, y);
+        put_row(lds_k, rr, part, k_swz(rr), x, y);
+        widen_v(vr[i], x, y);
+        put_row(lds_v, rr, part, v_swz(rr), x, y);
+      }
+      const uint32_t vs_t[2] = {(uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(vsc[0])),
+                                (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(vsc[2]))};
+      if (t + SNW < ntiles) {
+        load(t + SNW);
+        if (t + 2 * SNW < ntiles) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) en[i] = page_of(t + 2 * SNW, i);
+        }
+      }
+      asm volatile("" ::: "memory");
+      f32x16 sv = scores();
+      const int khi = hi - (lo + t * SK);
+      const float msub = softmax_max(khi < SK, 0, khi, sv);
+      float psum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        u32x4 pv;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y], scale_log2, -msub));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y + 1], scale_log2, -msub));
+          psum += p0 + p1;
+          pv[y] = f2h2_bits(p0, p1);
+        }
+        if (vs_t[c] != vcur) {
+          const float f = scale_quotient(vcur, vs_t[c]);
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
+          vcur = vs_t[c];
+        }
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+          oacc[db] = mfma32_f16(__builtin_bit_cast(f16x8, v_frag((v_base ^ (db << 5)) + 2048 * c)),
+                                __builtin_bit_cast(f16x8, pv), oacc[db]);
+      }
+      l_run += psum;
+      asm volatile("" ::: "memory");
+    }
+  }
+  if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  // ---- the block keys (rows <= 32, so K L <= 32: one tile), in bf16 with P as a bf16 pair, by the last wave
+  if (with_block && w == SNW - 1) {
+    const float unit = __uint_as_float(vcur);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) oacc[db] *= unit;
+    vcur = 0x3f800000u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = r0 + 8 * i;
+      const int64_t tk = (int64_t)b * KL + min(rr, KL - 1);
+      const u32x4* kp = reinterpret_cast<const u32x4*>(a.kn + tk * a.kn_st + (int64_t)kvh * a.kn_sh + part * 16);
+      const u32x4* vp = reinterpret_cast<const u32x4*>(a.vn + tk * a.vn_st + (int64_t)kvh * a.vn_sh + part * 16);
+      const u32x4 kx = kp[0], ky = kp[1], vx = vp[0], vy = vp[1];
+      put_row(lds_k, rr, part, k_swz(rr), kx, ky);
+      put_row(lds_v, rr, part, v_swz(rr), vx, vy);
+    }
+    asm volatile("" ::: "memory");
+    f32x16 sv = scores();
+    const float msub = softmax_max(true, mode_lo, a.causal ? qi + 1 : mode_lo + Lb, sv);
+    float psum = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      u32x4 ph, pl;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y], scale_log2, -msub));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y + 1], scale_log2, -msub));
+        psum += p0 + p1;
+        ph[y] = f2bf2_bits(p0, p1);
+        pl[y] = f2bf2_bits(p0 - __uint_as_float(ph[y] << 16), p1 - __uint_as_float(ph[y] & 0xffff0000u));
+      }
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, v_frag((v_base ^ (db << 5)) + 2048 * c));
+        oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, ph), oacc[db]);
+        oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, pl), oacc[db]);
+      }
+    }
+    l_run += psum;
+  }
+  // ---- the waves' results: each brings its accumulators to the common reference and into its part of LDS as
+  //      [row][d] fp32 (16 KB); thread (row tid / 8, 16 d's tid % 8) adds them in wave order
+  const float l_w = half_sum(l_run);
+  if (half == 0) {
+    lds_m[w][l32] = m_run;
+    lds_l[w][l32] = l_w;
+  }
+  lds_barrier();
+  float m_tot = lds_m[0][l32];
+#pragma unroll
+  for (int x = 1; x < SNW; ++x) m_tot = fmaxf(m_tot, lds_m[x][l32]);
+  const float fac = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_tot) * __uint_as_float(vcur);
+  float* const own = reinterpret_cast<float*>(lds) + w * (UROWS * D);
+  // 16-byte piece c of row r at c ^ r, so that the lanes of a write or a read spread over the banks
+  if (w < ntiles || (with_block && w == SNW - 1)) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const int c = db * 8 + gq * 2 + half;
+        *reinterpret_cast<f32x4*>(own + l32 * D + ((c ^ l32) & 31) * 4) =
+            (f32x4){oacc[db][gq * 4 + 0] * fac, oacc[db][gq * 4 + 1] * fac, oacc[db][gq * 4 + 2] * fac,
+                    oacc[db][gq * 4 + 3] * fac};
+      }
+  }
+  lds_barrier();
+  const int row = tid >> 3;
+  f32x4 o[4] = {};
+  float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+  for (int x = 0; x < SNW; ++x) mt = fmaxf(mt, lds_m[x][row]);
+#pragma unroll
+  for (int x = 0; x < SNW; ++x) {
+    if (!(x < ntiles || (with_block && x == SNW - 1))) continue;  // a wave without keys
+    const float mw = lds_m[x][row];
+    lt += mw == -INFINITY ? (lds_l[x][row] == 0.f ? 0.f : lds_l[x][row]) : lds_l[x][row] * __builtin_amdgcn_exp2f(mw - mt);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      o[c] += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + x * (UROWS * D) + row * D +
+                                              (((4 * (tid & 7) + c) ^ row) & 31) * 4);
+  }
+  if (row >= rows) return;  // (whole groups of eight threads)
+  const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+  const float lse2 = lt > 0.f ? mt + __log2f(lt) : (lt == 0.f ? -INFINITY : lt);
+  const int d0 = (tid & 7) * 16;
+  if (a.S == 1) {
+    const int64_t token = (int64_t)b * KL + row % KL;
+    const int head = kvh * a.G + row / KL;
+    uint16_t* op = a.out + token * a.o_st + (int64_t)head * a.o_sh + d0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      u16x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = f2bf_bits(o[2 * c + (e >> 2)][e & 3] * inv);
+      *reinterpret_cast<u16x8*>(op + 8 * c) = v;
+    }
+    if (a.lse && (tid & 7) == 0) a.lse[token * a.H + head] = lse2 * LN2;
+    return;
+  }
+  float mx = 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(o[c][e] * inv));
+#pragma unroll
+  for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+  const int ex = mx > 0.f ? __builtin_amdgcn_frexp_expf(mx) : 0;
+  const float down = __builtin_ldexpf(inv, -ex);
+  const int64_t prow = partial_row(a, s, b, kvh, row);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    u32x4 hv;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      hv[e] = f2h2_bits(o[2 * c + (e >> 1)][2 * (e & 1)] * down, o[2 * c + (e >> 1)][2 * (e & 1) + 1] * down);
+    *reinterpret_cast<u32x4*>(a.ws_o + prow * D + d0 + 8 * c) = hv;
+  }
+  if ((tid & 7) == 0) {
+    a.ws_lse[prow] = lse2;
+    a.ws_exp[prow] = (float)ex;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- merge
+
+// 16 threads per row, 8 d's each; the partials in batches of 8, all loads of a batch in flight together, joined with a
+// running log-sum-exp. An empty partial (lse -inf) wrote no row.
+__global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
+  constexpr int SB = 8;
+  const int64_t per = (int64_t)a.bs * a.Hkv * a.rows;
+  const int64_t prow = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (prow >= per) return;
+  const int d0 = (threadIdx.x & 15) * 8;
+  float m = -INFINITY, tot = 0.f;
+  float acc[8] = {};
+  for (int s0 = 0; s0 < a.S; s0 += SB) {
+    float l[SB], ex[SB];
+    u32x4 oh[SB];
+#pragma unroll
+    for (int j = 0; j < SB; ++j) l[j] = s0 + j < a.S ? a.ws_lse[(s0 + j) * per + prow] : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < SB; ++j) {
+      ex[j] = 0.f;
+      oh[j] = (u32x4){};
+      if (l[j] != -INFINITY) {
+        ex[j] = a.ws_exp[(s0 + j) * per + prow];
+        oh[j] = *reinterpret_cast<const u32x4*>(a.ws_o + ((s0 + j) * per + prow) * D + d0);
+      }
+    }
+    float mb = l[0];
+#pragma unroll
+    for (int j = 1; j < SB; ++j) mb = fmaxf(mb, l[j]);
+    const float mn = fmaxf(m, mb);
+    const float sc = m == -INFINITY ? 0.f : exp2f(m - mn);
+    tot *= sc;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= sc;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < SB; ++j) {
+      if (l[j] == -INFINITY) continue;
+      const float wgt = exp2f(l[j] - m);  // NaN stays NaN
+      const float wo = __builtin_ldexpf(wgt, (int)ex[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x2 x = h2_to_f2(oh[j][e]);
+        acc[2 * e] += x[0] * wo;
+        acc[2 * e + 1] += x[1] * wo;
+      }
+      tot += wgt;
+    }
+  }
+  const float inv = tot > 0.f ? 1.f / tot : (tot == 0.f ? 0.f : tot);
+  const int r = (int)(prow % a.rows);
+  const int kvh = (int)(prow / a.rows % a.Hkv);
+  const int64_t b = prow / a.rows / a.Hkv;
+  const int64_t token = b * a.KL + r % a.KL;
+  const int head = kvh * a.G + r / a.KL;
+  u16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = f2bf_bits(acc[e] * inv);
+  *reinterpret_cast<u16x8*>(a.out + token * a.o_st + (int64_t)head * a.o_sh + d0) = v;
+  if (a.lse && d0 == 0) a.lse[token * a.H + head] = tot > 0.f ? (m + log2f(tot)) * LN2 : (tot == 0.f ? -INFINITY : tot);
+}
+
+// ----------------------------------------------------------------------------------------------------- weights
+
+// Attention weight per cached token. A workgroup takes 256 keys of one (request, KV head), 64 a wave: the wave's keys are
+// widened once through LDS into MFMA operands (64 registers) and stay there, while the KV head's query rows stream by in
+// units of 32 through a double buffer in LDS that the waves share. A lane then holds, for its query row, the 32 keys of its
+// half; p = exp2(s scale - lse) is added up per key over the units in registers, and once at the end over the 32 lanes.
+// Every sum has one owner and one order: no atomics. Bound by the exponentials (one per product of 256 flops).
+constexpr int WNW = 4;
+constexpr int WKEYS = WNW * TK;
+
+struct WArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const float* lse;  // [bs K L][H], natural
+  const uint8_t* kc;
+  int64_t kc_ss, kc_sh;
+  const float* ks;
+  Pages pages;
+  const int64_t* ctx_lens;
+  float* w;  // [rows][Hkv][width]
+  int64_t w_sr, w_sh;
+  int w_rows, width;
+  int bs, H, Hkv, G, KL, rows;
+  float scale_log2, decay;
+  int32_t* err_flag;
+};
+
+__global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_weights_kernel(WArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[WNW * TILE];  // keys first, then two Q units of 8 KB
+  __shared__ float lds_lse[2][UROWS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, l32 = lane & 31;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int32_t* trow = kv8::table_row(a.pages, b);
+  const int64_t wrow = a.pages.req_idx ? a.pages.req_idx[b] : b;
+  const int shift = a.pages.page_shift, pmask = (1 << shift) - 1;
+  int ctx = trow && a.pages.num_pages > 0 && wrow < a.w_rows ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0;
+  if (tid == 0 && blockIdx.x == 0 && kvh == 0 && (ctx > a.width || ctx != a.ctx_lens[b]))
+    kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  ctx = __builtin_amdgcn_readfirstlane(min(ctx, a.width));
+  const int lo = blockIdx.x * WKEYS;
+  if (lo >= ctx) return;
+
+  // keys of this wave: 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i
+  {
+    const int r0 = lane >> 3, part = lane & 7;
+    uint16_t* tile = lds + w * TILE;
+    int bad = 0;
+    int e[8];
+    u32x4 c[8];
+    float sc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = min(lo + w * TK + r0 + 8 * i, ctx - 1);
+      e[i] = trow[key >> shift];
+      if ((uint32_t)e[i] >= (uint32_t)a.pages.num_pages) {
+        bad = 1;
+        e[i] = 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = min(lo + w * TK + r0 + 8 * i, ctx - 1);
+      const int64_t slot = ((int64_t)e[i] << shift) + (key & pmask);
+      c[i] = *reinterpret_cast<const u32x4*>(a.kc + slot * a.kc_ss + (int64_t)kvh * a.kc_sh + part * 16);
+      sc[i] = a.ks[(int64_t)e[i] * a.Hkv + kvh];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u32x4 x, y;
+      widen_k(c[i], sc[i], x, y);
+      put_row(tile, r0 + 8 * i, part, k_swz(r0 + 8 * i), x, y);
+    }
+    if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  }
+  asm volatile("" ::: "memory");
+  const int base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
+  bf16x8 kf[2][D / 16];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      kf[ks][c] = as_bf16x8(*reinterpret_cast<const u16x8*>(lds + w * TILE + (base ^ (c << 4)) + ks * 32 * 128));
+  lds_barrier();
+
+  // Q unit u: row tid / 8 of 32, 16 elements tid % 8. A row's lse in base 2; padding rows and rows whose lse is -inf
+  // (they saw no key) get +inf: their probabilities are 0.
+  const int units = (a.rows + UROWS - 1) / UROWS;
+  const int qr = tid >> 3, qpart = tid & 7;
+  u32x4 qx, qy;
+  float ql = 0.f;
+  auto load_q = [&](int u) __attribute__((always_inline)) {
+    const int rr = u * UROWS + qr;
+    const int r = min(rr, a.rows - 1);
+    const int head = kvh * a.G + r / a.KL;
+    const int64_t token = (int64_t)b * a.KL + r % a.KL;
+    const u32x4* qp = reinterpret_cast<const u32x4*>(a.q + token * a.q_st + (int64_t)head * a.q_sh + qpart * 16);
+    qx = qp[0];
+    qy = qp[1];
+    const float l = a.lse[token * a.H + head];
+    ql = rr < a.rows && l != -INFINITY ? l * 1.4426950408889634f : INFINITY;
+  };
+  auto put_q = [&](int j) __attribute__((always_inline)) {
+    put_row(lds + j * (UROWS * D), qr, qpart, k_swz(qr), qx, qy);
+    if (qpart == 0) lds_lse[j][qr] = ql;
+  };
+  float acc[32];
+#pragma unroll
+  for (int x = 0; x < 32; ++x) acc[x] = 0.f;
+  load_q(0);
+  put_q(0);
+  if (units > 1) load_q(1);
+  lds_barrier();
+  for (int u = 0; u < units; ++u) {
+    const int j = u & 1;
+    if (u + 1 < units) {  // buffer j ^ 1 was last read in iteration u - 1
+      put_q(j ^ 1);
+      if (u + 2 < units) load_q(u + 2);
+    }
+    const uint16_t* qb = lds + j * (UROWS * D);
+    f32x16 s0 = {}, s1 = {};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const bf16x8 qf = as_bf16x8(*reinterpret_cast<const u16x8*>(qb + (base ^ (c << 4))));
+      s0 = mfma32(kf[0][c], qf, s0);
+      s1 = mfma32(kf[1][c], qf, s1);
+    }
+    const float l = lds_lse[j][l32];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      acc[x] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[x], a.scale_log2, -l));
+      acc[16 + x] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[x], a.scale_log2, -l));
+    }
+    lds_barrier();
+  }
+  // Sum over the 32 lanes of a half, halving the registers as the lanes are joined: in step m a lane keeps the half of its
+  // registers that its bit m names and gives the other half to lane ^ m. Register x ends in the lane whose bits 4 .. 0
+  // (m = 16, 8, 4, 2, 1) spell x.
+#pragma unroll
+  for (int n = 16; n >= 1; n >>= 1) {
+    const bool up = (l32 & n) != 0;
+#pragma unroll
+    for (int x = 0; x < n; ++x) {
+      const float give = up ? acc[x] : acc[x + n], keep = up ? acc[x + n] : acc[x];
+      acc[x] = keep + __shfl_xor(give, n);
+    }
+  }
+  const int x = l32 & 15, key = lo + w * TK + (l32 >> 4) * 32 + 8 * (x >> 2) + 4 * half + (x & 3);
+  if (key < ctx) {
+    float* p = a.w + wrow * a.w_sr + (int64_t)kvh * a.w_sh + key;
+    *p = a.decay != 0.f ? a.decay * *p + acc[0] : acc[0];  // (a decay of 0 does not read the old sum)
+  }
+}
+
+}  // namespace
+
+static int64_t partials(int with_block, int num_ctx_splits, int rows) {
+  if (num_ctx_splits <= 1) return 1;
+  return num_ctx_splits + (with_block && rows > UROWS ? 1 : 0);
+}
+
+extern "C" int64_t mfd_kv8_attn_workspace_bytes(int bs, int num_modes, int block_size, int H, int Hkv, int with_block,
+                                                int num_ctx_splits) {
+  if (num_ctx_splits <= 1 || bs < 1 || num_modes < 1 || block_size < 1 || H < 1 || Hkv < 1) return 0;
+  const int64_t rows = (int64_t)bs * H * num_modes * block_size;
+  return partials(with_block, num_ctx_splits, (int)(H / Hkv * (int64_t)num_modes * block_size)) * rows * (D * 2 + 4 + 4);
+}
+
+static int check_attn(const char* who, int bs, int num_modes, int block_size, int H, int Hkv, float scale,
+                      const void* q, int64_t q_st, int64_t q_sh) {
+  if (bs < 0 || bs > 65535 || num_modes < 1 || block_size < 1 || H < 1 || Hkv < 1 || H % Hkv != 0)
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: bad sizes bs=%d K=%d L=%d H=%d Hkv=%d", who, bs, num_modes, block_size,
+                         H, Hkv);
+  if ((int64_t)num_modes * block_size > (1 << 16) || (int64_t)H / Hkv * num_modes * block_size > (1 << 24))
+    return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: num_modes * block_size = %lld above 65536 (or 2^24 rows per KV head)",
+                         who, (long long)num_modes * block_size);
+  if (!(scale > 0.f)) return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: scale must be positive", who);
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || ((q_st | q_sh) & 7))
+    return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: q needs 16-byte aligned rows", who);
+  return MFD_OK;
+}
+
+extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* k_new, const uint16_t* v_new,
+                            int64_t kn_st, int64_t kn_sh, int64_t vn_st, int64_t vn_sh, const uint8_t* k_cache,
+                            const uint8_t* v_cache, int64_t kc_ss, int64_t kc_sh, int64_t vc_ss, int64_t vc_sh,
+                            const float* k_scale, const float* v_scale, int num_pages, const int32_t* page_table,
+                            int64_t table_stride, int table_rows, int table_width, int page_size,
+                            const int64_t* req_idx, const int64_t* ctx_lens, int bs, int num_modes, int block_size,
+                            int H, int Hkv, int D_, float scale, int causal_in_block, int num_ctx_splits,
+                            int split_keys, uint16_t* out, int64_t o_st, int64_t o_sh, float* lse, void* workspace,
+                            int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+  const char* who = "mfd_kv8_attn";
+  int rc = kv8::check_cache(who, k_cache, v_cache, kc_ss, kc_sh, vc_ss, vc_sh, page_size, Hkv, D_, page_table, table_rows,
+                            table_width, num_pages);
+  if (rc == MFD_OK) rc = check_attn(who, bs, num_modes, block_size, H, Hkv, scale, q, q_st, q_sh);
+  if (rc != MFD_OK) return rc;
+  if (num_ctx_splits < 1 || num_ctx_splits > 1024 ||
+      (num_ctx_splits > 1 && (split_keys < TK || split_keys % TK != 0)))
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: num_ctx_splits %d (1..1024) of split_keys %d (a multiple of %d)", who,
+                         num_ctx_splits, split_keys, TK);
+  if (bs == 0) return MFD_OK;
+  if (!q || !out || !ctx_lens || (!k_new) != (!v_new) ||
+      (num_pages > 0 && table_rows > 0 && table_width > 0 && (!k_cache || !v_cache || !k_scale || !v_scale)))
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: null tensor pointer", who);
+  if (((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new) | reinterpret_cast<uintptr_t>(out)) & 15) ||
+      ((kn_st | kn_sh | vn_st | vn_sh | o_st | o_sh) & 7))
+    return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: tensors need 16-byte aligned rows (strides in multiples of 8)", who);
+  const int64_t need = mfd_kv8_attn_workspace_bytes(bs, num_modes, block_size, H, Hkv, k_new != nullptr, num_ctx_splits);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: 16-byte aligned workspace of %lld bytes needed", who, (long long)need);
+  Args a{};
+  a.q = q; a.q_st = q_st; a.q_sh = q_sh;
+  a.kn = k_new; a.vn = v_new; a.kn_st = kn_st; a.kn_sh = kn_sh; a.vn_st = vn_st; a.vn_sh = vn_sh;
+  a.kc = k_cache; a.vc = v_cache; a.kc_ss = kc_ss; a.kc_sh = kc_sh; a.vc_ss = vc_ss; a.vc_sh = vc_sh;
+  a.ks = k_scale; a.vs = v_scale;
+  a.pages = {page_table, table_stride, table_rows, table_width, req_idx, num_pages, __builtin_ctz((unsigned)page_size)};
+  a.ctx_lens = ctx_lens;
+  a.out = out; a.o_st = o_st; a.o_sh = o_sh; a.lse = lse;
+  a.bs = bs; a.K = num_modes; a.L = block_size; a.H = H; a.Hkv = Hkv; a.G = H / Hkv;
+  a.KL = num_modes * block_size;
+  a.rows = a.G * a.KL;
+  a.SC = num_ctx_splits; a.split_keys = split_keys;
+  a.S = (int)partials(k_new != nullptr, num_ctx_splits, a.rows);
+  a.causal = causal_in_block ? 1 : 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.err_flag = err_flag;
+  const int64_t prows = (int64_t)bs * H * a.KL;
+  a.ws_o = static_cast<uint16_t*>(workspace);
+  a.ws_lse = workspace ? reinterpret_cast<float*>(a.ws_o + a.S * prows * D) : nullptr;
+  a.ws_exp = workspace ? a.ws_lse + a.S * prows : nullptr;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t programs = (int64_t)bs * Hkv * a.S;
+  const int units = (a.rows + UROWS - 1) / UROWS;
+  const int NW = units % 8 == 0 ? 8 : 4;
+  a.ngroups = (units + NW - 1) / NW;
+  const int64_t grid = units == 1 ? programs : (programs + 7) / 8 * 8 * a.ngroups;
+  if (grid > 0x7fffffff || (prows + 15) / 16 > 0x7fffffff)
+    return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
+  if (units == 1)
+    hipLaunchKernelGGL(kv8_attn_stream_kernel, dim3((unsigned)grid), dim3(SNW * 64), 0, st, a);
+  else if (NW == 8)
+    hipLaunchKernelGGL(kv8_attn_tile_kernel<8>, dim3((unsigned)grid), dim3(512), 0, st, a);
+  else
+    hipLaunchKernelGGL(kv8_attn_tile_kernel<4>, dim3((unsigned)grid), dim3(256), 0, st, a);
+  MFD_CHECK_LAUNCH();
+  if (a.S > 1) {
+    hipLaunchKernelGGL(kv8_attn_merge_kernel, dim3((unsigned)((prows + 15) / 16)), dim3(256), 0, st, a);
+    MFD_CHECK_LAUNCH();
+  }
+  return MFD_OK;
+}
+
+extern "C" int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, const float* lse, const uint8_t* k_cache,
+                               int64_t kc_ss, int64_t kc_sh, const float* k_scale, int num_pages,
+                               const int32_t* page_table, int64_t table_stride, int table_rows, int table_width,
+                               int page_size, const int64_t* req_idx, const int64_t* ctx_lens, int bs, int num_modes,
+                               int block_size, int H, int Hkv, int D_, float scale, float decay, float* weights,
+                               int64_t w_row_stride, int64_t w_head_stride, int w_rows, int width, int32_t* err_flag,
+                               void* stream) {
+  const char* who = "mfd_kv8_weights";
+  int rc = kv8::check_cache(who, k_cache, k_cache, kc_ss, kc_sh, 0, 0, page_size, Hkv, D_, page_table, table_rows,
+                            table_width, num_pages);
+  if (rc == MFD_OK) rc = check_attn(who, bs, num_modes, block_size, H, Hkv, scale, q, q_st, q_sh);
+  if (rc != MFD_OK) return rc;
+  if (w_rows < 0 || width < 0 || !(decay >= 0.f && decay <= 1.f))
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: bad weights rows=%d width=%d, or decay %g outside [0, 1]", who, w_rows,
+                         width, (double)decay);
+  if (bs == 0 || width == 0 || num_pages == 0 || table_width == 0 || table_rows == 0) return MFD_OK;
+  if (!q || !lse || !k_cache || !k_scale || !weights || !ctx_lens)
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: null tensor pointer", who);
+  WArgs a{};
+  a.q = q; a.q_st = q_st; a.q_sh = q_sh; a.lse = lse;
+  a.kc = k_cache; a.kc_ss = kc_ss; a.kc_sh = kc_sh; a.ks = k_scale;
+  a.pages = {page_table, table_stride, table_rows, table_width, req_idx, num_pages, __builtin_ctz((unsigned)page_size)};
+  a.ctx_lens = ctx_lens;
+  a.w = weights; a.w_sr = w_row_stride; a.w_sh = w_head_stride; a.w_rows = w_rows; a.width = width;
+  a.bs = bs; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.KL = num_modes * block_size; a.rows = a.G * a.KL;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.decay = decay;
+  a.err_flag = err_flag;
+  const int64_t keys = std::min<int64_t>(width, (int64_t)table_width * page_size);
+  const dim3 grid((unsigned)((keys + WKEYS - 1) / WKEYS), (unsigned)Hkv, (unsigned)bs);
+  hipLaunchKernelGGL(kv8_weights_kernel, grid, dim3(WNW * 64), 0, static_cast<hipStream_t>(stream), a);
+  MFD_CHECK_LAUNCH();
+  return MFD_OK;
+}

@@ -40,6 +40,13 @@ _lib.mfd_tree_ctx_bytes.argtypes = [_I, _I]
 _lib.mfd_tree_gdn_workspace_bytes.restype = _I64
 _lib.mfd_tree_gdn_workspace_bytes.argtypes = [_I, _I, _I, _I, _I]
 
+_lib.mfd_kv8_attn_workspace_bytes.restype = _I64
+_lib.mfd_kv8_attn_workspace_bytes.argtypes = [_I, _I, _I, _I, _I, _I, _I]
+_lib.mfd_evict_select_workspace_bytes.restype = _I64
+_lib.mfd_evict_select_workspace_bytes.argtypes = [_I, _I]
+
+DEVERR_BAD_PAGE = 64  # MFD_DEVERR_BAD_PAGE
+
 _SIGNATURES = {
     # name: argtypes (all return int status)
     "mfd_tree_gdn": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I64, _P],
@@ -72,6 +79,30 @@ _SIGNATURES = {
     "mfd_draft_prepare": [_P, _P, _P, _P, _I64, _I, _I64, _P, _P, _P, _I, _I, _I, _P],
     "mfd_mode_mask": [_P, _P, _P, _I, _I, _I, _P],
     "mfd_tree_prep": [_P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P],
+    "mfd_kv8_store": [_P, _P, _I64, _I64, _I64, _I64,       # k, v, strides
+                      _P, _P, _I64, _I64, _I64, _I64,      # k_cache, v_cache, strides
+                      _P, _P, _I,                          # k_scale, v_scale, pages
+                      _P, _I64, _I, _I, _I,                # page table, row stride, rows, width, page size
+                      _P, _P, _P, _I, _I, _I, _I, _I,      # req_idx, start_lens, cu_tokens, N, bs, max_tokens, Hkv, D
+                      _P, _P],                             # err_flag, stream
+    "mfd_kv8_attn": [_P, _I64, _I64,                       # q, token / head strides
+                     _P, _P, _I64, _I64, _I64, _I64,       # k_new, v_new, strides
+                     _P, _P, _I64, _I64, _I64, _I64,       # k_cache, v_cache, strides
+                     _P, _P, _I,                           # k_scale, v_scale, pages
+                     _P, _I64, _I, _I, _I,                 # page table, row stride, rows, width, page size
+                     _P, _P, _I, _I, _I, _I, _I, _I,       # req_idx, ctx_lens, bs, K, L, H, Hkv, D
+                     _F, _I, _I, _I,                       # scale, causal, splits, split_keys
+                     _P, _I64, _I64, _P, _P, _I64, _P, _P],  # out, strides, lse, workspace, bytes, err_flag, stream
+    "mfd_kv8_weights": [_P, _I64, _I64, _P,                # q, strides, lse
+                        _P, _I64, _I64, _P, _I,            # k_cache, strides, k_scale, pages
+                        _P, _I64, _I, _I, _I,              # page table, row stride, rows, width, page size
+                        _P, _P, _I, _I, _I, _I, _I, _I, _F, _F,  # req_idx, ctx_lens, bs, K, L, H, Hkv, D, scale, decay
+                        _P, _I64, _I64, _I, _I, _P, _P],   # weights, strides, rows, width, err_flag, stream
+    "mfd_evict_select": [_P, _I64, _I64, _I, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I64, _P, _P],
+    "mfd_evict_compact_kv8": [_P, _I, _P, _P,              # keep, budget, new_lens, ctx_lens
+                              _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I,  # caches, strides, scales, pages
+                              _P, _I64, _I, _I, _P, _I64, _I, _I, _I,      # source and destination tables, page size
+                              _P, _P, _I64, _I64, _I, _I, _I, _I, _I, _P, _P],  # req_idx, weights .., bs, Hkv, D, ..
     "mfd_gdn_commit": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, _I, _I, _I, _P, _I64, _P, _I64,
                        _I64, _P, _I, _I, _P, _P],
 }
@@ -126,6 +157,11 @@ def stream_of(t: torch.Tensor) -> int:
     return _raw_stream(index)
 
 
+def current_stream(index: int) -> int:
+    """The current stream's handle of GPU ``index``."""
+    return _raw_stream(index)
+
+
 def as_dtype(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """``t.to(dtype)``, not called (0.5 us) where nothing changes: a layer makes a handful of these checks."""
     return t if t.dtype == dtype else t.to(dtype)
@@ -140,7 +176,8 @@ def require_cuda(*tensors) -> None:
 def exported_symbols() -> list[str]:
     return ["mfd_last_error", "mfd_version", "mfd_mode_attn_workspace_bytes", "mfd_topk_logz_workspace_bytes",
             "mfd_build_mixture_smem_bytes", "mfd_build_single_smem_bytes", "mfd_tree_ctx_bytes",
-            "mfd_tree_gdn_workspace_bytes", *_SIGNATURES]
+            "mfd_tree_gdn_workspace_bytes", "mfd_kv8_attn_workspace_bytes", "mfd_evict_select_workspace_bytes",
+            *_SIGNATURES]
 
 
 _CU_COUNT = {}
