@@ -471,6 +471,21 @@ int mfd_evict_compact_kv8(const int32_t* keep, int budget, const int64_t* new_le
                           int64_t w_row_stride, int64_t w_head_stride, int w_rows, int width, int bs, int Hkv, int D,
                           int32_t* err_flag, void* stream);
 
+/* ---------------------------------------------------------------- draft head with a 4-bit weight
+ * mfd_draft_head_gemm / mfd_draft_topk_head with the weight in the OCP microscaling format MXFP4:
+ *   W[n][k] = e2m1(half k % 2 (low first) of codes[n][k / 2]) * 2^(exps[n][k / 32] - 127)
+ *   codes [N][K / 2] uint8, 16-byte aligned;  exps [N][K / 32] uint8, 4-byte aligned, values 1 .. 252;  K % 128 == 0
+ * The other arguments are as there (drafted row m at x + (m / rows_per_group) * group_stride + (m % rows_per_group) *
+ * row_stride; out_stride a multiple of 4). Products are exact, sums fp32, logits rounded once to bf16. */
+int mfd_draft_head_mxfp4(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t group_stride,
+                         const uint8_t* codes, const uint8_t* exps, int M, int N, int K, uint16_t* out,
+                         int64_t out_stride, void* stream);
+int mfd_draft_topk_head_mxfp4(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t group_stride,
+                              const uint8_t* codes, const uint8_t* exps, int M, int N, int K, uint16_t* logits,
+                              int64_t logits_stride, int k, float* out_logp, void* out_ids, int ids_int64,
+                              float* out_logz, const int32_t* vocab_ids, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

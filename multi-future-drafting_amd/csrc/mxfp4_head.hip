@@ -1,0 +1,351 @@
+// Draft LM head with a 4-bit weight for gfx950: logits = bf16(x W^T) over the drafted rows,
+//   W[n][k] = e2m1(codes[n][k / 2], half k % 2) * 2^(exps[n][k / 32] - 127),
+// the weight as in the OCP microscaling format MXFP4 (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; an e8m0 scale for 32
+// weights), row-major, low half of a byte first. An e2m1 value has two significant bits and the scale is a power of two, so
+// W is exact in bf16 and gfx950 makes it there in one instruction for two weights, scale included: products are exact in
+// fp32, sums are fp32 (v_mfma_f32_16x16x32_bf16), and the only rounding is the logit's own.
+//
+// The weight (4.25 bits each: 207 MB at 151936 x 2560) streams once per 128 drafted rows, straight to registers: a lane takes
+// 16 bytes, 32 weights of one row under one scale, and the four lane groups of a 16-row tile take 128 k together. Which k a
+// lane holds is free as long as both operands agree, so the four MFMAs of such a step use k = 32 (lane / 16) + 8 j + 0 .. 7.
+//  * Wide form: a workgroup of eight waves takes an even share of the vocabulary, a wave up to VT 16-row tiles of it
+//    against all of the launch's drafted rows (MTL 16-row tiles), which come through LDS in blocks of 2048 / MTL k by
+//    direct loads, double buffered, one barrier per block. Bound by the weight's way from memory with few drafted rows, by
+//    the matrix pipes with 128.
+//  * K-split form, for vocabularies that leave a wave of the wide form without a tile: a workgroup takes VT tiles, each of
+//    its four waves every fourth step of k; the drafted rows come from L2 straight to registers, the partial sums meet in
+//    LDS and are added in wave order.
+#include <algorithm>
+
+#include "mfd_common.h"
+
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int MT = 128;   // drafted rows of one launch
+constexpr int KS = 128;   // k per step
+constexpr int NW = 8;     // waves of the wide form
+constexpr int VT_MAX = 5;
+constexpr int BLOCK = 64 * 1024;  // bytes of a drafted-row block in LDS
+constexpr int KNW = 4;    // waves of the k-split form
+
+struct HeadArgs {
+  const uint16_t* x;  // drafted row m at x + (m / rpg) * group_stride + (m % rpg) * row_stride
+  int64_t row_stride, group_stride;
+  int rpg, row0;      // the launch's drafted rows are row0 .. row0 + M - 1
+  const uint8_t* codes;  // [N][K / 2]
+  const uint8_t* exps;   // [N][K / 32]
+  uint16_t* out;      // [M][out_stride], row 0 = drafted row row0
+  int64_t out_stride;
+  int M, N, K, nwg;
+};
+
+// One direct-to-LDS load: lane l's 16 bytes at g land at LDS byte address lds_byte + 16 l (lds_byte wave-uniform). Inline asm:
+// the compiler does not count it among its own loads; the kernel waits for it explicitly.
+__device__ __forceinline__ void dma16(const void* g, uint32_t lds_byte) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane(lds_byte);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(g) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ const uint16_t* drafted_row(const HeadArgs& a, int r) {
+  const int m = a.row0 + min(r, a.M - 1);  // rows past the last repeat it and are not stored
+  return a.x + (int64_t)(m / a.rpg) * a.group_stride + (int64_t)(m % a.rpg) * a.row_stride;
+}
+// First vocabulary row of workgroup g: an even split, in multiples of 8 rows
+__host__ __device__ __forceinline__ int wg_row0(int g, int N, int nwg) {
+  return g >= nwg ? N : (int)(((int64_t)g * N / nwg) & ~(int64_t)7);
+}
+
+// Eight codes times the scale as bf16: exact
+__device__ __forceinline__ bf16x8 widen(uint32_t c, float s) {
+  const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3)};
+  return __builtin_bit_cast(bf16x8, v);
+}
+// The scale of lane group g4 among a step's four
+__device__ __forceinline__ float scale_of(uint32_t e4, int g4) { return __uint_as_float(((e4 >> (8 * g4)) & 0xffu) << 23); }
+
+// C registers of a tile pair to bf16 and out: weight rows n .. n + 3 of the range, the drafted row's output at orow
+__device__ __forceinline__ void store4(uint16_t* orow, int n, int rows, const f32x4& c) {
+  const u32x2 pk = {__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){c[0], c[1]}, bf16x2)),
+                    __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){c[2], c[3]}, bf16x2))};
+  if (n + 4 <= rows) {
+    *reinterpret_cast<u32x2*>(orow + n) = pk;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < rows) orow[n + e] = (uint16_t)(pk[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+template <int VT, int MTL>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void mxfp4_wide_kernel(HeadArgs a) {
+  constexpr int HB = 2048 / MTL;        // k per drafted block
+  constexpr int CPR = HB / 8;           // 16-byte chunks of a row's block
+  constexpr int SPB = HB / KS;          // steps per block
+  constexpr int LPW = BLOCK / 1024 / NW;  // direct loads of a wave per block
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R0 = wg_row0(blockIdx.x, a.N, a.nwg);
+  const int rows = wg_row0(blockIdx.x + 1, a.N, a.nwg) - R0;
+  if (rows <= 0) return;
+  const int K = a.K, S = K / KS;
+  const int l16 = lane & 15, g4 = lane >> 4;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+
+  // chunk c of drafted row r sits at c ^ (r & 15) of the row's block, so that the 16 rows of an operand read hit all
+  // banks; chunks past the last k repeat the last one and are never read
+  auto issue_x = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int at = (i * NW + w) * 64 + lane;
+      const int r = at / CPR, c = (at % CPR) ^ (r & 15);
+      dma16(drafted_row(a, r) + min(b * HB + 8 * c, K - 8), lds0 + (uint32_t)(b & 1) * BLOCK + (uint32_t)(i * NW + w) * 1024u);
+    }
+  };
+  // this wave's tiles t0 .. t0 + vtv - 1; past them it loads (but does not multiply) the last one again
+  const int T = (rows + 15) / 16;
+  const int t0 = __builtin_amdgcn_readfirstlane(w * T / NW);
+  const int vtv = __builtin_amdgcn_readfirstlane((w + 1) * T / NW) - t0;
+  const uint8_t* cp[VT];
+  const uint8_t* ep[VT];
+#pragma unroll
+  for (int i = 0; i < VT; ++i) {
+    const int64_t row = R0 + min(16 * (t0 + min(i, max(vtv - 1, 0))) + l16, rows - 1);
+    cp[i] = a.codes + row * (K / 2) + 16 * g4;
+    ep[i] = a.exps + row * (K / 32);
+  }
+  f32x4 acc[VT][MTL];
+#pragma unroll
+  for (int i = 0; i < VT; ++i)
+#pragma unroll
+    for (int j = 0; j < MTL; ++j) acc[i][j] = (f32x4){};
+  u32x4 wf[2][VT];
+  uint32_t ef[2][VT];
+  auto load_w = [&](int p, int v) __attribute__((always_inline)) {
+    const int u = min(v, S - 1);
+#pragma unroll
+    for (int i = 0; i < VT; ++i) {
+      wf[p][i] = *reinterpret_cast<const u32x4*>(cp[i] + 64 * u);
+      ef[p][i] = *reinterpret_cast<const uint32_t*>(ep[i] + 4 * u);
+    }
+  };
+  auto step = [&](int p, int v) __attribute__((always_inline)) {
+    const uint8_t* base = smem + ((v / SPB) & 1) * BLOCK + l16 * (HB * 2);
+    const int c0 = (v % SPB) * (KS / 8) + 4 * g4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 xf[MTL];
+#pragma unroll
+      for (int m = 0; m < MTL; ++m)
+        xf[m] = *reinterpret_cast<const bf16x8*>(base + 16 * m * (HB * 2) + (((c0 + j) ^ l16) << 4));
+#pragma unroll
+      for (int i = 0; i < VT; ++i) {
+        if (i >= vtv) break;
+        const bf16x8 f = widen(wf[p][i][j], scale_of(ef[p][i], g4));
+#pragma unroll
+        for (int m = 0; m < MTL; ++m) acc[i][m] = mfma16(f, xf[m], acc[i][m]);
+      }
+    }
+  };
+  issue_x(0);
+  load_w(0, 0);
+  load_w(1, 1);
+  for (int b = 0; b * SPB < S; ++b) {
+    // the block's direct loads have landed: the 4 VT weight loads of two steps are younger
+    wait_vmcnt<4 * VT>();
+    __syncthreads();  // in every wave; and block b - 1 is read, so its half is free
+    if ((b + 1) * SPB < S) issue_x(b + 1);
+    const int end = min((b + 1) * SPB, S);
+#pragma unroll 1
+    for (int v = b * SPB; v < end; v += 2) {
+      step(0, v);
+      load_w(0, v + 2);
+      if (v + 1 < end) step(1, v + 1);
+      load_w(1, v + 3);
+    }
+  }
+  wait_vmcnt<0>();
+  // C register r of accumulator (i, m): weight row 16 (t0 + i) + 4 g4 + r of the range, drafted row 16 m + l16
+#pragma unroll
+  for (int m = 0; m < MTL; ++m) {
+    const int mm = 16 * m + l16;
+    if (mm >= a.M) continue;
+    uint16_t* orow = a.out + (int64_t)mm * a.out_stride + R0;
+#pragma unroll
+    for (int i = 0; i < VT; ++i)
+      if (i < vtv) store4(orow, 16 * (t0 + i) + 4 * g4, rows, acc[i][m]);
+  }
+}
+
+template <int VT, int MTL>
+__global__ __launch_bounds__(KNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void mxfp4_ksplit_kernel(HeadArgs a) {
+  constexpr int TT = VT * MTL;
+  __shared__ f32x4 part[KNW * TT * 64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R0 = blockIdx.x * (16 * VT);
+  const int rows = min(16 * VT, a.N - R0);
+  const int K = a.K, S = K / KS;
+  const int l16 = lane & 15, g4 = lane >> 4;
+  const uint8_t* cp[VT];
+  const uint8_t* ep[VT];
+#pragma unroll
+  for (int i = 0; i < VT; ++i) {
+    const int64_t row = R0 + min(16 * i + l16, rows - 1);
+    cp[i] = a.codes + row * (K / 2) + 16 * g4;
+    ep[i] = a.exps + row * (K / 32);
+  }
+  const uint16_t* xp[MTL];
+#pragma unroll
+  for (int m = 0; m < MTL; ++m) xp[m] = drafted_row(a, 16 * m + l16) + 32 * g4;
+  f32x4 acc[VT][MTL];
+#pragma unroll
+  for (int i = 0; i < VT; ++i)
+#pragma unroll
+    for (int m = 0; m < MTL; ++m) acc[i][m] = (f32x4){};
+  // few drafted rows: two steps' operands in registers, else one
+  constexpr int NB = MTL <= 2 ? 2 : 1;
+  u32x4 wf[NB][VT];
+  uint32_t ef[NB][VT];
+  bf16x8 xf[NB][MTL][4];
+  auto load = [&](int s, int v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < VT; ++i) {
+      wf[s][i] = *reinterpret_cast<const u32x4*>(cp[i] + 64 * v);
+      ef[s][i] = *reinterpret_cast<const uint32_t*>(ep[i] + 4 * v);
+    }
+#pragma unroll
+    for (int m = 0; m < MTL; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xf[s][m][j] = *reinterpret_cast<const bf16x8*>(xp[m] + KS * v + 8 * j);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto products = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < VT; ++i) {
+      const float sc = scale_of(ef[s][i], g4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bf16x8 f = widen(wf[s][i][j], sc);
+#pragma unroll
+        for (int m = 0; m < MTL; ++m) acc[i][m] = mfma16(f, xf[s][m][j], acc[i][m]);
+      }
+    }
+  };
+  if constexpr (NB == 2) {
+    if (w < S) load(0, w);
+    for (int v = w; v < S; v += 2 * KNW) {
+      if (v + KNW < S) load(1, v + KNW);
+      products(0);
+      if (v + KNW < S) {
+        if (v + 2 * KNW < S) load(0, v + 2 * KNW);
+        products(1);
+      }
+    }
+  } else {
+    for (int v = w; v < S; v += KNW) {
+      load(0, v);
+      products(0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VT; ++i)
+#pragma unroll
+    for (int m = 0; m < MTL; ++m) part[(w * TT + i * MTL + m) * 64 + lane] = acc[i][m];
+  __syncthreads();
+  for (int t = w; t < TT; t += KNW) {
+    const int i = t / MTL, m = 16 * (t % MTL) + l16;
+    f32x4 c = part[t * 64 + lane];
+#pragma unroll
+    for (int x = 1; x < KNW; ++x) {
+      const f32x4 d = part[(x * TT + t) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] += d[e];
+    }
+    if (m < a.M) store4(a.out + (int64_t)m * a.out_stride + R0, 16 * i + 4 * g4, rows, c);
+  }
+}
+
+template <int VT, int MTL>
+int launch_wide(const HeadArgs& a, hipStream_t st) {
+  const int rc = mfd_set_max_lds(reinterpret_cast<const void*>(&mxfp4_wide_kernel<VT, MTL>), 2 * BLOCK);
+  if (rc != MFD_OK) return rc;
+  hipLaunchKernelGGL((mxfp4_wide_kernel<VT, MTL>), dim3((unsigned)a.nwg), dim3(NW * 64), 2 * BLOCK, st, a);
+  return MFD_OK;
+}
+template <int MTL>
+int launch_rows(const HeadArgs& a, int cus, hipStream_t st) {
+  if ((int64_t)a.N <= (int64_t)NW * 16 * cus / 2) {
+    hipLaunchKernelGGL((mxfp4_ksplit_kernel<1, MTL>), dim3((unsigned)((a.N + 15) / 16)), dim3(KNW * 64), 0, st, a);
+    return MFD_OK;
+  }
+  const int vt = (a.N / a.nwg + 8 + 16 * NW - 1) / (16 * NW);  // tiles of a wave
+  switch (vt) {
+    case 1: return launch_wide<1, MTL>(a, st);
+    case 2: return launch_wide<2, MTL>(a, st);
+    case 3: return launch_wide<3, MTL>(a, st);
+    case 4: return launch_wide<4, MTL>(a, st);
+    default: return launch_wide<5, MTL>(a, st);
+  }
+}
+
+int head_gemm(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t group_stride, const uint8_t* codes,
+              const uint8_t* exps, int M, int N, int K, uint16_t* out, int64_t out_stride, void* stream, const char* who) {
+  if (M < 0 || N < 1 || K < 1 || rows_per_group < 1 || row_stride < 0 || group_stride < 0)
+    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: bad sizes M=%d N=%d K=%d rows_per_group=%d", who, M, N, K, rows_per_group);
+  if (K % KS != 0) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: needs K %% %d == 0 (K=%d)", who, KS, K);
+  if (M == 0) return MFD_OK;
+  if (!x || !codes || !exps || !out) return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (row_stride % 8 != 0 || group_stride % 8 != 0 || out_stride < N || out_stride % 4 != 0 ||
+      (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(codes) & 15) ||
+      (reinterpret_cast<uintptr_t>(exps) & 3) || (reinterpret_cast<uintptr_t>(out) & 7))
+    return mfd_set_error(MFD_ERR_UNSUPPORTED,
+                         "%s: x and codes need 16-byte alignment, exps 4, output rows 8 (row_stride=%lld group_stride=%lld "
+                         "out_stride=%lld)",
+                         who, (long long)row_stride, (long long)group_stride, (long long)out_stride);
+  const int cus = mfd_num_cus();
+  int nwg = cus;  // whole rounds of the CUs, as few as hold the vocabulary
+  while (N / nwg + 8 > NW * VT_MAX * 16) nwg += cus;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int m0 = 0; m0 < M; m0 += MT) {
+    const HeadArgs a{x, row_stride, group_stride, rows_per_group, m0, codes, exps, out + (int64_t)m0 * out_stride, out_stride,
+                     std::min(MT, M - m0), N, K, nwg};
+    const int rc = a.M <= 16 ? launch_rows<1>(a, cus, st) : a.M <= 32 ? launch_rows<2>(a, cus, st)
+                   : a.M <= 64 ? launch_rows<4>(a, cus, st) : launch_rows<8>(a, cus, st);
+    if (rc != MFD_OK) return rc;
+    MFD_CHECK_LAUNCH();
+  }
+  return MFD_OK;
+}
+
+}  // namespace
+
+extern "C" int mfd_draft_head_mxfp4(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t group_stride,
+                                    const uint8_t* codes, const uint8_t* exps, int M, int N, int K, uint16_t* out,
+                                    int64_t out_stride, void* stream) {
+  return head_gemm(x, row_stride, rows_per_group, group_stride, codes, exps, M, N, K, out, out_stride, stream,
+                   "mfd_draft_head_mxfp4");
+}
+
+extern "C" int mfd_draft_topk_head_mxfp4(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t group_stride,
+                                         const uint8_t* codes, const uint8_t* exps, int M, int N, int K, uint16_t* logits,
+                                         int64_t logits_stride, int k, float* out_logp, void* out_ids, int ids_int64,
+                                         float* out_logz, const int32_t* vocab_ids, void* workspace, int64_t workspace_bytes,
+                                         void* stream) {
+  const int rc = head_gemm(x, row_stride, rows_per_group, group_stride, codes, exps, M, N, K, logits, logits_stride, stream,
+                           "mfd_draft_topk_head_mxfp4");
+  if (rc != MFD_OK || M == 0) return rc;
+  return vocab_ids ? mfd_topk_logz_vocab(logits, M, N, logits_stride, k, out_logp, out_ids, ids_int64, out_logz, vocab_ids,
+                                         workspace, workspace_bytes, stream)
+                   : mfd_topk_logz(logits, M, N, logits_stride, k, out_logp, out_ids, ids_int64, out_logz, workspace,
+                                   workspace_bytes, stream);
+}

@@ -91,15 +91,6 @@ def _same_device(*tensors):
     return device
 
 
-def _call(device, name: str, *args) -> None:
-    """mfd_hip.call on the tensors' device (the current one in nearly every program) and its current stream."""
-    if device.index == torch.cuda.current_device():
-        mfd_hip.call(name, *args, mfd_hip.current_stream(device.index))
-    else:
-        with torch.cuda.device(device):
-            mfd_hip.call(name, *args, mfd_hip.current_stream(device.index))
-
-
 # ----------------------------------------------------------------------------------------------------------- store
 
 
@@ -130,7 +121,7 @@ def kv8_store(*, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     if k_scale.shape != v_scale.shape:
         raise ValueError("the K and V caches have different sizes")
     rows, starts = _index(req_pool_indices, bs, "req_pool_indices"), _index(start_lens, bs, "start_lens")
-    _call(device, "mfd_kv8_store", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp, vp,
+    mfd_hip.call_on(device, "mfd_kv8_store", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp, vp,
           kss, ksh, vss, vsh, ksp, vsp, k_scale.shape[0], *_table_args(page_table), page_size, rows.data_ptr(),
           starts.data_ptr(), cu_tokens.data_ptr(), k.shape[0], bs, int(max_tokens), heads, HEAD_DIM,
           mfd_hip.ptr(err_flag))
@@ -251,7 +242,7 @@ def paged_mode_block_attention_kv8(
             elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
                 raise ValueError(f"a contiguous workspace of {need} bytes is needed")
         rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
-        _call(device, "mfd_kv8_attn", q.data_ptr(), q.stride(0), q.stride(1), *fresh_args, kp, vp, kss, ksh, vss, vsh,
+        mfd_hip.call_on(device, "mfd_kv8_attn", q.data_ptr(), q.stride(0), q.stride(1), *fresh_args, kp, vp, kss, ksh, vss, vsh,
               ksp, vsp, k_scale.shape[0], *_table_args(page_table), page_size, rows.data_ptr(), lens.data_ptr(), bs,
               num_modes, block_size, H, heads, HEAD_DIM, float(scaling), 1 if causal_in_block else 0, splits, keys,
               out.data_ptr(), out.stride(0), out.stride(1), mfd_hip.ptr(lse_out), workspace.data_ptr() if need else None,
@@ -305,7 +296,7 @@ def attention_weights_kv8(*, q: torch.Tensor, lse: torch.Tensor, k_cache: torch.
     device = _same_device(q, lse, k_cache, k_scale, page_table, req_pool_indices, ctx_lens, weights, err_flag)
     kp, kss, ksh, ksp = _cache_args(k_cache, k_scale, "k", page_size)
     rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
-    _call(device, "mfd_kv8_weights", q.data_ptr(), q.stride(0), q.stride(1), lse.data_ptr(), kp, kss, ksh, ksp,
+    mfd_hip.call_on(device, "mfd_kv8_weights", q.data_ptr(), q.stride(0), q.stride(1), lse.data_ptr(), kp, kss, ksh, ksp,
           k_scale.shape[0], *_table_args(page_table), page_size, rows.data_ptr(), lens.data_ptr(), bs, num_modes,
           block_size, H, heads, HEAD_DIM, float(scaling), float(decay), *_weights_args(weights, heads),
           mfd_hip.ptr(err_flag))
@@ -334,7 +325,7 @@ def evict_select(*, weights: torch.Tensor, req_pool_indices: torch.Tensor, ctx_l
     elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
         raise ValueError(f"a contiguous workspace of {need} bytes is needed")
     rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
-    _call(device, "mfd_evict_select", *wargs, heads, rows.data_ptr(), lens.data_ptr(), bs, int(budget), int(sink),
+    mfd_hip.call_on(device, "mfd_evict_select", *wargs, heads, rows.data_ptr(), lens.data_ptr(), bs, int(budget), int(sink),
           int(recent), keep.data_ptr(), new_lens.data_ptr(), workspace.data_ptr() if need else None, need,
           mfd_hip.ptr(err_flag))
     return keep, new_lens
@@ -363,7 +354,7 @@ def evict_compact_kv8(*, keep: torch.Tensor, new_lens: torch.Tensor, ctx_lens: t
     wargs = _weights_args(weights, heads) if weights is not None else (None, 0, 0, 0, 0)
     new, lens = _index(new_lens, bs, "new_lens"), _index(ctx_lens, bs, "ctx_lens")
     rows = _index(req_pool_indices, bs, "req_pool_indices")
-    _call(device, "mfd_evict_compact_kv8", keep.data_ptr(), budget, new.data_ptr(), lens.data_ptr(), kp, vp, kss, ksh, vss,
+    mfd_hip.call_on(device, "mfd_evict_compact_kv8", keep.data_ptr(), budget, new.data_ptr(), lens.data_ptr(), kp, vp, kss, ksh, vss,
           vsh, ksp, vsp, k_scale.shape[0], *_table_args(src_table), *_table_args(dst_table), page_size, rows.data_ptr(),
           *wargs, bs, heads, HEAD_DIM, mfd_hip.ptr(err_flag))
 

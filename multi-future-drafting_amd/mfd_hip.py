@@ -79,6 +79,8 @@ _SIGNATURES = {
     "mfd_draft_prepare": [_P, _P, _P, _P, _I64, _I, _I64, _P, _P, _P, _I, _I, _I, _P],
     "mfd_mode_mask": [_P, _P, _P, _I, _I, _I, _P],
     "mfd_tree_prep": [_P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P],
+    "mfd_draft_head_mxfp4": [_P, _I64, _I, _I64, _P, _P, _I, _I, _I, _P, _I64, _P],
+    "mfd_draft_topk_head_mxfp4": [_P, _I64, _I, _I64, _P, _P, _I, _I, _I, _P, _I64, _I, _P, _P, _I, _P, _P, _P, _I64, _P],
     "mfd_kv8_store": [_P, _P, _I64, _I64, _I64, _I64,       # k, v, strides
                       _P, _P, _I64, _I64, _I64, _I64,      # k_cache, v_cache, strides
                       _P, _P, _I,                          # k_scale, v_scale, pages
@@ -157,9 +159,14 @@ def stream_of(t: torch.Tensor) -> int:
     return _raw_stream(index)
 
 
-def current_stream(index: int) -> int:
-    """The current stream's handle of GPU ``index``."""
-    return _raw_stream(index)
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() with that GPU's current stream as the last argument, and the GPU as the current one (which it is in nearly
+    every program: a launch belongs to the current device, whatever its tensors')."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _raw_stream(device.index))
 
 
 def as_dtype(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
