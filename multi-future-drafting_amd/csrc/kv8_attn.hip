@@ -109,33 +109,44 @@ __device__ __forceinline__ f32x16 mfma32_f16(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// 16 codes -> 16 bf16 values times s (exact), as two 16-byte chunks; 16 codes -> 16 fp16 values (exact)
-__device__ __forceinline__ void widen_k(const u32x4& c, float s, u32x4& lo, u32x4& hi) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s, false));
-    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s, true));
-    if (e < 2) { lo[2 * e] = a; lo[2 * e + 1] = b; }
-    else { hi[2 * e - 4] = a; hi[2 * e - 3] = b; }
-  }
+// Eight codes -> eight bf16 values times s (exact); eight codes -> eight fp16 values (exact)
+__device__ __forceinline__ u32x4 widen_k(uint32_t c0, uint32_t c1, float s) {
+  return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0, s, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, s, true))};
 }
-__device__ __forceinline__ void widen_v(const u32x4& c, u32x4& lo, u32x4& hi) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[e], 1.f, false));
-    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[e], 1.f, true));
-    if (e < 2) { lo[2 * e] = a; lo[2 * e + 1] = b; }
-    else { hi[2 * e - 4] = a; hi[2 * e - 3] = b; }
-  }
+__device__ __forceinline__ u32x4 widen_v(uint32_t c0, uint32_t c1) {
+  return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c0, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c0, 1.f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c1, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c1, 1.f, true))};
 }
 // A row's 16-byte chunks 2 part and 2 part + 1 into a widened tile ([key][d] rows of 256 bytes, chunk c of key r at
 // position c ^ swz). Parts 4 .. 7 write the upper one first: the eight lanes of a row then hit all banks at once.
-__device__ __forceinline__ void put_row(uint16_t* tile, int r, int part, int swz, const u32x4& lo, const u32x4& hi) {
-  const bool up = part >= 4;
-  const u32x4 first = up ? hi : lo, second = up ? lo : hi;
-  const int c0 = 2 * part + (up ? 1 : 0);
+__device__ __forceinline__ void put_chunks(uint16_t* tile, int r, int part, int swz, const u32x4& first,
+                                           const u32x4& second) {
+  const int c0 = 2 * part + (part >> 2);
   *reinterpret_cast<u32x4*>(tile + (r * 16 + (c0 ^ swz)) * 8) = first;
   *reinterpret_cast<u32x4*>(tile + (r * 16 + ((c0 ^ 1) ^ swz)) * 8) = second;
+}
+__device__ __forceinline__ void put_row(uint16_t* tile, int r, int part, int swz, const u32x4& lo, const u32x4& hi) {
+  const bool up = part >= 4;
+  put_chunks(tile, r, part, swz, up ? hi : lo, up ? lo : hi);
+}
+__device__ __forceinline__ void put_k_codes(uint16_t* tile, int r, int part, const u32x4& c, float s) {
+  const bool up = part >= 4;
+  put_chunks(tile, r, part, r & 15, widen_k(up ? c[2] : c[0], up ? c[3] : c[1], s),
+             widen_k(up ? c[0] : c[2], up ? c[1] : c[3], s));
+}
+__device__ __forceinline__ void put_v_codes(uint16_t* tile, int r, int part, const u32x4& c) {
+  const bool up = part >= 4;
+  put_chunks(tile, r, part, (r & 3) << 2, widen_v(up ? c[2] : c[0], up ? c[3] : c[1]),
+             widen_v(up ? c[0] : c[2], up ? c[1] : c[3]));
+}
+// Row `slot` of a cache (ids and strides below 2^31: one 32 x 32 + 64 bit instruction)
+__device__ __forceinline__ const uint8_t* slot_row(const uint8_t* cache, int slot, uint32_t ss) {
+  return cache + (uint64_t)(uint32_t)slot * ss;
 }
 __device__ __forceinline__ int k_swz(int r) { return r & 15; }
 __device__ __forceinline__ int v_swz(int r) { return (r & 3) << 2; }
@@ -181,13 +192,15 @@ __device__ __forceinline__ int64_t partial_row(const Args& a, int s, int b, int 
 
 // ------------------------------------------------------------------------------------------------ tile kernel
 
-template <int NW>
+// WHOLE: pages of at least 64 tokens, so that a tile lies in one page: its page id, address and scales are wave-uniform,
+// come by scalar loads and live in scalar registers. Else each thread looks up its own keys' pages.
+template <int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attn_tile_kernel(Args a) {
   static_assert(NW == 4 || NW == 8, "workgroups of 4 or 8 waves");
   constexpr int NPT = 8 / NW;   // 16-code pieces of a K or V tile per thread
   constexpr int RSTEP = NW * 8;
   __shared__ __attribute__((aligned(1024))) uint16_t lds_k[2 * TILE], lds_v[2 * TILE];
-  __shared__ uint32_t lds_vs[2 * TK];
+  __shared__ uint32_t lds_vs[WHOLE ? 1 : 2 * TK];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
@@ -304,41 +317,67 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     return (m_run == -INFINITY) ? 0.f : m_run;
   };
 
-  // ---- staging: thread (row tid / 8 + i RSTEP, 16 codes tid % 8) of a tile
+  // ---- staging: thread (row tid / 8 + i RSTEP, 16 codes tid % 8) of a tile. Keys past the range repeat its last one
+  //      (probability 0).
   const int r0 = tid >> 3, part = tid & 7;
-  const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh + part * 16;
-  const uint8_t* vc_h = a.vc + (int64_t)kvh * a.vc_sh + part * 16;
+  const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh;
+  const uint8_t* vc_h = a.vc + (int64_t)kvh * a.vc_sh;
   const float* ks_h = a.ks + kvh;
   const float* vs_h = a.vs + kvh;
-  const int64_t kc_ss = a.kc_ss, vc_ss = a.vc_ss;
+  const uint32_t kc_ss = (uint32_t)a.kc_ss, vc_ss = (uint32_t)a.vc_ss;
   const int Hkv = a.Hkv;
   int bad = 0;
-  // keys past the range repeat its last one (probability 0)
+  typedef const __attribute__((address_space(4))) int32_t* const_i32p;
+  typedef const __attribute__((address_space(4))) float* const_f32p;
+  constexpr int NE = WHOLE ? 1 : NPT;  // page ids of a tile that a thread keeps
   auto key_of = [&](int t, int i) __attribute__((always_inline)) { return min(lo + t * TK + r0 + i * RSTEP, hi - 1); };
-  auto page_of = [&](int t, int i) __attribute__((always_inline)) {
-    const int e = trow[key_of(t, i) >> shift];
-    const bool ok = (uint32_t)e < (uint32_t)num_pages;
-    bad |= ok ? 0 : 1;
-    return ok ? e : 0;
+  auto pages_of = [&](int t, int (&e)[NE]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      int x;
+      if constexpr (WHOLE) x = ((const_i32p)trow)[__builtin_amdgcn_readfirstlane((lo + t * TK) >> shift)];
+      else x = trow[key_of(t, i) >> shift];
+      const bool ok = (uint32_t)x < (uint32_t)num_pages;
+      bad |= ok ? 0 : 1;
+      e[i] = ok ? x : 0;
+    }
   };
-  auto load = [&](const uint8_t* cache, int64_t ss, const float* scale, int t, int i, int e, u32x4& c, float& sc)
-                  __attribute__((always_inline)) {
-    const int64_t slot = ((int64_t)e << shift) + (key_of(t, i) & pmask);
-    c = *reinterpret_cast<const u32x4*>(cache + slot * ss);
-    sc = scale[(int64_t)e * Hkv];
+  auto load = [&](const uint8_t* cache, uint32_t ss, const float* scale, int t, const int (&e)[NE], u32x4 (&c)[NPT],
+                  float (&sc)[NE]) __attribute__((always_inline)) {
+    if constexpr (WHOLE) {
+      const int k0 = lo + t * TK;
+      const uint8_t* base = slot_row(cache, __builtin_amdgcn_readfirstlane((e[0] << shift) + (k0 & pmask)), ss);
+      const int nv = hi - k0;
+      if (nv >= TK) {
+#pragma unroll
+        for (int i = 0; i < NPT; ++i)
+          c[i] = *reinterpret_cast<const u32x4*>(base + i * RSTEP * ss + ((uint32_t)r0 * ss + (uint32_t)part * 16));
+      } else {
+#pragma unroll
+        for (int i = 0; i < NPT; ++i)
+          c[i] = *reinterpret_cast<const u32x4*>(
+              base + ((uint32_t)min(r0 + i * RSTEP, nv - 1) * ss + (uint32_t)part * 16));
+      }
+      sc[0] = ((const_f32p)scale)[__builtin_amdgcn_readfirstlane(e[0] * Hkv)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        c[i] = *reinterpret_cast<const u32x4*>(slot_row(cache, (e[i] << shift) + (key_of(t, i) & pmask), ss) + part * 16);
+        sc[i] = scale[e[i] * Hkv];
+      }
+    }
   };
-  auto put_k = [&](int j, int i, const u32x4& c, float sc) __attribute__((always_inline)) {
-    u32x4 x, y;
-    widen_k(c, sc, x, y);
-    const int rr = r0 + i * RSTEP;
-    put_row(lds_k + j * TILE, rr, part, k_swz(rr), x, y);
+  auto put_k = [&](int j, const u32x4 (&c)[NPT], const float (&sc)[NE]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NPT; ++i) put_k_codes(lds_k + j * TILE, r0 + i * RSTEP, part, c[i], sc[WHOLE ? 0 : i]);
   };
-  auto put_v = [&](int j, int i, const u32x4& c, float sc) __attribute__((always_inline)) {
-    u32x4 x, y;
-    widen_v(c, x, y);
-    const int rr = r0 + i * RSTEP;
-    put_row(lds_v + j * TILE, rr, part, v_swz(rr), x, y);
-    if (part == 0) lds_vs[j * TK + rr] = __float_as_uint(sc);
+  auto put_v = [&](int j, const u32x4 (&c)[NPT], const float (&sc)[NE]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NPT; ++i) {
+      put_v_codes(lds_v + j * TILE, r0 + i * RSTEP, part, c[i]);
+      if constexpr (!WHOLE)
+        if (part == 0) lds_vs[j * TK + r0 + i * RSTEP] = __float_as_uint(sc[i]);
+    }
   };
 
   if (ntiles > 0) {
@@ -346,36 +385,26 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // V(t + 1) in (or on their way to) registers and S(t) is computed; it writes those two into the buffers that
     // iteration t - 1 read last, asks for K(t + 3) and V(t + 2), and computes S(t + 1) and O += V(t) P(t).
     u32x4 kr[NPT], vr[NPT];
-    float ksc[NPT], vsc[NPT];
-    int ev[NPT], ek[NPT];  // pages of tiles t + 2 and t + 3
+    float ksc[NE], vsc[NE];
+    int ev[NE], ek[NE];  // pages of tiles t + 2 and t + 3
+    uint32_t vs_t;       // WHOLE: scale of V(t)
     {
       u32x4 k0[NPT], v0[NPT];
-      float k0s[NPT], v0s[NPT];
-      int e0[NPT], e1[NPT];
-#pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        e0[i] = page_of(0, i);
-        e1[i] = page_of(min(1, last), i);
-        ev[i] = page_of(min(2, last), i);
-        ek[i] = page_of(min(3, last), i);
-      }
-#pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        load(kc_h, kc_ss, ks_h, 0, i, e0[i], k0[i], k0s[i]);
-        load(vc_h, vc_ss, vs_h, 0, i, e0[i], v0[i], v0s[i]);
-        load(kc_h, kc_ss, ks_h, min(1, last), i, e1[i], kr[i], ksc[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        put_k(0, i, k0[i], k0s[i]);
-        put_v(0, i, v0[i], v0s[i]);
-        put_k(1, i, kr[i], ksc[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        load(kc_h, kc_ss, ks_h, min(2, last), i, ev[i], kr[i], ksc[i]);
-        load(vc_h, vc_ss, vs_h, min(1, last), i, e1[i], vr[i], vsc[i]);
-      }
+      float k0s[NE], v0s[NE];
+      int e0[NE], e1[NE];
+      pages_of(0, e0);
+      pages_of(min(1, last), e1);
+      pages_of(min(2, last), ev);
+      pages_of(min(3, last), ek);
+      load(kc_h, kc_ss, ks_h, 0, e0, k0, k0s);
+      load(vc_h, vc_ss, vs_h, 0, e0, v0, v0s);
+      load(kc_h, kc_ss, ks_h, min(1, last), e1, kr, ksc);
+      put_k(0, k0, k0s);
+      put_v(0, v0, v0s);
+      put_k(1, kr, ksc);
+      vs_t = __float_as_uint(v0s[0]);
+      load(kc_h, kc_ss, ks_h, min(2, last), ev, kr, ksc);
+      load(vc_h, vc_ss, vs_h, min(1, last), e1, vr, vsc);
     }
     f32x16 s_a[2], s_b[2];
     lds_barrier();
@@ -394,45 +423,44 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         return *reinterpret_cast<const u32x4*>(lds_k + ((kb ^ ((sl & 7) << 4)) + (sl >= 16 ? 32 * 128 : 0)));
       return v_frag((vb ^ ((sl & 3) << 5)) + 2048 * chunk_of(sl));
     };
+    auto set_unit = [&](uint32_t vsn) __attribute__((always_inline)) {
+      if (vsn != vcur) {
+        const float f = scale_quotient(vcur, vsn);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
+        vcur = vsn;
+      }
+    };
     auto iteration = [&](int t, f32x16 (&s_cur)[2], f32x16 (&s_nxt)[2]) __attribute__((always_inline)) {
       const int j = t & 1;
-#pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        put_k(j, i, kr[i], ksc[i]);
-        put_v(j ^ 1, i, vr[i], vsc[i]);
-      }
+      put_k(j, kr, ksc);
+      put_v(j ^ 1, vr, vsc);
+      const uint32_t vs_next = __float_as_uint(vsc[0]);
       if (t + 2 < ntiles) {
+        load(vc_h, vc_ss, vs_h, t + 2, ev, vr, vsc);
+        load(kc_h, kc_ss, ks_h, min(t + 3, last), ek, kr, ksc);
 #pragma unroll
-        for (int i = 0; i < NPT; ++i) {
-          load(vc_h, vc_ss, vs_h, t + 2, i, ev[i], vr[i], vsc[i]);
-          load(kc_h, kc_ss, ks_h, min(t + 3, last), i, ek[i], kr[i], ksc[i]);
-          ev[i] = ek[i];
-          ek[i] = page_of(min(t + 4, last), i);
-        }
+        for (int i = 0; i < NE; ++i) ev[i] = ek[i];
+        pages_of(min(t + 4, last), ek);
       }
       if (active) {
         const int khi = hi - (lo + t * TK);
         const float msub = softmax_max(khi < TK, 0, khi, s_cur);
         const int kb = k_base + (j ^ 1) * TILE, vb = v_base + j * TILE;
+        if constexpr (WHOLE) set_unit(vs_t);
         u32x4 opnd[32];
 #pragma unroll
         for (int sl = 0; sl < FD; ++sl) opnd[sl] = fetch(sl, kb, vb);
-        const uint32_t vs_l = lds_vs[j * TK + 16 * (lane & 3)];  // scales of the four 16-key chunks
+        uint32_t vs_l = 0;  // scales of the four 16-key chunks
+        if constexpr (!WHOLE) vs_l = lds_vs[j * TK + 16 * (lane & 3)];
         u32x4 pv[4];  // P^T B fragments (fp16 pairs) of the chunks
         float psum = 0.f;
         f32x16 acc0 = {}, acc1 = {};
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int sl = 0; sl < 32; ++sl) {
-          if (sl == 8 || sl == 12 || sl == 24 || sl == 28) {
-            const uint32_t vsn = __builtin_amdgcn_readlane(vs_l, chunk_of(sl));
-            if (vsn != vcur) {
-              const float f = scale_quotient(vcur, vsn);
-#pragma unroll
-              for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
-              vcur = vsn;
-            }
-          }
+          if constexpr (!WHOLE)
+            if (sl == 8 || sl == 12 || sl == 24 || sl == 28) set_unit(__builtin_amdgcn_readlane(vs_l, chunk_of(sl)));
           if (sl + FD < 32) opnd[sl + FD] = fetch(sl + FD, kb, vb);
           if (slot_is_qk(sl)) {
             if (sl < 8) acc0 = mfma32(__builtin_bit_cast(bf16x8, opnd[sl]), qf[sl & 7], acc0);
@@ -455,6 +483,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         s_nxt[0] = acc0;
         s_nxt[1] = acc1;
       }
+      vs_t = vs_next;
       lds_barrier();
     };
     for (int t = 0;;) {
@@ -662,7 +691,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int Hkv = a.Hkv;
   const float* ks_h = a.ks + kvh;
   const float* vs_h = a.vs + kvh;
-  const int64_t kc_ss = a.kc_ss, vc_ss = a.vc_ss;
+  const uint32_t kc_ss = (uint32_t)a.kc_ss, vc_ss = (uint32_t)a.vc_ss;
   const int ntiles = (hi - lo + SK - 1) / SK;
   int bad = 0;
   auto key_of = [&](int t, int i) __attribute__((always_inline)) { return min(lo + t * SK + r0 + 8 * i, hi - 1); };
@@ -679,11 +708,11 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto load = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t slot = ((int64_t)en[i] << shift) + (key_of(t, i) & pmask);
-        kr[i] = *reinterpret_cast<const u32x4*>(kc_h + slot * kc_ss);
-        vr[i] = *reinterpret_cast<const u32x4*>(vc_h + slot * vc_ss);
-        ksc[i] = ks_h[(int64_t)en[i] * Hkv];
-        vsc[i] = vs_h[(int64_t)en[i] * Hkv];
+        const int slot = (en[i] << shift) + (key_of(t, i) & pmask);
+        kr[i] = *reinterpret_cast<const u32x4*>(slot_row(kc_h, slot, kc_ss));
+        vr[i] = *reinterpret_cast<const u32x4*>(slot_row(vc_h, slot, vc_ss));
+        ksc[i] = ks_h[en[i] * Hkv];
+        vsc[i] = vs_h[en[i] * Hkv];
       }
     };
 #pragma unroll
@@ -697,12 +726,8 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       // (a wave's LDS operations complete in order: nothing of the last tile is still to be read)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u32x4 x, y;
-        const int rr = r0 + 8 * i;
-        widen_k(kr[i], ksc[i], x, y);
-        put_row(lds_k, rr, part, k_swz(rr), x, y);
-        widen_v(vr[i], x, y);
-        put_row(lds_v, rr, part, v_swz(rr), x, y);
+        put_k_codes(lds_k, r0 + 8 * i, part, kr[i], ksc[i]);
+        put_v_codes(lds_v, r0 + 8 * i, part, vr[i]);
       }
       const uint32_t vs_t[2] = {(uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(vsc[0])),
                                 (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(vsc[2]))};
@@ -938,6 +963,7 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
 // Every sum has one owner and one order: no atomics. Bound by the exponentials (one per product of 256 flops).
 constexpr int WNW = 4;
 constexpr int WKEYS = WNW * TK;
+constexpr int WOCC = 3;  // waves per SIMD
 
 struct WArgs {
   const uint16_t* q;
@@ -956,8 +982,9 @@ struct WArgs {
   int32_t* err_flag;
 };
 
-__global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_weights_kernel(WArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[WNW * TILE];  // keys first, then two Q units of 8 KB
+__global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, WOCC))) void kv8_weights_kernel(WArgs a) {
+  // 32 keys of each wave at a time first, then two Q units of 8 KB
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[WNW * SK * D];
   __shared__ float lds_lse[2][UROWS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -973,10 +1000,47 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int lo = blockIdx.x * WKEYS;
   if (lo >= ctx) return;
 
-  // keys of this wave: 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i
+  // Q unit u: row tid / 8 of 32, 16 elements tid % 8. A row's lse in base 2; padding rows and rows whose lse is -inf
+  // (they saw no key) get +inf: their probabilities are 0.
+  const int units = (a.rows + UROWS - 1) / UROWS;
+  const int qr = tid >> 3, qpart = tid & 7;
+  const int dg = UROWS / a.KL, dq = UROWS % a.KL;
+  const int64_t q_step = dg * a.q_sh + dq * a.q_st, q_wrap = a.q_sh - a.KL * a.q_st;
+  const int64_t l_step = dg + (int64_t)dq * a.H, l_wrap = 1 - (int64_t)a.KL * a.H;
+  int rr = qr, rq = qr % a.KL;  // the next unit's row and its query (padding rows repeat the first row)
+  const uint16_t* const q_first = a.q + (int64_t)b * a.KL * a.q_st + (int64_t)kvh * a.G * a.q_sh + qpart * 16;
+  const float* const l_first = a.lse + (int64_t)b * a.KL * a.H + kvh * a.G;
+  const uint16_t* qp = q_first + (qr / a.KL) * a.q_sh + rq * a.q_st;
+  const float* lp = l_first + qr / a.KL + (int64_t)rq * a.H;
+  u32x4 qx, qy;
+  float ql = 0.f;
+  bool q_ok = false;
+  auto load_q = [&]() __attribute__((always_inline)) {
+    q_ok = rr < a.rows;
+    const u32x4* p = reinterpret_cast<const u32x4*>(q_ok ? qp : q_first);
+    qx = p[0];
+    qy = p[1];
+    ql = *(q_ok ? lp : l_first);
+    rr += UROWS;
+    rq += dq;
+    const bool wrap = rq >= a.KL;
+    rq -= wrap ? a.KL : 0;
+    qp += q_step + (wrap ? q_wrap : 0);
+    lp += l_step + (wrap ? l_wrap : 0);
+  };
+  auto put_q = [&](int j) __attribute__((always_inline)) {
+    put_row(lds + j * (UROWS * D), qr, qpart, k_swz(qr), qx, qy);
+    if (qpart == 0) lds_lse[j][qr] = q_ok && ql != -INFINITY ? ql * 1.4426950408889634f : INFINITY;
+  };
+  load_q();
+
+  // keys of this wave: 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i, 32 rows through LDS at a time
+  const int base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
+  bf16x8 kf[2][D / 16];
   {
     const int r0 = lane >> 3, part = lane & 7;
-    uint16_t* tile = lds + w * TILE;
+    const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh + part * 16;
+    uint16_t* tile = lds + w * (SK * D);
     int bad = 0;
     int e[8];
     u32x4 c[8];
@@ -993,61 +1057,33 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int key = min(lo + w * TK + r0 + 8 * i, ctx - 1);
-      const int64_t slot = ((int64_t)e[i] << shift) + (key & pmask);
-      c[i] = *reinterpret_cast<const u32x4*>(a.kc + slot * a.kc_ss + (int64_t)kvh * a.kc_sh + part * 16);
-      sc[i] = a.ks[(int64_t)e[i] * a.Hkv + kvh];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      u32x4 x, y;
-      widen_k(c[i], sc[i], x, y);
-      put_row(tile, r0 + 8 * i, part, k_swz(r0 + 8 * i), x, y);
+      c[i] = *reinterpret_cast<const u32x4*>(slot_row(kc_h, (e[i] << shift) + (key & pmask), (uint32_t)a.kc_ss));
+      sc[i] = a.ks[e[i] * a.Hkv + kvh];
     }
     if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put_k_codes(tile, r0 + 8 * i, part, c[4 * ks + i], sc[4 * ks + i]);
+      asm volatile("" ::: "memory");  // (a wave's LDS operations complete in order)
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+        kf[ks][d] = as_bf16x8(*reinterpret_cast<const u16x8*>(tile + (base ^ (d << 4))));
+      asm volatile("" ::: "memory");
+    }
   }
-  asm volatile("" ::: "memory");
-  const int base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
-  bf16x8 kf[2][D / 16];
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c)
-      kf[ks][c] = as_bf16x8(*reinterpret_cast<const u16x8*>(lds + w * TILE + (base ^ (c << 4)) + ks * 32 * 128));
   lds_barrier();
-
-  // Q unit u: row tid / 8 of 32, 16 elements tid % 8. A row's lse in base 2; padding rows and rows whose lse is -inf
-  // (they saw no key) get +inf: their probabilities are 0.
-  const int units = (a.rows + UROWS - 1) / UROWS;
-  const int qr = tid >> 3, qpart = tid & 7;
-  u32x4 qx, qy;
-  float ql = 0.f;
-  auto load_q = [&](int u) __attribute__((always_inline)) {
-    const int rr = u * UROWS + qr;
-    const int r = min(rr, a.rows - 1);
-    const int head = kvh * a.G + r / a.KL;
-    const int64_t token = (int64_t)b * a.KL + r % a.KL;
-    const u32x4* qp = reinterpret_cast<const u32x4*>(a.q + token * a.q_st + (int64_t)head * a.q_sh + qpart * 16);
-    qx = qp[0];
-    qy = qp[1];
-    const float l = a.lse[token * a.H + head];
-    ql = rr < a.rows && l != -INFINITY ? l * 1.4426950408889634f : INFINITY;
-  };
-  auto put_q = [&](int j) __attribute__((always_inline)) {
-    put_row(lds + j * (UROWS * D), qr, qpart, k_swz(qr), qx, qy);
-    if (qpart == 0) lds_lse[j][qr] = ql;
-  };
   float acc[32];
 #pragma unroll
   for (int x = 0; x < 32; ++x) acc[x] = 0.f;
-  load_q(0);
   put_q(0);
-  if (units > 1) load_q(1);
+  if (units > 1) load_q();
   lds_barrier();
   for (int u = 0; u < units; ++u) {
     const int j = u & 1;
     if (u + 1 < units) {  // buffer j ^ 1 was last read in iteration u - 1
       put_q(j ^ 1);
-      if (u + 2 < units) load_q(u + 2);
+      if (u + 2 < units) load_q();
     }
     const uint16_t* qb = lds + j * (UROWS * D);
     f32x16 s0 = {}, s1 = {};
@@ -1058,12 +1094,12 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       s1 = mfma32(kf[1][c], qf, s1);
     }
     const float l = lds_lse[j][l32];
+    lds_barrier();
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       acc[x] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[x], a.scale_log2, -l));
       acc[16 + x] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[x], a.scale_log2, -l));
     }
-    lds_barrier();
   }
   // Sum over the 32 lanes of a half, halving the registers as the lanes are joined: in step m a lane keeps the half of its
   // registers that its bit m names and gives the other half to lane ^ m. Register x ends in the lane whose bits 4 .. 0
@@ -1170,10 +1206,14 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
     return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   if (units == 1)
     hipLaunchKernelGGL(kv8_attn_stream_kernel, dim3((unsigned)grid), dim3(SNW * 64), 0, st, a);
+  else if (NW == 8 && page_size >= TK)
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<8, true>), dim3((unsigned)grid), dim3(512), 0, st, a);
   else if (NW == 8)
-    hipLaunchKernelGGL(kv8_attn_tile_kernel<8>, dim3((unsigned)grid), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<8, false>), dim3((unsigned)grid), dim3(512), 0, st, a);
+  else if (page_size >= TK)
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<4, true>), dim3((unsigned)grid), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL(kv8_attn_tile_kernel<4>, dim3((unsigned)grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<4, false>), dim3((unsigned)grid), dim3(256), 0, st, a);
   MFD_CHECK_LAUNCH();
   if (a.S > 1) {
     hipLaunchKernelGGL(kv8_attn_merge_kernel, dim3((unsigned)((prows + 15) / 16)), dim3(256), 0, st, a);

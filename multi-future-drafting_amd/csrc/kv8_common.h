@@ -87,6 +87,10 @@ inline int check_cache(const char* who, const void* k_cache, const void* v_cache
   if (((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) ||
       ((kc_ss | kc_sh | vc_ss | vc_sh) & 15))
     return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: cache rows need 16-byte alignment (bases and strides)", who);
+  // slot ids and strides are 32-bit in the kernels, and so is a tile's row offset: 63 strides
+  if ((int64_t)num_pages * page_size > 0x7fffffff || (int64_t)num_pages * Hkv > 0x7fffffff || kc_ss < 0 || vc_ss < 0 ||
+      kc_ss > (1 << 25) || vc_ss > (1 << 25))
+    return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: needs fewer than 2^31 slots and scales, and slot strides in [0, 2^25]", who);
   return MFD_OK;
 }
 

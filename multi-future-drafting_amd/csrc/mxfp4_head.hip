@@ -27,8 +27,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int MT = 128;   // drafted rows of one launch
 constexpr int KS = 128;   // k per step
 constexpr int NW = 8;     // waves of the wide form
-constexpr int VT_MAX = 5;
-constexpr int BLOCK = 64 * 1024;  // bytes of a drafted-row block in LDS
 constexpr int KNW = 4;    // waves of the k-split form
 
 struct HeadArgs {
@@ -52,6 +50,10 @@ template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   static_assert(N >= 0 && N < 64, "vmcnt");
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), (short)0, (int)bytes, 0x00020000);
 }
 
 __device__ __forceinline__ const uint16_t* drafted_row(const HeadArgs& a, int r) {
@@ -85,19 +87,31 @@ __device__ __forceinline__ void store4(uint16_t* orow, int n, int rows, const f3
   }
 }
 
+// Sizes of the wide form by MTL
+template <int MTL>
+struct Wide {
+  static constexpr int BLOCK = (MTL <= 2 ? 32 : 64) * 1024;  // bytes of a drafted-row block
+  static constexpr int HPS = MTL == 8 ? 1 : 2;   // 128-k halves per step
+  static constexpr int WPC = MTL <= 2 ? 2 : 1;   // workgroups per CU
+  static constexpr int VT_MAX = MTL <= 2 ? 3 : 5;
+};
+
 template <int VT, int MTL>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void mxfp4_wide_kernel(HeadArgs a) {
-  constexpr int HB = 2048 / MTL;        // k per drafted block
-  constexpr int CPR = HB / 8;           // 16-byte chunks of a row's block
-  constexpr int SPB = HB / KS;          // steps per block
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2 * Wide<MTL>::WPC, 2 * Wide<MTL>::WPC)))
+void mxfp4_wide_kernel(HeadArgs a) {
+  constexpr int BLOCK = Wide<MTL>::BLOCK, HPS = Wide<MTL>::HPS;
+  constexpr int HB = BLOCK / (32 * MTL);  // k per drafted block
+  constexpr int CPR = HB / 8;             // 16-byte chunks of a row's block
+  constexpr int SPB = HB / (KS * HPS);    // steps per block
   constexpr int LPW = BLOCK / 1024 / NW;  // direct loads of a wave per block
+  static_assert(SPB % 2 == 0, "steps go in pairs");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R0 = wg_row0(blockIdx.x, a.N, a.nwg);
   const int rows = wg_row0(blockIdx.x + 1, a.N, a.nwg) - R0;
   if (rows <= 0) return;
-  const int K = a.K, S = K / KS;
+  const int K = a.K, S = (K + KS * HPS - 1) / (KS * HPS);
   const int l16 = lane & 15, g4 = lane >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
 
@@ -111,48 +125,60 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       dma16(drafted_row(a, r) + min(b * HB + 8 * c, K - 8), lds0 + (uint32_t)(b & 1) * BLOCK + (uint32_t)(i * NW + w) * 1024u);
     }
   };
-  // this wave's tiles t0 .. t0 + vtv - 1; past them it loads (but does not multiply) the last one again
+  // this wave's tiles t0 .. t0 + vtv - 1; past them it loads (but does not multiply) the last one again, so that the number
+  // of its loads is known. Rows past the range read as zero by the buffers' bounds.
   const int T = (rows + 15) / 16;
   const int t0 = __builtin_amdgcn_readfirstlane(w * T / NW);
   const int vtv = __builtin_amdgcn_readfirstlane((w + 1) * T / NW) - t0;
-  const uint8_t* cp[VT];
-  const uint8_t* ep[VT];
-#pragma unroll
-  for (int i = 0; i < VT; ++i) {
-    const int64_t row = R0 + min(16 * (t0 + min(i, max(vtv - 1, 0))) + l16, rows - 1);
-    cp[i] = a.codes + row * (K / 2) + 16 * g4;
-    ep[i] = a.exps + row * (K / 32);
-  }
+  const __amdgpu_buffer_rsrc_t rc = buffer_of(a.codes + (int64_t)R0 * (K / 2), (uint32_t)rows * (uint32_t)(K / 2));
+  const __amdgpu_buffer_rsrc_t re = buffer_of(a.exps + (int64_t)R0 * (K / 32), (uint32_t)rows * (uint32_t)(K / 32));
+  const uint32_t coff = (uint32_t)(16 * min(t0, T - 1) + l16) * (uint32_t)(K / 2) + 16u * g4;
+  const uint32_t eoff = (uint32_t)(16 * min(t0, T - 1) + l16) * (uint32_t)(K / 32);
   f32x4 acc[VT][MTL];
 #pragma unroll
   for (int i = 0; i < VT; ++i)
 #pragma unroll
     for (int j = 0; j < MTL; ++j) acc[i][j] = (f32x4){};
-  u32x4 wf[2][VT];
-  uint32_t ef[2][VT];
+  u32x4 wf[2][VT][HPS];
+  uint32_t ef[2][VT][HPS];
   auto load_w = [&](int p, int v) __attribute__((always_inline)) {
-    const int u = min(v, S - 1);
+    const uint32_t u = (uint32_t)min(v, S - 1);
 #pragma unroll
     for (int i = 0; i < VT; ++i) {
-      wf[p][i] = *reinterpret_cast<const u32x4*>(cp[i] + 64 * u);
-      ef[p][i] = *reinterpret_cast<const uint32_t*>(ep[i] + 4 * u);
+      const uint32_t tile = (uint32_t)min(i, max(vtv - 1, 0));
+      const uint32_t cs = tile * (uint32_t)(8 * K) + u * (64u * HPS), es = tile * (uint32_t)(K / 2) + u * (4u * HPS);
+#pragma unroll
+      for (int h = 0; h < HPS; ++h)
+        wf[p][i][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, coff, cs + 64u * h, 0));
+      if constexpr (HPS == 1) {
+        ef[p][i][0] = __builtin_amdgcn_raw_buffer_load_b32(re, eoff, es, 0);
+      } else {
+        const u32x2 e = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(re, eoff, es, 0));
+        ef[p][i][0] = e[0];
+        ef[p][i][HPS - 1] = e[1];
+      }
     }
   };
   auto step = [&](int p, int v) __attribute__((always_inline)) {
     const uint8_t* base = smem + ((v / SPB) & 1) * BLOCK + l16 * (HB * 2);
-    const int c0 = (v % SPB) * (KS / 8) + 4 * g4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bf16x8 xf[MTL];
+    for (int h = 0; h < HPS; ++h) {
+      if (h > 0 && (v * HPS + h) * KS >= K) break;  // K is an odd number of halves
+      const int c0 = ((v % SPB) * HPS + h) * (KS / 8) + 4 * g4;
 #pragma unroll
-      for (int m = 0; m < MTL; ++m)
-        xf[m] = *reinterpret_cast<const bf16x8*>(base + 16 * m * (HB * 2) + (((c0 + j) ^ l16) << 4));
+      for (int j = 0; j < 4; ++j) {
+        bf16x8 f[VT];
 #pragma unroll
-      for (int i = 0; i < VT; ++i) {
-        if (i >= vtv) break;
-        const bf16x8 f = widen(wf[p][i][j], scale_of(ef[p][i], g4));
+        for (int i = 0; i < VT; ++i) f[i] = widen(wf[p][i][h][j], scale_of(ef[p][i][h], g4));
 #pragma unroll
-        for (int m = 0; m < MTL; ++m) acc[i][m] = mfma16(f, xf[m], acc[i][m]);
+        for (int m = 0; m < MTL; ++m) {
+          const bf16x8 xf = *reinterpret_cast<const bf16x8*>(base + 16 * m * (HB * 2) + (((c0 + j) ^ l16) << 4));
+#pragma unroll
+          for (int i = 0; i < VT; ++i) {
+            if (i >= vtv) break;
+            acc[i][m] = mfma16(f[i], xf, acc[i][m]);
+          }
+        }
       }
     }
   };
@@ -160,8 +186,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   load_w(0, 0);
   load_w(1, 1);
   for (int b = 0; b * SPB < S; ++b) {
-    // the block's direct loads have landed: the 4 VT weight loads of two steps are younger
-    wait_vmcnt<4 * VT>();
+    // the block's direct loads have landed: the weight loads of two steps, VT (HPS + 1) each, are younger
+    wait_vmcnt<2 * VT * (HPS + 1)>();
     __syncthreads();  // in every wave; and block b - 1 is read, so its half is free
     if ((b + 1) * SPB < S) issue_x(b + 1);
     const int end = min((b + 1) * SPB, S);
@@ -277,17 +303,24 @@ __global__ __launch_bounds__(KNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 template <int VT, int MTL>
 int launch_wide(const HeadArgs& a, hipStream_t st) {
-  const int rc = mfd_set_max_lds(reinterpret_cast<const void*>(&mxfp4_wide_kernel<VT, MTL>), 2 * BLOCK);
-  if (rc != MFD_OK) return rc;
-  hipLaunchKernelGGL((mxfp4_wide_kernel<VT, MTL>), dim3((unsigned)a.nwg), dim3(NW * 64), 2 * BLOCK, st, a);
+  if constexpr (VT <= Wide<MTL>::VT_MAX) {
+    constexpr int lds = 2 * Wide<MTL>::BLOCK;
+    const int rc = mfd_set_max_lds(reinterpret_cast<const void*>(&mxfp4_wide_kernel<VT, MTL>), lds);
+    if (rc != MFD_OK) return rc;
+    hipLaunchKernelGGL((mxfp4_wide_kernel<VT, MTL>), dim3((unsigned)a.nwg), dim3(NW * 64), lds, st, a);
+  }
   return MFD_OK;
 }
 template <int MTL>
-int launch_rows(const HeadArgs& a, int cus, hipStream_t st) {
+int launch_rows(HeadArgs a, int cus, hipStream_t st) {
   if ((int64_t)a.N <= (int64_t)NW * 16 * cus / 2) {
     hipLaunchKernelGGL((mxfp4_ksplit_kernel<1, MTL>), dim3((unsigned)((a.N + 15) / 16)), dim3(KNW * 64), 0, st, a);
     return MFD_OK;
   }
+  // whole rounds of the workgroups that run together, as few as hold the vocabulary
+  const int slots = Wide<MTL>::WPC * cus;
+  a.nwg = slots;
+  while (a.N / a.nwg + 8 > NW * Wide<MTL>::VT_MAX * 16) a.nwg += slots;
   const int vt = (a.N / a.nwg + 8 + 16 * NW - 1) / (16 * NW);  // tiles of a wave
   switch (vt) {
     case 1: return launch_wide<1, MTL>(a, st);
@@ -313,12 +346,10 @@ int head_gemm(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t
                          "out_stride=%lld)",
                          who, (long long)row_stride, (long long)group_stride, (long long)out_stride);
   const int cus = mfd_num_cus();
-  int nwg = cus;  // whole rounds of the CUs, as few as hold the vocabulary
-  while (N / nwg + 8 > NW * VT_MAX * 16) nwg += cus;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   for (int m0 = 0; m0 < M; m0 += MT) {
     const HeadArgs a{x, row_stride, group_stride, rows_per_group, m0, codes, exps, out + (int64_t)m0 * out_stride, out_stride,
-                     std::min(MT, M - m0), N, K, nwg};
+                     std::min(MT, M - m0), N, K, 0};
     const int rc = a.M <= 16 ? launch_rows<1>(a, cus, st) : a.M <= 32 ? launch_rows<2>(a, cus, st)
                    : a.M <= 64 ? launch_rows<4>(a, cus, st) : launch_rows<8>(a, cus, st);
     if (rc != MFD_OK) return rc;
