@@ -10,8 +10,9 @@
 // v_mfma_f32_32x32x16: only the last unit of a KV head is padded, whatever K L is. Scores are S^T = K Q^T in bf16 (a code
 // has four significant bits and the scale is a power of two, so k is exact in bf16 and every product in fp32) and
 // O^T += V^T P^T in fp16: V as bare codes (exact), P rounded to fp16 (2^-11 at most, an eighth of the bf16 output's own
-// rounding), the accumulators kept in units of the current page's v_scale and multiplied by the quotient of two scales,
-// a power of two, where the next 16 tokens have another one. Statistics are fp32.
+// rounding), times the quotient of the page's v_scale and the accumulators' unit: a power of two, which the exponential
+// takes along in its argument and the row sum leaves out again, both exactly. The accumulators are brought to another unit
+// only where that quotient leaves [2^-2, 2^6] (P stays below 2^14 and mostly above fp16's subnormals). Statistics are fp32.
 //
 // Two kernels, by the units of a KV head:
 //  * tile kernel: the waves of a workgroup (a unit each) share 64-key tiles. The codes come from memory to registers, two
@@ -24,6 +25,7 @@
 // Both split a context over workgroups (a fixed number of keys each, so that a batch's long contexts become more
 // workgroups, not longer ones) and merge by log-sum-exp.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_common.h"
 
@@ -34,7 +36,6 @@ using kv8::Pages;
 using kv8::u32x4;
 
 constexpr int TK = 64;         // keys per tile of the tile kernel
-constexpr int TILE = TK * D;   // 16-bit elements of a widened tile (16 KB)
 constexpr int UROWS = 32;      // query rows per unit
 constexpr int SK = 32;         // keys per tile of the stream kernel
 constexpr int SNW = 4;         // its waves
@@ -73,6 +74,12 @@ struct Args {
 };
 
 __device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+__device__ __forceinline__ void wait_vmcnt0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// One direct-to-LDS load: lane l's 16 bytes at g land at LDS byte address lds_byte + 16 l (lds_byte wave-uniform)
+__device__ __forceinline__ void dma16(const uint16_t* g, uint32_t lds_byte) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane(lds_byte);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(g) : "memory", "m0");
+}
 // Workgroup barrier that is also a compiler memory barrier, with this wave's LDS operations done. Global loads in
 // flight are not waited for: the next tiles' codes stay on their way across it.
 __device__ __forceinline__ void lds_barrier() {
@@ -122,37 +129,65 @@ __device__ __forceinline__ u32x4 widen_v(uint32_t c0, uint32_t c1) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c1, 1.f, false)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c1, 1.f, true))};
 }
-// A row's 16-byte chunks 2 part and 2 part + 1 into a widened tile ([key][d] rows of 256 bytes, chunk c of key r at
-// position c ^ swz). Parts 4 .. 7 write the upper one first: the eight lanes of a row then hit all banks at once.
-__device__ __forceinline__ void put_chunks(uint16_t* tile, int r, int part, int swz, const u32x4& first,
-                                           const u32x4& second) {
+// A widened tile in LDS is [key][d] with padded rows, so that every operand read is a lane's base plus a constant: K rows of
+// 272 bytes (16 lanes read 16 bytes of 16 rows: 16 bytes apart modulo 256, all banks once), V rows of 288 (the transpose
+// read takes 32 bytes of each of four rows: 32 bytes apart).
+constexpr int KROW = 272, VROW = 288;
+// 16-byte chunks 2 part and 2 part + 1 of a row. Parts 4 .. 7 write the upper one first: the eight lanes of a row then hit
+// all banks at once.
+__device__ __forceinline__ void put_chunks(uint8_t* row, int part, const u32x4& first, const u32x4& second) {
   const int c0 = 2 * part + (part >> 2);
-  *reinterpret_cast<u32x4*>(tile + (r * 16 + (c0 ^ swz)) * 8) = first;
-  *reinterpret_cast<u32x4*>(tile + (r * 16 + ((c0 ^ 1) ^ swz)) * 8) = second;
+  *reinterpret_cast<u32x4*>(row + 16 * c0) = first;
+  *reinterpret_cast<u32x4*>(row + 16 * (c0 ^ 1)) = second;
 }
-__device__ __forceinline__ void put_row(uint16_t* tile, int r, int part, int swz, const u32x4& lo, const u32x4& hi) {
+__device__ __forceinline__ void put_row(uint8_t* row, int part, const u32x4& lo, const u32x4& hi) {
   const bool up = part >= 4;
-  put_chunks(tile, r, part, swz, up ? hi : lo, up ? lo : hi);
+  put_chunks(row, part, up ? hi : lo, up ? lo : hi);
 }
-__device__ __forceinline__ void put_k_codes(uint16_t* tile, int r, int part, const u32x4& c, float s) {
+__device__ __forceinline__ void put_k_codes(uint8_t* row, int part, const u32x4& c, float s) {
   const bool up = part >= 4;
-  put_chunks(tile, r, part, r & 15, widen_k(up ? c[2] : c[0], up ? c[3] : c[1], s),
-             widen_k(up ? c[0] : c[2], up ? c[1] : c[3], s));
+  put_chunks(row, part, widen_k(up ? c[2] : c[0], up ? c[3] : c[1], s), widen_k(up ? c[0] : c[2], up ? c[1] : c[3], s));
 }
-__device__ __forceinline__ void put_v_codes(uint16_t* tile, int r, int part, const u32x4& c) {
+__device__ __forceinline__ void put_v_codes(uint8_t* row, int part, const u32x4& c) {
   const bool up = part >= 4;
-  put_chunks(tile, r, part, (r & 3) << 2, widen_v(up ? c[2] : c[0], up ? c[3] : c[1]),
-             widen_v(up ? c[0] : c[2], up ? c[1] : c[3]));
+  put_chunks(row, part, widen_v(up ? c[2] : c[0], up ? c[3] : c[1]), widen_v(up ? c[0] : c[2], up ? c[1] : c[3]));
+}
+// Byte offsets of a lane's operands within a tile. K: row l32 (+ 32 rows for the second subtile), d chunk 2 c + half: + 32 c.
+// V^T fragment of d block db and 16-key chunk c (ds_read_b64_tr_b16): + 64 db + 16 c rows, and eight rows further the chunk's
+// second 4-key group. The k order within a chunk is the row order of S^T's accumulators, so P needs no move.
+__device__ __forceinline__ int k_operand(int lane) { return (lane & 31) * KROW + (lane >> 5) * 16; }
+__device__ __forceinline__ int v_operand(int lane) {
+  const int sl = lane & 15;
+  return (4 * (lane >> 5) + (sl >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (sl & 3) * 8;
+}
+__device__ __forceinline__ u32x4 v_fragment(const uint8_t* p) {
+  const v4i16 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)p);
+  const v4i16 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p + 8 * VROW));
+  const v4i16 v[2] = {x0, x1};
+  return __builtin_bit_cast(u32x4, v);
 }
 // Row `slot` of a cache (ids and strides below 2^31: one 32 x 32 + 64 bit instruction)
 __device__ __forceinline__ const uint8_t* slot_row(const uint8_t* cache, int slot, uint32_t ss) {
   return cache + (uint64_t)(uint32_t)slot * ss;
 }
-__device__ __forceinline__ int k_swz(int r) { return r & 15; }
-__device__ __forceinline__ int v_swz(int r) { return (r & 3) << 2; }
 
-// Quotient a / b of two scales given as bits: powers of two
+// Quotient a / b of two scales given as bits: powers of two; and its logarithm
 __device__ __forceinline__ float scale_quotient(uint32_t a, uint32_t b) { return __uint_as_float(a - b + 0x3f800000u); }
+__device__ __forceinline__ int quotient_log2(uint32_t a, uint32_t b) { return (int)(a - b) >> 23; }
+// The accumulators' unit for values of scale vs (bits): kept while vs / unit is in [2^-2, 2^6], else a quarter of vs
+__device__ __forceinline__ uint32_t unit_for(uint32_t vs, uint32_t unit) {
+  const int q = quotient_log2(vs, unit);
+  return q < -2 || q > 6 ? vs - (2u << 23) : unit;
+}
+// The accumulators brought to unit `to` (wave-uniform)
+__device__ __forceinline__ void set_unit(uint32_t to, uint32_t& unit, f32x16 (&oacc)[D / 32]) {
+  if (to != unit) {
+    const float f = scale_quotient(unit, to);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
+    unit = to;
+  }
+}
 
 // Request of scheduling rank rho: requests by context length, longest first (ties by index), so that the longest
 // workgroups start first and short ones fill in behind them.
@@ -199,14 +234,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   static_assert(NW == 4 || NW == 8, "workgroups of 4 or 8 waves");
   constexpr int NPT = 8 / NW;   // 16-code pieces of a K or V tile per thread
   constexpr int RSTEP = NW * 8;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds_k[2 * TILE], lds_v[2 * TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t lds_k[2 * TK * KROW], lds_v[2 * TK * VROW];
   __shared__ uint32_t lds_vs[WHOLE ? 1 : 2 * TK];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
   const int KL = a.KL, Lb = a.L, rows = a.rows;
   const bool causal = a.causal != 0;
-  const float scale_log2 = a.scale_log2;
+  const float scale = a.scale_log2;
 
   // workgroup -> (request by rank, KV head, split, unit group); the unit groups that read the same keys are consecutive
   // on one XCD (workgroup id modulo 8) and share its L2
@@ -258,32 +293,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   f32x16 oacc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) oacc[db] = (f32x16){};
-  uint32_t vcur = 0x3f800000u;  // the accumulators' unit: bits of the page scale of the last 16 keys
+  uint32_t unit = 0x3f800000u;  // of the accumulators: bits of a power of two
 
-  // LDS offsets (elements) of the MFMA operands. K row 32 ks + l32, d chunk 2 c + half: (k_base ^ (c << 4)) + 4096 ks.
-  // V^T fragment of d block db and 16-key chunk c (ds_read_b64_tr_b16): (v_base ^ (db << 5)) + 2048 c, + 1024 for the
-  // chunk's second 4-key group. The k order within a chunk is the row order of S^T's accumulators, so P needs no move.
-  const int k_base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
-  int v_base;
-  {
-    const int grp = lane >> 4, sl = lane & 15, sw = sl >> 2;
-    v_base = (4 * half + sw) * 128 + (sw << 5) + (2 * (grp & 1) + ((sl & 3) >> 1)) * 8 + (sl & 1) * 4;
-  }
-  auto v_frag = [&](int off) __attribute__((always_inline)) {
-    const v4i16 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off));
-    const v4i16 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off + 1024));
-    const v4i16 v[2] = {x0, x1};
-    return __builtin_bit_cast(u32x4, v);
-  };
-  // S^T of the tile in K buffer j: keys 32 ks + 8 (x / 4) + 4 half + x % 4 (x: register), column = this lane's row
-  auto scores = [&](int j, f32x16 (&sv)[2]) __attribute__((always_inline)) {
-    const int kb = k_base + j * TILE;
+  const uint8_t* const kb = lds_k + k_operand(lane);
+  const uint8_t* const vb = lds_v + v_operand(lane);
+  // S^T of the tile in K buffer 0: keys 32 ks + 8 (x / 4) + 4 half + x % 4 (x: register), column = this lane's row
+  auto scores = [&](f32x16 (&sv)[2]) __attribute__((always_inline)) {
     sv[0] = sv[1] = (f32x16){};
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      const int off = kb ^ (c << 4);
-      const u16x8 k0f = *reinterpret_cast<const u16x8*>(lds_k + off);
-      const u16x8 k1f = *reinterpret_cast<const u16x8*>(lds_k + off + 32 * 128);
+      const u16x8 k0f = *reinterpret_cast<const u16x8*>(kb + 32 * c);
+      const u16x8 k1f = *reinterpret_cast<const u16x8*>(kb + 32 * c + 32 * KROW);
       sv[0] = mfma32(as_bf16x8(k0f), qf[c], sv[0]);
       sv[1] = mfma32(as_bf16x8(k1f), qf[c], sv[1]);
     }
@@ -305,7 +325,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int x = 0; x < 16; ++x) tmax = fmaxf(tmax, sv[ks][x]);
-    const float tm = half_max(tmax) * scale_log2;
+    const float tm = half_max(tmax) * scale;
     if (__builtin_amdgcn_ballot_w64(tm > m_run + 8.f) != 0) {
       const float m_new = fmaxf(m_run, tm);
       const float alpha = (m_run == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -342,7 +362,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       e[i] = ok ? x : 0;
     }
   };
-  auto load = [&](const uint8_t* cache, uint32_t ss, const float* scale, int t, const int (&e)[NE], u32x4 (&c)[NPT],
+  auto load = [&](const uint8_t* cache, uint32_t ss, const float* scales, int t, const int (&e)[NE], u32x4 (&c)[NPT],
                   float (&sc)[NE]) __attribute__((always_inline)) {
     if constexpr (WHOLE) {
       const int k0 = lo + t * TK;
@@ -358,23 +378,23 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
           c[i] = *reinterpret_cast<const u32x4*>(
               base + ((uint32_t)min(r0 + i * RSTEP, nv - 1) * ss + (uint32_t)part * 16));
       }
-      sc[0] = ((const_f32p)scale)[__builtin_amdgcn_readfirstlane(e[0] * Hkv)];
+      sc[0] = ((const_f32p)scales)[__builtin_amdgcn_readfirstlane(e[0] * Hkv)];
     } else {
 #pragma unroll
       for (int i = 0; i < NPT; ++i) {
         c[i] = *reinterpret_cast<const u32x4*>(slot_row(cache, (e[i] << shift) + (key_of(t, i) & pmask), ss) + part * 16);
-        sc[i] = scale[e[i] * Hkv];
+        sc[i] = scales[e[i] * Hkv];
       }
     }
   };
   auto put_k = [&](int j, const u32x4 (&c)[NPT], const float (&sc)[NE]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NPT; ++i) put_k_codes(lds_k + j * TILE, r0 + i * RSTEP, part, c[i], sc[WHOLE ? 0 : i]);
+    for (int i = 0; i < NPT; ++i) put_k_codes(lds_k + (j * TK + r0 + i * RSTEP) * KROW, part, c[i], sc[WHOLE ? 0 : i]);
   };
   auto put_v = [&](int j, const u32x4 (&c)[NPT], const float (&sc)[NE]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NPT; ++i) {
-      put_v_codes(lds_v + j * TILE, r0 + i * RSTEP, part, c[i]);
+      put_v_codes(lds_v + (j * TK + r0 + i * RSTEP) * VROW, part, c[i]);
       if constexpr (!WHOLE)
         if (part == 0) lds_vs[j * TK + r0 + i * RSTEP] = __float_as_uint(sc[i]);
     }
@@ -408,7 +428,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
     f32x16 s_a[2], s_b[2];
     lds_barrier();
-    scores(0, s_a);
+    scores(s_a);
     lds_barrier();  // every wave is done with K buffer 0
 
     // The 32 MFMAs of an iteration as a fixed sequence of slots: s < 8 is S^T subtile 0 of tile t + 1 (d chunk s), 8 .. 15
@@ -418,21 +438,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     constexpr int FD = 2;
     auto slot_is_qk = [](int sl) __attribute__((always_inline)) { return sl < 8 || (sl >= 16 && sl < 24); };
     auto chunk_of = [](int sl) __attribute__((always_inline)) { return sl < 12 ? 0 : sl < 16 ? 1 : sl < 28 ? 2 : 3; };
-    auto fetch = [&](int sl, int kb, int vb) __attribute__((always_inline)) {
+    // (j: the buffer of V(t); K(t + 1) is in the other one)
+    auto fetch = [&](int sl, int j) __attribute__((always_inline)) {
       if (slot_is_qk(sl))
-        return *reinterpret_cast<const u32x4*>(lds_k + ((kb ^ ((sl & 7) << 4)) + (sl >= 16 ? 32 * 128 : 0)));
-      return v_frag((vb ^ ((sl & 3) << 5)) + 2048 * chunk_of(sl));
+        return *reinterpret_cast<const u32x4*>(kb + (j ^ 1) * (TK * KROW) + 32 * (sl & 7) + (sl >= 16 ? 32 * KROW : 0));
+      return v_fragment(vb + j * (TK * VROW) + 64 * (sl & 3) + 16 * VROW * chunk_of(sl));
     };
-    auto set_unit = [&](uint32_t vsn) __attribute__((always_inline)) {
-      if (vsn != vcur) {
-        const float f = scale_quotient(vcur, vsn);
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
-        vcur = vsn;
-      }
-    };
-    auto iteration = [&](int t, f32x16 (&s_cur)[2], f32x16 (&s_nxt)[2]) __attribute__((always_inline)) {
-      const int j = t & 1;
+    auto iteration = [&](int t, auto parity, f32x16 (&s_cur)[2], f32x16 (&s_nxt)[2]) __attribute__((always_inline)) {
+      constexpr int j = decltype(parity)::value;  // t % 2: LDS addresses become constants
       put_k(j, kr, ksc);
       put_v(j ^ 1, vr, vsc);
       const uint32_t vs_next = __float_as_uint(vsc[0]);
@@ -446,40 +459,56 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       if (active) {
         const int khi = hi - (lo + t * TK);
         const float msub = softmax_max(khi < TK, 0, khi, s_cur);
-        const int kb = k_base + (j ^ 1) * TILE, vb = v_base + j * TILE;
-        if constexpr (WHOLE) set_unit(vs_t);
+        // each 16-key chunk's quotient of scale and unit: in the exponent, and out of the row sum
+        constexpr int NC = WHOLE ? 1 : 4;  // chunks with a scale of their own
+        float sub[NC], back[NC];
+        uint32_t units[NC];
+        {
+          uint32_t vs_l = vs_t;
+          if constexpr (!WHOLE) vs_l = lds_vs[j * TK + 16 * (lane & 3)];
+          uint32_t u = unit;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const uint32_t vs = WHOLE ? vs_t : (uint32_t)__builtin_amdgcn_readlane(vs_l, c);
+            u = unit_for(vs, u);
+            units[c] = u;
+            sub[c] = msub - (float)quotient_log2(vs, u);
+            back[c] = scale_quotient(u, vs);
+          }
+        }
         u32x4 opnd[32];
 #pragma unroll
-        for (int sl = 0; sl < FD; ++sl) opnd[sl] = fetch(sl, kb, vb);
-        uint32_t vs_l = 0;  // scales of the four 16-key chunks
-        if constexpr (!WHOLE) vs_l = lds_vs[j * TK + 16 * (lane & 3)];
+        for (int sl = 0; sl < FD; ++sl) opnd[sl] = fetch(sl, j);
         u32x4 pv[4];  // P^T B fragments (fp16 pairs) of the chunks
         float psum = 0.f;
         f32x16 acc0 = {}, acc1 = {};
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int sl = 0; sl < 32; ++sl) {
-          if constexpr (!WHOLE)
-            if (sl == 8 || sl == 12 || sl == 24 || sl == 28) set_unit(__builtin_amdgcn_readlane(vs_l, chunk_of(sl)));
-          if (sl + FD < 32) opnd[sl + FD] = fetch(sl + FD, kb, vb);
+          if (sl == 8 || (!WHOLE && (sl == 12 || sl == 24 || sl == 28))) set_unit(units[WHOLE ? 0 : chunk_of(sl)], unit, oacc);
+          if (sl + FD < 32) opnd[sl + FD] = fetch(sl + FD, j);
           if (slot_is_qk(sl)) {
             if (sl < 8) acc0 = mfma32(__builtin_bit_cast(bf16x8, opnd[sl]), qf[sl & 7], acc0);
             else acc1 = mfma32(__builtin_bit_cast(bf16x8, opnd[sl]), qf[sl & 7], acc1);
             // key pair y of chunk c: S^T registers x, x + 1 of subtile c / 2
             const int c = (sl < 8 ? 0 : 2) + ((sl & 7) >> 2), y = sl & 3;
             const int x = (c & 1) * 8 + 2 * y;
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[c >> 1][x], scale_log2, -msub));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[c >> 1][x + 1], scale_log2, -msub));
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[c >> 1][x], scale, -sub[WHOLE ? 0 : c]));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[c >> 1][x + 1], scale, -sub[WHOLE ? 0 : c]));
             psum += p0 + p1;
             asm volatile("" : "+v"(psum));  // keeps the add in this slot
             pv[c][y] = f2h2_bits(p0, p1);
+            if (!WHOLE && y == 3) {
+              l_run = __builtin_fmaf(psum, back[c], l_run);
+              psum = 0.f;
+            }
           } else {
             const int c = chunk_of(sl), db = sl & 3;
             oacc[db] = mfma32_f16(__builtin_bit_cast(f16x8, opnd[sl]), __builtin_bit_cast(f16x8, pv[c]), oacc[db]);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        l_run += psum;
+        if constexpr (WHOLE) l_run = __builtin_fmaf(psum, back[0], l_run);
         s_nxt[0] = acc0;
         s_nxt[1] = acc1;
       }
@@ -487,9 +516,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       lds_barrier();
     };
     for (int t = 0;;) {
-      iteration(t, s_a, s_b);
+      iteration(t, std::integral_constant<int, 0>{}, s_a, s_b);
       if (++t >= ntiles) break;
-      iteration(t, s_b, s_a);
+      iteration(t, std::integral_constant<int, 1>{}, s_b, s_a);
       if (++t >= ntiles) break;
     }
   }
@@ -504,10 +533,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       blo = (g0 % KL) / Lb * Lb;
       bhi = ((g1 % KL) / Lb + 1) * Lb;
     }
-    const float unit = __uint_as_float(vcur);
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) oacc[db] *= unit;
-    vcur = 0x3f800000u;
+    set_unit(0x3f800000u, unit, oacc);
     for (int b0 = blo; b0 < bhi; b0 += TK) {
       lds_barrier();  // every wave is done with the buffers
 #pragma unroll
@@ -517,14 +543,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const u32x4* kp = reinterpret_cast<const u32x4*>(a.kn + tk * a.kn_st + (int64_t)kvh * a.kn_sh + part * 16);
         const u32x4* vp = reinterpret_cast<const u32x4*>(a.vn + tk * a.vn_st + (int64_t)kvh * a.vn_sh + part * 16);
         const u32x4 kx = kp[0], ky = kp[1], vx = vp[0], vy = vp[1];
-        put_row(lds_k, rr, part, k_swz(rr), kx, ky);
-        put_row(lds_v, rr, part, v_swz(rr), vx, vy);
+        put_row(lds_k + rr * KROW, part, kx, ky);
+        put_row(lds_v + rr * VROW, part, vx, vy);
       }
       lds_barrier();
       const int klo = mode_lo - b0, khi = min(mode_lo + (causal ? qi - mode_lo + 1 : Lb), bhi) - b0;
       if (active && __builtin_amdgcn_ballot_w64(klo < TK && khi > 0) != 0) {
         f32x16 sv[2];
-        scores(0, sv);
+        scores(sv);
         const float msub = softmax_max(true, klo, khi, sv);
         float psum = 0.f;
 #pragma unroll
@@ -533,15 +559,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const int x = (c & 1) * 8 + 2 * y;
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c >> 1][x], scale_log2, -msub));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c >> 1][x + 1], scale_log2, -msub));
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c >> 1][x], scale, -msub));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c >> 1][x + 1], scale, -msub));
             psum += p0 + p1;
             ph[y] = f2bf2_bits(p0, p1);
             pl[y] = f2bf2_bits(p0 - __uint_as_float(ph[y] << 16), p1 - __uint_as_float(ph[y] & 0xffff0000u));
           }
 #pragma unroll
           for (int db = 0; db < D / 32; ++db) {
-            const bf16x8 vf = __builtin_bit_cast(bf16x8, v_frag((v_base ^ (db << 5)) + 2048 * c));
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, v_fragment(vb + 64 * db + 16 * VROW * c));
             oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, ph), oacc[db]);
             oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, pl), oacc[db]);
           }
@@ -554,7 +580,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if (!active) return;
 
   const float l_tot = half_sum(l_run);
-  const float inv = l_tot > 0.f ? __uint_as_float(vcur) / l_tot : (l_tot == 0.f ? 0.f : l_tot);  // (NaN stays NaN)
+  const float inv = l_tot > 0.f ? __uint_as_float(unit) / l_tot : (l_tot == 0.f ? 0.f : l_tot);  // (NaN stays NaN)
   const float lse2 = l_tot > 0.f ? m_run + __log2f(l_tot) : (l_tot == 0.f ? -INFINITY : l_tot);
   if (a.S == 1) {
     if (!row_ok) return;
@@ -600,14 +626,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // ---------------------------------------------------------------------------------------------- stream kernel
 
 __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attn_stream_kernel(Args a) {
-  constexpr int STILE = SK * D;  // elements of a widened 32-key tile (8 KB)
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[SNW * 2 * STILE];
+  constexpr int WLDS = SK * (KROW + VROW);  // bytes of a wave's widened K and V tile (17.5 KB)
+  static_assert(UROWS * D * 4 <= WLDS, "a wave's result fits its tiles");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[SNW * WLDS];
   __shared__ float lds_m[SNW][UROWS], lds_l[SNW][UROWS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
   const int KL = a.KL, Lb = a.L, rows = a.rows;
-  const float scale_log2 = a.scale_log2;
+  const float scale = a.scale_log2;
   const int s = blockIdx.x % a.S;
   const int kvh = (blockIdx.x / a.S) % a.Hkv;
   const int rho = blockIdx.x / a.S / a.Hkv;
@@ -633,32 +660,22 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) qf[c] = as_bf16x8(*reinterpret_cast<const u16x8*>(qp + c * 16));
   }
-  uint16_t* const lds_k = lds + w * 2 * STILE;
-  uint16_t* const lds_v = lds_k + STILE;
-  const int k_base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
-  int v_base;
-  {
-    const int grp = lane >> 4, sl = lane & 15, sw = sl >> 2;
-    v_base = (4 * half + sw) * 128 + (sw << 5) + (2 * (grp & 1) + ((sl & 3) >> 1)) * 8 + (sl & 1) * 4;
-  }
+  uint8_t* const lds_k = lds + w * WLDS;
+  uint8_t* const lds_v = lds_k + SK * KROW;
+  const uint8_t* const kb = lds_k + k_operand(lane);
+  const uint8_t* const vb = lds_v + v_operand(lane);
   float m_run = -INFINITY, l_run = 0.f;
   f32x16 oacc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) oacc[db] = (f32x16){};
-  uint32_t vcur = 0x3f800000u;
+  uint32_t unit = 0x3f800000u;  // of the accumulators: bits of a power of two
 
   auto scores = [&]() __attribute__((always_inline)) {
     f32x16 acc = {};
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
-      acc = mfma32(as_bf16x8(*reinterpret_cast<const u16x8*>(lds_k + (k_base ^ (c << 4)))), qf[c], acc);
+      acc = mfma32(as_bf16x8(*reinterpret_cast<const u16x8*>(kb + 32 * c)), qf[c], acc);
     return acc;
-  };
-  auto v_frag = [&](int off) __attribute__((always_inline)) {
-    const v4i16 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off));
-    const v4i16 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(lds_v + off + 1024));
-    const v4i16 v[2] = {x0, x1};
-    return __builtin_bit_cast(u32x4, v);
   };
   // register x of a 32-key score tile is key 8 (x / 4) + 4 half + x % 4
   auto softmax_max = [&](bool masked, int klo, int khi, f32x16& sv) __attribute__((always_inline)) {
@@ -672,7 +689,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
     float tmax = -INFINITY;
 #pragma unroll
     for (int x = 0; x < 16; ++x) tmax = fmaxf(tmax, sv[x]);
-    const float tm = half_max(tmax) * scale_log2;
+    const float tm = half_max(tmax) * scale;
     if (__builtin_amdgcn_ballot_w64(tm > m_run + 8.f) != 0) {
       const float m_new = fmaxf(m_run, tm);
       const float alpha = (m_run == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -726,8 +743,8 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       // (a wave's LDS operations complete in order: nothing of the last tile is still to be read)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        put_k_codes(lds_k, r0 + 8 * i, part, kr[i], ksc[i]);
-        put_v_codes(lds_v, r0 + 8 * i, part, vr[i]);
+        put_k_codes(lds_k + (r0 + 8 * i) * KROW, part, kr[i], ksc[i]);
+        put_v_codes(lds_v + (r0 + 8 * i) * VROW, part, vr[i]);
       }
       const uint32_t vs_t[2] = {(uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(vsc[0])),
                                 (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(vsc[2]))};
@@ -742,39 +759,32 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       f32x16 sv = scores();
       const int khi = hi - (lo + t * SK);
       const float msub = softmax_max(khi < SK, 0, khi, sv);
-      float psum = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        set_unit(unit_for(vs_t[c], unit), unit, oacc);
+        const float sub = msub - (float)quotient_log2(vs_t[c], unit);
         u32x4 pv;
+        float psum = 0.f;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y], scale_log2, -msub));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y + 1], scale_log2, -msub));
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y], scale, -sub));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y + 1], scale, -sub));
           psum += p0 + p1;
           pv[y] = f2h2_bits(p0, p1);
         }
-        if (vs_t[c] != vcur) {
-          const float f = scale_quotient(vcur, vs_t[c]);
-#pragma unroll
-          for (int db = 0; db < D / 32; ++db) oacc[db] *= f;
-          vcur = vs_t[c];
-        }
+        l_run = __builtin_fmaf(psum, scale_quotient(unit, vs_t[c]), l_run);
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
-          oacc[db] = mfma32_f16(__builtin_bit_cast(f16x8, v_frag((v_base ^ (db << 5)) + 2048 * c)),
+          oacc[db] = mfma32_f16(__builtin_bit_cast(f16x8, v_fragment(vb + 64 * db + 16 * VROW * c)),
                                 __builtin_bit_cast(f16x8, pv), oacc[db]);
       }
-      l_run += psum;
       asm volatile("" ::: "memory");
     }
   }
   if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   // ---- the block keys (rows <= 32, so K L <= 32: one tile), in bf16 with P as a bf16 pair, by the last wave
   if (with_block && w == SNW - 1) {
-    const float unit = __uint_as_float(vcur);
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) oacc[db] *= unit;
-    vcur = 0x3f800000u;
+    set_unit(0x3f800000u, unit, oacc);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int rr = r0 + 8 * i;
@@ -782,8 +792,8 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       const u32x4* kp = reinterpret_cast<const u32x4*>(a.kn + tk * a.kn_st + (int64_t)kvh * a.kn_sh + part * 16);
       const u32x4* vp = reinterpret_cast<const u32x4*>(a.vn + tk * a.vn_st + (int64_t)kvh * a.vn_sh + part * 16);
       const u32x4 kx = kp[0], ky = kp[1], vx = vp[0], vy = vp[1];
-      put_row(lds_k, rr, part, k_swz(rr), kx, ky);
-      put_row(lds_v, rr, part, v_swz(rr), vx, vy);
+      put_row(lds_k + rr * KROW, part, kx, ky);
+      put_row(lds_v + rr * VROW, part, vx, vy);
     }
     asm volatile("" ::: "memory");
     f32x16 sv = scores();
@@ -794,15 +804,15 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       u32x4 ph, pl;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y], scale_log2, -msub));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y + 1], scale_log2, -msub));
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y], scale, -msub));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[8 * c + 2 * y + 1], scale, -msub));
         psum += p0 + p1;
         ph[y] = f2bf2_bits(p0, p1);
         pl[y] = f2bf2_bits(p0 - __uint_as_float(ph[y] << 16), p1 - __uint_as_float(ph[y] & 0xffff0000u));
       }
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) {
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, v_frag((v_base ^ (db << 5)) + 2048 * c));
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, v_fragment(vb + 64 * db + 16 * VROW * c));
         oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, ph), oacc[db]);
         oacc[db] = mfma32(vf, __builtin_bit_cast(bf16x8, pl), oacc[db]);
       }
@@ -820,8 +830,8 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   float m_tot = lds_m[0][l32];
 #pragma unroll
   for (int x = 1; x < SNW; ++x) m_tot = fmaxf(m_tot, lds_m[x][l32]);
-  const float fac = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_tot) * __uint_as_float(vcur);
-  float* const own = reinterpret_cast<float*>(lds) + w * (UROWS * D);
+  const float fac = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_tot) * __uint_as_float(unit);
+  float* const own = reinterpret_cast<float*>(lds + w * WLDS);
   // 16-byte piece c of row r at c ^ r, so that the lanes of a write or a read spread over the banks
   if (w < ntiles || (with_block && w == SNW - 1)) {
 #pragma unroll
@@ -847,7 +857,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
     lt += mw == -INFINITY ? (lds_l[x][row] == 0.f ? 0.f : lds_l[x][row]) : lds_l[x][row] * __builtin_amdgcn_exp2f(mw - mt);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      o[c] += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + x * (UROWS * D) + row * D +
+      o[c] += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WLDS) + row * D +
                                               (((4 * (tid & 7) + c) ^ row) & 31) * 4);
   }
   if (row >= rows) return;  // (whole groups of eight threads)
@@ -964,6 +974,7 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
 constexpr int WNW = 4;
 constexpr int WKEYS = WNW * TK;
 constexpr int WOCC = 3;  // waves per SIMD
+constexpr int QS = 2;    // units per stage of query rows
 
 struct WArgs {
   const uint16_t* q;
@@ -983,56 +994,63 @@ struct WArgs {
 };
 
 __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, WOCC))) void kv8_weights_kernel(WArgs a) {
-  // 32 keys of each wave at a time first, then two Q units of 8 KB
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[WNW * SK * D];
-  __shared__ float lds_lse[2][UROWS];
+  // 32 keys of each wave at a time first, then two stages of query rows
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[WNW * SK * KROW];
+  static_assert(2 * QS * UROWS * D * 2 <= WNW * SK * KROW, "two stages fit");
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  // KV heads fastest, key ranges slowest: with eight heads each XCD (workgroup id modulo 8) has one, whose query rows stay in
+  // its L2, and ranges that only the longest requests reach are spread over all of them
+  const int kvh = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv % a.bs, range = blockIdx.x / a.Hkv / a.bs;
   const int32_t* trow = kv8::table_row(a.pages, b);
   const int64_t wrow = a.pages.req_idx ? a.pages.req_idx[b] : b;
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1;
   int ctx = trow && a.pages.num_pages > 0 && wrow < a.w_rows ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0;
-  if (tid == 0 && blockIdx.x == 0 && kvh == 0 && (ctx > a.width || ctx != a.ctx_lens[b]))
+  if (tid == 0 && range == 0 && kvh == 0 && (ctx > a.width || ctx != a.ctx_lens[b]))
     kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   ctx = __builtin_amdgcn_readfirstlane(min(ctx, a.width));
-  const int lo = blockIdx.x * WKEYS;
+  const int lo = range * WKEYS;
   if (lo >= ctx) return;
 
-  // Q unit u: row tid / 8 of 32, 16 elements tid % 8. A row's lse in base 2; padding rows and rows whose lse is -inf
-  // (they saw no key) get +inf: their probabilities are 0.
-  const int units = (a.rows + UROWS - 1) / UROWS;
-  const int qr = tid >> 3, qpart = tid & 7;
-  const int dg = UROWS / a.KL, dq = UROWS % a.KL;
+  // Query rows come by direct-to-LDS loads, QS units (64 rows, 16 KB) at a time, double buffered. A load moves four whole
+  // rows: load i of wave w takes rows 16 i + 4 w + lane / 16 of the stage, and chunk c of row r lands at c ^ (r % 16) of
+  // the row (the lane at position p asks for chunk p ^ (r % 16)). Rows past the last repeat the first.
+  const int stages = (a.rows + QS * UROWS - 1) / (QS * UROWS);
+  const int qr = 4 * w + (lane >> 4);
+  const int dg = 16 / a.KL, dq = 16 % a.KL;
   const int64_t q_step = dg * a.q_sh + dq * a.q_st, q_wrap = a.q_sh - a.KL * a.q_st;
-  const int64_t l_step = dg + (int64_t)dq * a.H, l_wrap = 1 - (int64_t)a.KL * a.H;
-  int rr = qr, rq = qr % a.KL;  // the next unit's row and its query (padding rows repeat the first row)
-  const uint16_t* const q_first = a.q + (int64_t)b * a.KL * a.q_st + (int64_t)kvh * a.G * a.q_sh + qpart * 16;
-  const float* const l_first = a.lse + (int64_t)b * a.KL * a.H + kvh * a.G;
+  int rr = qr, rq = qr % a.KL;  // the next load's row, and its query
+  const uint16_t* const q_first =
+      a.q + (int64_t)b * a.KL * a.q_st + (int64_t)kvh * a.G * a.q_sh + ((lane & 15) ^ (qr & 15)) * 8;
   const uint16_t* qp = q_first + (qr / a.KL) * a.q_sh + rq * a.q_st;
-  const float* lp = l_first + qr / a.KL + (int64_t)rq * a.H;
-  u32x4 qx, qy;
-  float ql = 0.f;
-  bool q_ok = false;
-  auto load_q = [&]() __attribute__((always_inline)) {
-    q_ok = rr < a.rows;
-    const u32x4* p = reinterpret_cast<const u32x4*>(q_ok ? qp : q_first);
-    qx = p[0];
-    qy = p[1];
-    ql = *(q_ok ? lp : l_first);
-    rr += UROWS;
-    rq += dq;
-    const bool wrap = rq >= a.KL;
-    rq -= wrap ? a.KL : 0;
-    qp += q_step + (wrap ? q_wrap : 0);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  auto load_q = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2 * QS; ++i) {
+      dma16(rr < a.rows ? qp : q_first, lds0 + (uint32_t)(j * QS * UROWS + 16 * i + 4 * w) * (D * 2));
+      rr += 16;
+      rq += dq;
+      const bool wrap = rq >= a.KL;
+      rq -= wrap ? a.KL : 0;
+      qp += q_step + (wrap ? q_wrap : 0);
+    }
+  };
+  // lse of row l32 of the next unit; padding rows get +inf (probability 0), and so do rows whose lse is -inf (they saw no key)
+  const int lg = UROWS / a.KL, lq = UROWS % a.KL;
+  const int64_t l_step = lg + (int64_t)lq * a.H, l_wrap = 1 - (int64_t)a.KL * a.H;
+  int lr = l32, lrq = l32 % a.KL;
+  const float* lp = a.lse + ((int64_t)b * a.KL + lrq) * a.H + kvh * a.G + l32 / a.KL;
+  auto load_lse = [&]() __attribute__((always_inline)) {
+    float l = INFINITY;
+    if (lr < a.rows) l = *lp;
+    lr += UROWS;
+    lrq += lq;
+    const bool wrap = lrq >= a.KL;
+    lrq -= wrap ? a.KL : 0;
     lp += l_step + (wrap ? l_wrap : 0);
+    return l;
   };
-  auto put_q = [&](int j) __attribute__((always_inline)) {
-    put_row(lds + j * (UROWS * D), qr, qpart, k_swz(qr), qx, qy);
-    if (qpart == 0) lds_lse[j][qr] = q_ok && ql != -INFINITY ? ql * 1.4426950408889634f : INFINITY;
-  };
-  load_q();
 
   // keys of this wave: 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i, 32 rows through LDS at a time
   const int base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
@@ -1040,7 +1058,7 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, 
   {
     const int r0 = lane >> 3, part = lane & 7;
     const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh + part * 16;
-    uint16_t* tile = lds + w * (SK * D);
+    uint8_t* tile = lds + w * (SK * KROW);
     int bad = 0;
     int e[8];
     u32x4 c[8];
@@ -1064,11 +1082,11 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, 
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) put_k_codes(tile, r0 + 8 * i, part, c[4 * ks + i], sc[4 * ks + i]);
+      for (int i = 0; i < 4; ++i) put_k_codes(tile + (r0 + 8 * i) * KROW, part, c[4 * ks + i], sc[4 * ks + i]);
       asm volatile("" ::: "memory");  // (a wave's LDS operations complete in order)
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
-        kf[ks][d] = as_bf16x8(*reinterpret_cast<const u16x8*>(tile + (base ^ (d << 4))));
+        kf[ks][d] = as_bf16x8(*reinterpret_cast<const u16x8*>(tile + k_operand(lane) + 32 * d));
       asm volatile("" ::: "memory");
     }
   }
@@ -1076,30 +1094,32 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, 
   float acc[32];
 #pragma unroll
   for (int x = 0; x < 32; ++x) acc[x] = 0.f;
-  put_q(0);
-  if (units > 1) load_q();
+  load_q(0);
+  float l_nxt = load_lse();
+  wait_vmcnt0();
   lds_barrier();
-  for (int u = 0; u < units; ++u) {
-    const int j = u & 1;
-    if (u + 1 < units) {  // buffer j ^ 1 was last read in iteration u - 1
-      put_q(j ^ 1);
-      if (u + 2 < units) load_q();
-    }
-    const uint16_t* qb = lds + j * (UROWS * D);
-    f32x16 s0 = {}, s1 = {};
+  for (int st = 0; st < stages; ++st) {
+    if (st + 1 < stages) load_q((st + 1) & 1);  // (that buffer was last read in stage st - 1)
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const bf16x8 qf = as_bf16x8(*reinterpret_cast<const u16x8*>(qb + (base ^ (c << 4))));
-      s0 = mfma32(kf[0][c], qf, s0);
-      s1 = mfma32(kf[1][c], qf, s1);
+    for (int x = 0; x < QS; ++x) {
+      const uint16_t* qb = reinterpret_cast<const uint16_t*>(lds) + ((st & 1) * QS + x) * (UROWS * D);
+      const float l = l_nxt == -INFINITY ? INFINITY : l_nxt * 1.4426950408889634f;
+      l_nxt = load_lse();
+      f32x16 s0 = {}, s1 = {};
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        const bf16x8 qf = as_bf16x8(*reinterpret_cast<const u16x8*>(qb + (base ^ (c << 4))));
+        s0 = mfma32(kf[0][c], qf, s0);
+        s1 = mfma32(kf[1][c], qf, s1);
+      }
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        acc[y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[y], a.scale_log2, -l));
+        acc[16 + y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[y], a.scale_log2, -l));
+      }
     }
-    const float l = lds_lse[j][l32];
+    wait_vmcnt0();
     lds_barrier();
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      acc[x] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[x], a.scale_log2, -l));
-      acc[16 + x] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[x], a.scale_log2, -l));
-    }
   }
   // Sum over the 32 lanes of a half, halving the registers as the lanes are joined: in step m a lane keeps the half of its
   // registers that its bit m names and gives the other half to lane ^ m. Register x ends in the lane whose bits 4 .. 0
@@ -1251,8 +1271,9 @@ extern "C" int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, co
   a.decay = decay;
   a.err_flag = err_flag;
   const int64_t keys = std::min<int64_t>(width, (int64_t)table_width * page_size);
-  const dim3 grid((unsigned)((keys + WKEYS - 1) / WKEYS), (unsigned)Hkv, (unsigned)bs);
-  hipLaunchKernelGGL(kv8_weights_kernel, grid, dim3(WNW * 64), 0, static_cast<hipStream_t>(stream), a);
+  const int64_t grid = (keys + WKEYS - 1) / WKEYS * Hkv * bs;
+  if (grid > 0x7fffffff) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
+  hipLaunchKernelGGL(kv8_weights_kernel, dim3((unsigned)grid), dim3(WNW * 64), 0, static_cast<hipStream_t>(stream), a);
   MFD_CHECK_LAUNCH();
   return MFD_OK;
 }

@@ -16,6 +16,7 @@
 //    its four waves every fourth step of k; the drafted rows come from L2 straight to registers, the partial sums meet in
 //    LDS and are added in wave order.
 #include <algorithm>
+#include <type_traits>
 
 #include "mfd_common.h"
 
@@ -52,6 +53,8 @@ __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Workgroup barrier that is also a compiler memory barrier, with this wave's LDS operations done; loads in flight go on
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), (short)0, (int)bytes, 0x00020000);
 }
@@ -60,6 +63,8 @@ __device__ __forceinline__ const uint16_t* drafted_row(const HeadArgs& a, int r)
   const int m = a.row0 + min(r, a.M - 1);  // rows past the last repeat it and are not stored
   return a.x + (int64_t)(m / a.rpg) * a.group_stride + (int64_t)(m % a.rpg) * a.row_stride;
 }
+// An operand read takes chunk 4 g4 + j of 16 rows: four rows apart the low bits differ, within four the high ones
+__device__ __forceinline__ int swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
 // First vocabulary row of workgroup g: an even split, in multiples of 8 rows
 __host__ __device__ __forceinline__ int wg_row0(int g, int N, int nwg) {
   return g >= nwg ? N : (int)(((int64_t)g * N / nwg) & ~(int64_t)7);
@@ -91,20 +96,19 @@ __device__ __forceinline__ void store4(uint16_t* orow, int n, int rows, const f3
 template <int MTL>
 struct Wide {
   static constexpr int BLOCK = (MTL <= 2 ? 32 : 64) * 1024;  // bytes of a drafted-row block
-  static constexpr int HPS = MTL == 8 ? 1 : 2;   // 128-k halves per step
   static constexpr int WPC = MTL <= 2 ? 2 : 1;   // workgroups per CU
-  static constexpr int VT_MAX = MTL <= 2 ? 3 : 5;
+  static constexpr int VT_MAX = MTL == 4 ? 5 : 3;
 };
 
 template <int VT, int MTL>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2 * Wide<MTL>::WPC, 2 * Wide<MTL>::WPC)))
 void mxfp4_wide_kernel(HeadArgs a) {
-  constexpr int BLOCK = Wide<MTL>::BLOCK, HPS = Wide<MTL>::HPS;
+  constexpr int BLOCK = Wide<MTL>::BLOCK, HPS = 2;  // 128-k halves per step
   constexpr int HB = BLOCK / (32 * MTL);  // k per drafted block
   constexpr int CPR = HB / 8;             // 16-byte chunks of a row's block
   constexpr int SPB = HB / (KS * HPS);    // steps per block
   constexpr int LPW = BLOCK / 1024 / NW;  // direct loads of a wave per block
-  static_assert(SPB % 2 == 0, "steps go in pairs");
+  static_assert(SPB == 1 || SPB % 2 == 0, "steps go in pairs");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -115,101 +119,121 @@ void mxfp4_wide_kernel(HeadArgs a) {
   const int l16 = lane & 15, g4 = lane >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
 
-  // chunk c of drafted row r sits at c ^ (r & 15) of the row's block, so that the 16 rows of an operand read hit all
-  // banks; chunks past the last k repeat the last one and are never read
+  // direct loads of drafted block b: chunk c of row r goes to c ^ swz(r) of the row's block, so that the lanes of an operand read hit all banks;
+  // chunks past the last k repeat the last one and are never read
   auto issue_x = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
       const int at = (i * NW + w) * 64 + lane;
-      const int r = at / CPR, c = (at % CPR) ^ (r & 15);
+      const int r = at / CPR, c = (at % CPR) ^ swz(r);
       dma16(drafted_row(a, r) + min(b * HB + 8 * c, K - 8), lds0 + (uint32_t)(b & 1) * BLOCK + (uint32_t)(i * NW + w) * 1024u);
     }
   };
-  // this wave's tiles t0 .. t0 + vtv - 1; past them it loads (but does not multiply) the last one again, so that the number
-  // of its loads is known. Rows past the range read as zero by the buffers' bounds.
+  // this wave's tiles: t0 .. t0 + VT - 1 or t0 + VT - 2 (an even split of at most 8 VT tiles, and more than 8 (VT - 1)
+  // rows' worth of them up to the range's rounding), the loop compiled for either: a test per product would cost more
+  // than the product. Rows past the range read as zero by the buffers' bounds.
   const int T = (rows + 15) / 16;
   const int t0 = __builtin_amdgcn_readfirstlane(w * T / NW);
   const int vtv = __builtin_amdgcn_readfirstlane((w + 1) * T / NW) - t0;
   const __amdgpu_buffer_rsrc_t rc = buffer_of(a.codes + (int64_t)R0 * (K / 2), (uint32_t)rows * (uint32_t)(K / 2));
   const __amdgpu_buffer_rsrc_t re = buffer_of(a.exps + (int64_t)R0 * (K / 32), (uint32_t)rows * (uint32_t)(K / 32));
-  const uint32_t coff = (uint32_t)(16 * min(t0, T - 1) + l16) * (uint32_t)(K / 2) + 16u * g4;
-  const uint32_t eoff = (uint32_t)(16 * min(t0, T - 1) + l16) * (uint32_t)(K / 32);
-  f32x4 acc[VT][MTL];
+  const uint32_t coff = (uint32_t)(16 * t0 + l16) * (uint32_t)(K / 2) + 16u * g4;
+  const uint32_t eoff = (uint32_t)(16 * t0 + l16) * (uint32_t)(K / 32);
+  auto walk = [&](auto tiles) __attribute__((always_inline)) {
+    constexpr int V = decltype(tiles)::value;
+    f32x4 acc[V + 1][MTL];
 #pragma unroll
-  for (int i = 0; i < VT; ++i)
+    for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int j = 0; j < MTL; ++j) acc[i][j] = (f32x4){};
-  u32x4 wf[2][VT][HPS];
-  uint32_t ef[2][VT][HPS];
-  auto load_w = [&](int p, int v) __attribute__((always_inline)) {
-    const uint32_t u = (uint32_t)min(v, S - 1);
+      for (int j = 0; j < MTL; ++j) acc[i][j] = (f32x4){};
+    u32x4 wf[2][V + 1][HPS];
+    u32x2 ef[2][V + 1];
+    // (past the last step: the last one, not used. The scheduler leaves a step's loads where they are: sunk to the next
+    // step's, they would be waited for together.)
+    auto load_w = [&](int p, int v) __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t u = (uint32_t)min(v, S - 1);
 #pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      const uint32_t tile = (uint32_t)min(i, max(vtv - 1, 0));
-      const uint32_t cs = tile * (uint32_t)(8 * K) + u * (64u * HPS), es = tile * (uint32_t)(K / 2) + u * (4u * HPS);
+      for (int i = 0; i < V; ++i) {
+        ef[p][i] = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_raw_buffer_load_b64(re, eoff, (uint32_t)i * (uint32_t)(K / 2) + u * (4u * HPS), 0));
 #pragma unroll
-      for (int h = 0; h < HPS; ++h)
-        wf[p][i][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, coff, cs + 64u * h, 0));
-      if constexpr (HPS == 1) {
-        ef[p][i][0] = __builtin_amdgcn_raw_buffer_load_b32(re, eoff, es, 0);
-      } else {
-        const u32x2 e = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(re, eoff, es, 0));
-        ef[p][i][0] = e[0];
-        ef[p][i][HPS - 1] = e[1];
+        for (int h = 0; h < HPS; ++h)
+          wf[p][i][h] = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, coff, (uint32_t)i * (uint32_t)(8 * K) + u * (64u * HPS) + 64u * h, 0));
       }
-    }
-  };
-  auto step = [&](int p, int v) __attribute__((always_inline)) {
-    const uint8_t* base = smem + ((v / SPB) & 1) * BLOCK + l16 * (HB * 2);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // A step's products in slots of V MFMAs: slot q is drafted tile q % MTL of the half's k chunk q / MTL. The drafted
+    // operand is read FD slots ahead (left alone, the compiler reads it just before its products), and a chunk's weights
+    // are widened in the slot before its first. A scheduling barrier closes each slot.
+    constexpr int FD = MTL <= 2 ? 2 : 4;
+    auto step = [&](int p, int v) __attribute__((always_inline)) {
+      const uint8_t* base = smem + ((v / SPB) & 1) * BLOCK + l16 * (HB * 2);
 #pragma unroll
-    for (int h = 0; h < HPS; ++h) {
-      if (h > 0 && (v * HPS + h) * KS >= K) break;  // K is an odd number of halves
-      const int c0 = ((v % SPB) * HPS + h) * (KS / 8) + 4 * g4;
+      for (int h = 0; h < HPS; ++h) {
+        if (h > 0 && (v * HPS + h) * KS >= K) break;  // K is an odd number of halves
+        const int c0 = ((v % SPB) * HPS + h) * (KS / 8) + 4 * g4;
+        auto fetch = [&](int q) __attribute__((always_inline)) {
+          return *reinterpret_cast<const bf16x8*>(base + 16 * (q % MTL) * (HB * 2) + (((c0 + q / MTL) ^ swz(l16)) << 4));
+        };
+        float sc[V + 1];
+        bf16x8 f[2][V + 1], xf[4 * MTL];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 f[VT];
+        for (int i = 0; i < V; ++i) sc[i] = scale_of(ef[p][i][h], g4);
 #pragma unroll
-        for (int i = 0; i < VT; ++i) f[i] = widen(wf[p][i][h][j], scale_of(ef[p][i][h], g4));
+        for (int q = 0; q < FD; ++q) xf[q] = fetch(q);
 #pragma unroll
-        for (int m = 0; m < MTL; ++m) {
-          const bf16x8 xf = *reinterpret_cast<const bf16x8*>(base + 16 * m * (HB * 2) + (((c0 + j) ^ l16) << 4));
+        for (int i = 0; i < V; ++i) f[0][i] = widen(wf[p][i][h][0], sc[i]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < VT; ++i) {
-            if (i >= vtv) break;
-            acc[i][m] = mfma16(f[i], xf, acc[i][m]);
+        for (int q = 0; q < 4 * MTL; ++q) {
+          const int j = q / MTL, m = q % MTL;
+          if (q + FD < 4 * MTL) xf[q + FD] = fetch(q + FD);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i][m] = mfma16(f[j & 1][i], xf[q], acc[i][m]);
+          if (m == MTL - 1 && j < 3) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[(j + 1) & 1][i] = widen(wf[p][i][h][j + 1], sc[i]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-    }
-  };
-  issue_x(0);
-  load_w(0, 0);
-  load_w(1, 1);
-  for (int b = 0; b * SPB < S; ++b) {
-    // the block's direct loads have landed: the weight loads of two steps, VT (HPS + 1) each, are younger
-    wait_vmcnt<2 * VT * (HPS + 1)>();
-    __syncthreads();  // in every wave; and block b - 1 is read, so its half is free
-    if ((b + 1) * SPB < S) issue_x(b + 1);
-    const int end = min((b + 1) * SPB, S);
+    };
+    // Block b's direct loads have landed in every wave (the weight loads of one or two steps, V (HPS + 1) each, are
+    // younger), block b - 1 is read, and its half takes block b + 1.
+    auto next_block = [&](int b) __attribute__((always_inline)) {
+      wait_vmcnt<(SPB == 1 ? 1 : 2) * V * (HPS + 1)>();
+      lds_barrier();
+      if ((b + 1) * SPB < S) issue_x(b + 1);
+    };
+    issue_x(0);
+    load_w(0, 0);
+    load_w(1, 1);
 #pragma unroll 1
-    for (int v = b * SPB; v < end; v += 2) {
+    for (int v = 0; v < S; v += 2) {
+      if (SPB <= 2 || v % SPB == 0) next_block(v / SPB);
       step(0, v);
       load_w(0, v + 2);
-      if (v + 1 < end) step(1, v + 1);
+      if (v + 1 < S) {
+        if (SPB == 1) next_block(v + 1);
+        step(1, v + 1);
+      }
       load_w(1, v + 3);
     }
-  }
-  wait_vmcnt<0>();
-  // C register r of accumulator (i, m): weight row 16 (t0 + i) + 4 g4 + r of the range, drafted row 16 m + l16
+    wait_vmcnt<0>();
+    // C register r of accumulator (i, m): weight row 16 (t0 + i) + 4 g4 + r of the range, drafted row 16 m + l16
 #pragma unroll
-  for (int m = 0; m < MTL; ++m) {
-    const int mm = 16 * m + l16;
-    if (mm >= a.M) continue;
-    uint16_t* orow = a.out + (int64_t)mm * a.out_stride + R0;
+    for (int m = 0; m < MTL; ++m) {
+      const int mm = 16 * m + l16;
+      if (mm >= a.M) continue;
+      uint16_t* orow = a.out + (int64_t)mm * a.out_stride + R0;
 #pragma unroll
-    for (int i = 0; i < VT; ++i)
-      if (i < vtv) store4(orow, 16 * (t0 + i) + 4 * g4, rows, acc[i][m]);
-  }
+      for (int i = 0; i < V; ++i) store4(orow, 16 * (t0 + i) + 4 * g4, rows, acc[i][m]);
+    }
+  };
+  if (vtv == VT) walk(std::integral_constant<int, VT>{});
+  else walk(std::integral_constant<int, VT - 1>{});
 }
 
 template <int VT, int MTL>

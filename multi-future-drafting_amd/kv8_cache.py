@@ -131,14 +131,16 @@ def kv8_store(*, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
 
 
 def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int, device) -> tuple[int, int]:
-    """(num_ctx_splits, split_keys) for num_ctx_splits < 0: contexts split until one round of workgroup slots is full, with
-    at least 256 keys in a split."""
+    """(num_ctx_splits, split_keys) for num_ctx_splits < 0: enough parts of the longest context for two rounds of workgroup
+    slots if all were as long (contexts of a batch differ, and short workgroups behind long ones even that out), of at least
+    256 keys each."""
     units = -(-rows // UNIT)
     waves = 8 if units % 8 == 0 else 4
     slots = mfd_hip.cu_count(device) * (1 if units > 1 and waves == 8 else 2)
-    programs = bs * heads * -(-units // waves)
-    splits = slots // max(1, programs)
-    if with_block and units > 1:
+    programs = max(1, bs * heads * -(-units // waves))
+    want = slots * (1 if bs == 1 else 2)
+    splits = want // programs if bs == 1 else -(-want // programs)
+    if bs == 1 and with_block and units > 1:
         splits -= 1
     splits = min(splits, -(-max_ctx // 256), 64)
     if splits <= 1:
