@@ -210,6 +210,16 @@ __device__ __forceinline__ int request_of_rank(const int64_t* ctx_lens, int bs, 
   return rho;
 }
 
+// Program p of bs Hkv S: (split, KV head, rank of the request). KV heads fastest: with eight of them each XCD (workgroup id
+// modulo 8) has one, and with fewer the turn of the splits with the rank keeps a split from meeting the same XCDs in every
+// request (short requests have only the first splits: a fixed pairing of splits and XCDs measured 462 us against 276).
+__device__ __forceinline__ void program_of(const Args& a, int p, int& s, int& kvh, int& rho) {
+  kvh = p % a.Hkv;
+  const int q = p / a.Hkv;
+  rho = q / a.S;
+  s = (q + rho) % a.S;
+}
+
 // The keys [lo, hi) of context split s
 __device__ __forceinline__ void split_range(const Args& a, int s, int ctx, int& lo, int& hi) {
   lo = 0;
@@ -227,8 +237,8 @@ __device__ __forceinline__ int64_t partial_row(const Args& a, int s, int b, int 
 
 // ------------------------------------------------------------------------------------------------ tile kernel
 
-// WHOLE: pages of at least 64 tokens, so that a tile lies in one page: its page id, address and scales are wave-uniform,
-// come by scalar loads and live in scalar registers. Else each thread looks up its own keys' pages.
+// WHOLE: pages of at least 64 tokens, so that a tile lies in one page: its page id, address and scales are wave-uniform. Else
+// each thread looks up its own keys' pages.
 template <int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attn_tile_kernel(Args a) {
   static_assert(NW == 4 || NW == 8, "workgroups of 4 or 8 waves");
@@ -243,16 +253,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const bool causal = a.causal != 0;
   const float scale = a.scale_log2;
 
-  // workgroup -> (request by rank, KV head, split, unit group); the unit groups that read the same keys are consecutive
-  // on one XCD (workgroup id modulo 8) and share its L2
+  // workgroup -> (program, unit group); the unit groups of a program read the same keys: consecutive on one XCD (workgroup
+  // id modulo 8), they share its L2
   const int P = a.bs * a.Hkv * a.S;
   const int jx = blockIdx.x >> 3;
   const int ug = jx % a.ngroups;
   const int pidx = (jx / a.ngroups) * 8 + (blockIdx.x & 7);
   if (pidx >= P) return;
-  const int s = pidx % a.S;
-  const int kvh = (pidx / a.S) % a.Hkv;
-  const int rho = pidx / a.S / a.Hkv;
+  int s, kvh, rho;
+  program_of(a, pidx, s, kvh, rho);
   const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
 
   // this lane's query row; a padding row computes a copy of the last one and stores nothing
@@ -347,26 +356,31 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const uint32_t kc_ss = (uint32_t)a.kc_ss, vc_ss = (uint32_t)a.vc_ss;
   const int Hkv = a.Hkv;
   int bad = 0;
-  typedef const __attribute__((address_space(4))) int32_t* const_i32p;
-  typedef const __attribute__((address_space(4))) float* const_f32p;
+  // A wave-uniform word by a vector load all the same: a scalar one shares its counter with LDS and returns out of order, so
+  // that the next wait for an LDS operand would wait for it too.
+  int lane0 = 0;
+  asm("v_mov_b32 %0, 0" : "=v"(lane0));
   constexpr int NE = WHOLE ? 1 : NPT;  // page ids of a tile that a thread keeps
   auto key_of = [&](int t, int i) __attribute__((always_inline)) { return min(lo + t * TK + r0 + i * RSTEP, hi - 1); };
+  // Page ids are asked for an iteration before they are used, and looked at (their bounds) only then: a test next to the
+  // load would wait for it.
   auto pages_of = [&](int t, int (&e)[NE]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      int x;
-      if constexpr (WHOLE) x = ((const_i32p)trow)[__builtin_amdgcn_readfirstlane((lo + t * TK) >> shift)];
-      else x = trow[key_of(t, i) >> shift];
-      const bool ok = (uint32_t)x < (uint32_t)num_pages;
-      bad |= ok ? 0 : 1;
-      e[i] = ok ? x : 0;
+      if constexpr (WHOLE) e[i] = trow[((lo + t * TK) >> shift) + lane0];
+      else e[i] = trow[key_of(t, i) >> shift];
     }
+  };
+  auto checked = [&](int e) __attribute__((always_inline)) {
+    const bool ok = (uint32_t)e < (uint32_t)num_pages;
+    bad |= ok ? 0 : 1;
+    return ok ? e : 0;
   };
   auto load = [&](const uint8_t* cache, uint32_t ss, const float* scales, int t, const int (&e)[NE], u32x4 (&c)[NPT],
                   float (&sc)[NE]) __attribute__((always_inline)) {
     if constexpr (WHOLE) {
-      const int k0 = lo + t * TK;
-      const uint8_t* base = slot_row(cache, __builtin_amdgcn_readfirstlane((e[0] << shift) + (k0 & pmask)), ss);
+      const int k0 = lo + t * TK, pg = checked(__builtin_amdgcn_readfirstlane(e[0]));
+      const uint8_t* base = slot_row(cache, __builtin_amdgcn_readfirstlane((pg << shift) + (k0 & pmask)), ss);
       const int nv = hi - k0;
       if (nv >= TK) {
 #pragma unroll
@@ -378,12 +392,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
           c[i] = *reinterpret_cast<const u32x4*>(
               base + ((uint32_t)min(r0 + i * RSTEP, nv - 1) * ss + (uint32_t)part * 16));
       }
-      sc[0] = ((const_f32p)scales)[__builtin_amdgcn_readfirstlane(e[0] * Hkv)];
+      sc[0] = scales[pg * Hkv + lane0];
     } else {
 #pragma unroll
       for (int i = 0; i < NPT; ++i) {
-        c[i] = *reinterpret_cast<const u32x4*>(slot_row(cache, (e[i] << shift) + (key_of(t, i) & pmask), ss) + part * 16);
-        sc[i] = scales[e[i] * Hkv];
+        const int pg = checked(e[i]);
+        c[i] = *reinterpret_cast<const u32x4*>(slot_row(cache, (pg << shift) + (key_of(t, i) & pmask), ss) + part * 16);
+        sc[i] = scales[pg * Hkv];
       }
     }
   };
@@ -422,7 +437,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       put_k(0, k0, k0s);
       put_v(0, v0, v0s);
       put_k(1, kr, ksc);
-      vs_t = __float_as_uint(v0s[0]);
+      vs_t = __builtin_amdgcn_readfirstlane(__float_as_uint(v0s[0]));
       load(kc_h, kc_ss, ks_h, min(2, last), ev, kr, ksc);
       load(vc_h, vc_ss, vs_h, min(1, last), e1, vr, vsc);
     }
@@ -448,7 +463,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       constexpr int j = decltype(parity)::value;  // t % 2: LDS addresses become constants
       put_k(j, kr, ksc);
       put_v(j ^ 1, vr, vsc);
-      const uint32_t vs_next = __float_as_uint(vsc[0]);
+      const uint32_t vs_next = __builtin_amdgcn_readfirstlane(__float_as_uint(vsc[0]));
       if (t + 2 < ntiles) {
         load(vc_h, vc_ss, vs_h, t + 2, ev, vr, vsc);
         load(kc_h, kc_ss, ks_h, min(t + 3, last), ek, kr, ksc);
@@ -635,9 +650,8 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int half = lane >> 5, l32 = lane & 31;
   const int KL = a.KL, Lb = a.L, rows = a.rows;
   const float scale = a.scale_log2;
-  const int s = blockIdx.x % a.S;
-  const int kvh = (blockIdx.x / a.S) % a.Hkv;
-  const int rho = blockIdx.x / a.S / a.Hkv;
+  int s, kvh, rho;
+  program_of(a, blockIdx.x, s, kvh, rho);
   const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
   const int32_t* trow = kv8::table_row(a.pages, b);
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
@@ -712,12 +726,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int ntiles = (hi - lo + SK - 1) / SK;
   int bad = 0;
   auto key_of = [&](int t, int i) __attribute__((always_inline)) { return min(lo + t * SK + r0 + 8 * i, hi - 1); };
-  auto page_of = [&](int t, int i) __attribute__((always_inline)) {
-    const int e = trow[key_of(t, i) >> shift];
-    const bool ok = (uint32_t)e < (uint32_t)num_pages;
-    bad |= ok ? 0 : 1;
-    return ok ? e : 0;
-  };
+  auto page_of = [&](int t, int i) __attribute__((always_inline)) { return trow[key_of(t, i) >> shift]; };
   if (w < ntiles) {
     u32x4 kr[4], vr[4];
     float ksc[4], vsc[4];
@@ -725,11 +734,14 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto load = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int slot = (en[i] << shift) + (key_of(t, i) & pmask);
+        const bool ok = (uint32_t)en[i] < (uint32_t)num_pages;  // (looked at here: the ids were asked for a tile ago)
+        bad |= ok ? 0 : 1;
+        const int pg = ok ? en[i] : 0;
+        const int slot = (pg << shift) + (key_of(t, i) & pmask);
         kr[i] = *reinterpret_cast<const u32x4*>(slot_row(kc_h, slot, kc_ss));
         vr[i] = *reinterpret_cast<const u32x4*>(slot_row(vc_h, slot, vc_ss));
-        ksc[i] = ks_h[en[i] * Hkv];
-        vsc[i] = vs_h[en[i] * Hkv];
+        ksc[i] = ks_h[pg * Hkv];
+        vsc[i] = vs_h[pg * Hkv];
       }
     };
 #pragma unroll

@@ -29,66 +29,98 @@ TILE_KEYS = 64   # split_keys come in multiples of it
 
 
 # ------------------------------------------------------------------------------------------------ argument checks
+# A draft step calls these for every layer, with kernels of 5 to 30 us behind them: each check reads a tensor's attributes
+# once (0.04 us each), dtypes are compared by identity.
 
 
-def _cache_args(cache, scale, name: str, page_size: int):
-    """(pointer, slot stride, head stride, scale pointer) of one side of the cache."""
-    if cache.dtype != CODE_DTYPE or cache.dim() != 3 or cache.shape[2] != HEAD_DIM or cache.stride(2) != 1:
-        raise ValueError(f"{name}_cache must be {CODE_DTYPE} [slots, KV heads, {HEAD_DIM}] with contiguous rows, got "
-                         f"{cache.dtype} {tuple(cache.shape)}")
-    pages, heads = scale.shape
-    if scale.dtype != torch.float32 or not scale.is_contiguous() or heads != cache.shape[1] or \
-            pages * page_size != cache.shape[0]:
-        raise ValueError(f"{name}_scale must be contiguous float32 [{cache.shape[0]} / {page_size}, {cache.shape[1]}], got "
-                         f"{scale.dtype} {tuple(scale.shape)}")
-    return cache.data_ptr(), cache.stride(0), cache.stride(1), scale.data_ptr()
-
-
-def _check_page_size(page_size: int) -> None:
+def _cache_args(k_cache, v_cache, k_scale, v_scale, page_size: int):
+    """(k pointer, v pointer, slot and head strides of both, scale pointers, pages) of a cache, and its KV heads."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size {page_size}: one of {PAGE_SIZES}")
+    shape, scales = k_cache.shape, k_scale.shape
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if k_cache.dtype is not CODE_DTYPE or v_cache.dtype is not CODE_DTYPE or len(shape) != 3 or shape[2] != HEAD_DIM or \
+            v_cache.shape != shape or ks[2] != 1 or vs[2] != 1:
+        raise ValueError(f"k_cache and v_cache must be {CODE_DTYPE} [slots, KV heads, {HEAD_DIM}] with contiguous rows, got "
+                         f"{k_cache.dtype} {tuple(shape)} and {v_cache.dtype} {tuple(v_cache.shape)}")
+    heads = shape[1]
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or len(scales) != 2 or \
+            v_scale.shape != scales or scales[1] != heads or scales[0] * page_size != shape[0] or \
+            not k_scale.is_contiguous() or not v_scale.is_contiguous():
+        raise ValueError(f"k_scale and v_scale must be contiguous float32 [{shape[0]} / {page_size}, {heads}], got "
+                         f"{k_scale.dtype} {tuple(scales)} and {v_scale.dtype} {tuple(v_scale.shape)}")
+    return (k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], vs[0], vs[1], k_scale.data_ptr(), v_scale.data_ptr(),
+            scales[0]), heads
 
 
 def _table_args(table):
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"a page table is int32 [rows, pages] with contiguous rows, got {table.dtype} "
-                         f"{tuple(table.shape)}")
-    return table.data_ptr(), table.stride(0), table.shape[0], table.shape[1]
+    shape, stride = table.shape, table.stride()
+    if table.dtype is not torch.int32 or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError(f"a page table is int32 [rows, pages] with contiguous rows, got {table.dtype} {tuple(shape)}")
+    return table.data_ptr(), stride[0], shape[0], shape[1]
 
 
 def _index(t, n: int, name: str):
     """The first n entries of an index tensor as contiguous int64."""
-    if t.dim() != 1 or t.numel() < n or t.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"{name} must be int64 or int32 [{n}], got {t.dtype} {tuple(t.shape)}")
-    t = t[:n] if t.numel() != n else t
-    t = t if t.dtype == torch.int64 else t.to(torch.int64)
-    return t if t.is_contiguous() else t.contiguous()
+    shape, dtype = t.shape, t.dtype
+    if dtype is torch.int64 and len(shape) == 1 and shape[0] == n and t.is_contiguous():
+        return t
+    if len(shape) != 1 or shape[0] < n or dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{name} must be int64 or int32 [{n}], got {dtype} {tuple(shape)}")
+    return t[:n].to(torch.int64).contiguous()
 
 
-def _rows3(t, heads: Optional[int], name: str, dtype=torch.bfloat16):
-    if t.dtype != dtype or t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1 or \
-            (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be {dtype} [rows, heads, {HEAD_DIM}] with contiguous rows, got {t.dtype} "
-                         f"{tuple(t.shape)}")
+def _rows(t, count: int, heads: int, name: str):
+    """Strides of bf16 rows [count, heads, 128]."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1 or shape[0] != count or \
+            shape[1] != heads:
+        raise ValueError(f"{name} must be bfloat16 [{count}, {heads}, {HEAD_DIM}] with contiguous rows, got {t.dtype} "
+                         f"{tuple(shape)}")
+    return stride
+
+
+def _query(q, heads: int, num_modes: int, block_size: int):
+    """(requests, query heads, strides) of a batch's queries."""
+    shape, KL = q.shape, num_modes * block_size
+    if num_modes < 1 or block_size < 1 or len(shape) != 3 or shape[0] % KL or heads < 1 or shape[1] % heads:
+        raise ValueError(f"q {tuple(shape)} is not bs * {num_modes} * {block_size} rows of a multiple of {heads} heads")
+    return shape[0] // KL, shape[1], _rows(q, shape[0], shape[1], "q")
 
 
 def _weights_args(weights, heads: int):
-    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[1] != heads or \
-            (weights.shape[2] > 1 and weights.stride(2) != 1):
+    shape, stride = weights.shape, weights.stride()
+    if weights.dtype is not torch.float32 or len(shape) != 3 or shape[1] != heads or (stride[2] != 1 and shape[2] > 1):
         raise ValueError(f"weights must be float32 [rows, {heads}, tokens] with contiguous rows, got {weights.dtype} "
-                         f"{tuple(weights.shape)}")
-    return weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[0], weights.shape[2]
+                         f"{tuple(shape)}")
+    return weights.data_ptr(), stride[0], stride[1], shape[0], shape[2]
 
 
-def _same_device(*tensors):
-    """The tensors' GPU, the same for all of them."""
-    device = tensors[0].device
-    if device.type != "cuda":
-        raise ValueError(f"MFD kernels take GPU tensors (got a tensor on {device})")
+def _device_of(*tensors) -> int:
+    """The GPU of the tensors, the same for all of them."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
-    return device
+        if t is not None and t.get_device() != index or index < 0:
+            raise ValueError(f"MFD kernels take GPU tensors of one device (got tensors on {tensors[0].device} and "
+                             f"{t.device})")
+    return index
+
+
+def _err(err_flag):
+    if err_flag is None:
+        return None
+    if err_flag.dtype is not torch.int32 or err_flag.numel() < 1:
+        raise ValueError(f"err_flag must be int32, got {err_flag.dtype}")
+    return err_flag.data_ptr()
+
+
+def _scratch(workspace, need: int, like):
+    """The caller's workspace if it is given and large enough, else a new one."""
+    if workspace is None:
+        return like.new_empty(need, dtype=torch.uint8)
+    if workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous() or workspace.data_ptr() % 16:
+        raise ValueError(f"a contiguous, 16-byte aligned workspace of {need} bytes is needed")
+    return workspace
 
 
 # ----------------------------------------------------------------------------------------------------------- store
@@ -105,47 +137,41 @@ def kv8_store(*, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     page begun earlier the scale only grows, and the entries before the new ones are rounded again when it does. Entries
     behind the new ones keep their bits. Infinities become +-448 s, NaN stays NaN. Two requests must not store into one
     page in the same call."""
-    _check_page_size(page_size)
-    heads = k_cache.shape[1]
-    _rows3(k, heads, "k")
-    _rows3(v, heads, "v")
-    if v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    bs = cu_tokens.numel() - 1
-    if cu_tokens.dtype != torch.int32 or cu_tokens.dim() != 1 or bs < 0 or not cu_tokens.is_contiguous():
+    cache, heads = _cache_args(k_cache, v_cache, k_scale, v_scale, page_size)
+    n, bs = k.shape[0], cu_tokens.numel() - 1
+    ks, vs = _rows(k, n, heads, "k"), _rows(v, n, heads, "v")
+    if cu_tokens.dtype is not torch.int32 or cu_tokens.dim() != 1 or bs < 0 or not cu_tokens.is_contiguous():
         raise ValueError(f"cu_tokens must be contiguous int32 [bs + 1], got {cu_tokens.dtype} {tuple(cu_tokens.shape)}")
-    device = _same_device(k, v, k_cache, v_cache, k_scale, v_scale, page_table, req_pool_indices, start_lens, cu_tokens,
-                          err_flag)
-    kp, kss, ksh, ksp = _cache_args(k_cache, k_scale, "k", page_size)
-    vp, vss, vsh, vsp = _cache_args(v_cache, v_scale, "v", page_size)
-    if k_scale.shape != v_scale.shape:
-        raise ValueError("the K and V caches have different sizes")
+    device = _device_of(k, v, k_cache, v_cache, k_scale, v_scale, page_table, req_pool_indices, start_lens, cu_tokens,
+                        err_flag)
     rows, starts = _index(req_pool_indices, bs, "req_pool_indices"), _index(start_lens, bs, "start_lens")
-    mfd_hip.call_on(device, "mfd_kv8_store", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp, vp,
-          kss, ksh, vss, vsh, ksp, vsp, k_scale.shape[0], *_table_args(page_table), page_size, rows.data_ptr(),
-          starts.data_ptr(), cu_tokens.data_ptr(), k.shape[0], bs, int(max_tokens), heads, HEAD_DIM,
-          mfd_hip.ptr(err_flag))
+    mfd_hip.call_on(device, "mfd_kv8_store", k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], *cache,
+                    *_table_args(page_table), page_size, rows.data_ptr(), starts.data_ptr(), cu_tokens.data_ptr(), n, bs,
+                    max_tokens, heads, HEAD_DIM, _err(err_flag))
 
 
 # ------------------------------------------------------------------------------------------------------- attention
 
 
 def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int, device) -> tuple[int, int]:
-    """(num_ctx_splits, split_keys) for num_ctx_splits < 0: enough parts of the longest context for two rounds of workgroup
-    slots if all were as long (contexts of a batch differ, and short workgroups behind long ones even that out), of at least
-    256 keys each."""
+    """(num_ctx_splits, split_keys) for num_ctx_splits < 0, from what the kernels' workgroup slots hold (two workgroups per CU,
+    one of eight waves) and the programs (request, KV head, group of units) that there are without a split.
+
+    A single request's splits fill one round of slots, less the block partial's; a batch's lengths differ and half a round
+    more evens them out, three rounds where a program is one unit (plain decoding: 16 requests of 4748 .. 32132 tokens, 40
+    heads: 173 us with one round, 146 with three, 152 with eight; 64 even ones, a workgroup per slot already: 66 us whole,
+    76 in two parts). At least 128 keys per split there and 256 else, at most 32 and 64 splits (32768 tokens, one request:
+    28 us in 32 parts, 34 in 64)."""
     units = -(-rows // UNIT)
     waves = 8 if units % 8 == 0 else 4
-    slots = mfd_hip.cu_count(device) * (1 if units > 1 and waves == 8 else 2)
+    slots = mfd_hip.cu_count(device) * (1 if waves == 8 else 2)
     programs = max(1, bs * heads * -(-units // waves))
-    want = slots * (1 if bs == 1 else 2)
-    splits = want // programs if bs == 1 else -(-want // programs)
-    if bs == 1 and with_block and units > 1:
-        splits -= 1
-    splits = min(splits, -(-max_ctx // 256), 64)
-    if splits <= 1:
-        return 1, 0
-    return _splits_of(splits, max_ctx)
+    if units == 1:
+        splits = 1 if programs >= slots else min((1 if bs == 1 else 3) * slots // programs, -(-max_ctx // 128), 32)
+    else:
+        splits = slots // programs - (1 if with_block else 0) if bs == 1 else 3 * slots // (2 * programs)
+        splits = min(splits, -(-max_ctx // 256), 64)
+    return _splits_of(splits, max_ctx) if splits > 1 else (1, 0)
 
 
 def _splits_of(splits: int, max_ctx: int) -> tuple[int, int]:
@@ -192,63 +218,45 @@ def paged_mode_block_attention_kv8(
     a longer last part), joined by log-sum-exp; 0 or 1: one pass; < 0: by the batch's sizes. ``max_ctx`` (default: what the
     page table's rows hold) only tunes the splits. ``workspace``: a uint8 buffer of workspace_bytes(...), for capture
     without allocation; one buffer must not serve two calls that may overlap."""
-    _check_page_size(page_size)
-    T, H, _ = q.shape
-    heads = k_cache.shape[1]
-    KL = num_modes * block_size
-    if num_modes < 1 or block_size < 1 or T % KL or H % heads:
-        raise ValueError(f"q {tuple(q.shape)} is not bs * {num_modes} * {block_size} rows of a multiple of {heads} heads")
-    _rows3(q, None, "q")
-    bs = T // KL
+    cache, heads = _cache_args(k_cache, v_cache, k_scale, v_scale, page_size)
+    bs, H, qs = _query(q, heads, num_modes, block_size)
+    T = q.shape[0]
     fresh = k_new is not None
     if fresh != (v_new is not None):
         raise ValueError("k_new and v_new go together")
     if fresh:
-        _rows3(k_new, heads, "k_new")
-        _rows3(v_new, heads, "v_new")
-        if k_new.shape[0] != T or v_new.shape[0] != T:
-            raise ValueError(f"k_new and v_new must have q's {T} rows")
-        fresh_args = (k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), k_new.stride(1), v_new.stride(0),
-                      v_new.stride(1))
+        ks, vs = _rows(k_new, T, heads, "k_new"), _rows(v_new, T, heads, "v_new")
+        new = (k_new.data_ptr(), v_new.data_ptr(), ks[0], ks[1], vs[0], vs[1])
     else:
-        fresh_args = (None, None, 0, 0, 0, 0)
-    device = _same_device(q, k_new, v_new, k_cache, v_cache, k_scale, v_scale, page_table, req_pool_indices, ctx_lens, out,
-                          lse_out, workspace, err_flag)
-    kp, kss, ksh, ksp = _cache_args(k_cache, k_scale, "k", page_size)
-    vp, vss, vsh, vsp = _cache_args(v_cache, v_scale, "v", page_size)
-    if k_scale.shape != v_scale.shape:
-        raise ValueError("the K and V caches have different sizes")
+        new = (None, None, 0, 0, 0, 0)
+    device = _device_of(q, k_new, v_new, k_cache, v_cache, k_scale, v_scale, page_table, req_pool_indices, ctx_lens, out,
+                        lse_out, workspace, err_flag)
+    table = _table_args(page_table)
     if out is None:
-        out = torch.empty((T, H, HEAD_DIM), device=device, dtype=torch.bfloat16)
-    else:
-        _rows3(out, H, "out")
-        if out.shape[0] != T:
-            raise ValueError(f"out must have q's {T} rows")
-    if lse_out is None and return_lse:
-        lse_out = torch.empty((T, H), device=device, dtype=torch.float32)
-    elif lse_out is not None and (lse_out.dtype != torch.float32 or tuple(lse_out.shape) != (T, H) or
-                                  not lse_out.is_contiguous()):
-        raise ValueError(f"lse_out must be contiguous float32 [{T}, {H}]")
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, H, HEAD_DIM))
+    os = _rows(out, T, H, "out")
+    if lse_out is not None:
+        if lse_out.dtype is not torch.float32 or tuple(lse_out.shape) != (T, H) or not lse_out.is_contiguous():
+            raise ValueError(f"lse_out must be contiguous float32 [{T}, {H}], got {lse_out.dtype} {tuple(lse_out.shape)}")
+    elif return_lse:
+        lse_out = q.new_empty((T, H), dtype=torch.float32)
     if bs:
-        cap = page_table.shape[1] * page_size
-        max_ctx = cap if max_ctx is None else max(1, min(int(max_ctx), cap))
+        cap = max(1, table[3] * page_size)
+        max_ctx = cap if max_ctx is None else max(1, min(max_ctx, cap))
         if num_ctx_splits < 0:
-            splits, keys = _auto_splits(bs, heads, H // heads * KL, fresh, max_ctx, device)
+            splits, keys = _auto_splits(bs, heads, H // heads * num_modes * block_size, fresh, max_ctx, q.device)
         else:
             splits, keys = _splits_of(num_ctx_splits, max_ctx) if num_ctx_splits > 1 else (1, 0)
         need = 0
         if splits > 1:
             need = mfd_hip.lib().mfd_kv8_attn_workspace_bytes(bs, num_modes, block_size, H, heads, fresh, splits)
-            if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
-                raise ValueError(f"a contiguous workspace of {need} bytes is needed")
+            workspace = _scratch(workspace, need, q)
         rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
-        mfd_hip.call_on(device, "mfd_kv8_attn", q.data_ptr(), q.stride(0), q.stride(1), *fresh_args, kp, vp, kss, ksh, vss, vsh,
-              ksp, vsp, k_scale.shape[0], *_table_args(page_table), page_size, rows.data_ptr(), lens.data_ptr(), bs,
-              num_modes, block_size, H, heads, HEAD_DIM, float(scaling), 1 if causal_in_block else 0, splits, keys,
-              out.data_ptr(), out.stride(0), out.stride(1), mfd_hip.ptr(lse_out), workspace.data_ptr() if need else None,
-              need, mfd_hip.ptr(err_flag))
+        mfd_hip.call_on(device, "mfd_kv8_attn", q.data_ptr(), qs[0], qs[1], *new, *cache, *table, page_size,
+                        rows.data_ptr(), lens.data_ptr(), bs, num_modes, block_size, H, heads, HEAD_DIM, scaling,
+                        1 if causal_in_block else 0, splits, keys, out.data_ptr(), os[0], os[1],
+                        None if lse_out is None else lse_out.data_ptr(), workspace.data_ptr() if need else None, need,
+                        _err(err_flag))
     return (out, lse_out) if lse_out is not None else out
 
 
@@ -285,23 +293,16 @@ def attention_weights_kv8(*, q: torch.Tensor, lse: torch.Tensor, k_cache: torch.
     lse -inf add nothing). weights: float32 [rows, KV heads, tokens], zero before a request's first call. With page tables
     that all layers share, one ``weights`` collects every layer's call: decay in the first, 1 in the others. decay 0 does not
     read the old sums. Results repeat bit for bit."""
-    _check_page_size(page_size)
-    T, H, _ = q.shape
-    heads = k_cache.shape[1]
-    KL = num_modes * block_size
-    if num_modes < 1 or block_size < 1 or T % KL or H % heads:
-        raise ValueError(f"q {tuple(q.shape)} is not bs * {num_modes} * {block_size} rows of a multiple of {heads} heads")
-    _rows3(q, None, "q")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (T, H) or not lse.is_contiguous():
-        raise ValueError(f"lse must be contiguous float32 [{T}, {H}], got {lse.dtype} {tuple(lse.shape)}")
-    bs = T // KL
-    device = _same_device(q, lse, k_cache, k_scale, page_table, req_pool_indices, ctx_lens, weights, err_flag)
-    kp, kss, ksh, ksp = _cache_args(k_cache, k_scale, "k", page_size)
+    cache, heads = _cache_args(k_cache, k_cache, k_scale, k_scale, page_size)
+    bs, H, qs = _query(q, heads, num_modes, block_size)
+    if lse.dtype is not torch.float32 or tuple(lse.shape) != (q.shape[0], H) or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous float32 [{q.shape[0]}, {H}], got {lse.dtype} {tuple(lse.shape)}")
+    device = _device_of(q, lse, k_cache, k_scale, page_table, req_pool_indices, ctx_lens, weights, err_flag)
     rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
-    mfd_hip.call_on(device, "mfd_kv8_weights", q.data_ptr(), q.stride(0), q.stride(1), lse.data_ptr(), kp, kss, ksh, ksp,
-          k_scale.shape[0], *_table_args(page_table), page_size, rows.data_ptr(), lens.data_ptr(), bs, num_modes,
-          block_size, H, heads, HEAD_DIM, float(scaling), float(decay), *_weights_args(weights, heads),
-          mfd_hip.ptr(err_flag))
+    mfd_hip.call_on(device, "mfd_kv8_weights", q.data_ptr(), qs[0], qs[1], lse.data_ptr(), cache[0], cache[2], cache[3],
+                    cache[6], cache[8], *_table_args(page_table), page_size, rows.data_ptr(), lens.data_ptr(), bs,
+                    num_modes, block_size, H, heads, HEAD_DIM, scaling, decay, *_weights_args(weights, heads),
+                    _err(err_flag))
 
 
 def evict_select(*, weights: torch.Tensor, req_pool_indices: torch.Tensor, ctx_lens: torch.Tensor, budget: int,
@@ -312,24 +313,19 @@ def evict_select(*, weights: torch.Tensor, req_pool_indices: torch.Tensor, ctx_l
     ``recent``, and of the rest those whose weights, summed over the KV heads (in float64, rounded once to float32), are
     largest (ties: the lowest position; NaN below everything). Returns (keep [bs, budget] int32: positions ascending, -1
     behind them; new_lens [bs] int64). bs is ctx_lens' length."""
-    bs = ctx_lens.numel()
-    heads = weights.shape[1]
-    device = _same_device(weights, req_pool_indices, ctx_lens, keep_out, new_lens_out, workspace, err_flag)
-    wargs = _weights_args(weights, heads)
-    keep = torch.empty((bs, budget), dtype=torch.int32, device=device) if keep_out is None else keep_out
-    new_lens = torch.empty(bs, dtype=torch.int64, device=device) if new_lens_out is None else new_lens_out
-    if keep.dtype != torch.int32 or tuple(keep.shape) != (bs, budget) or not keep.is_contiguous() or \
-            new_lens.dtype != torch.int64 or tuple(new_lens.shape) != (bs,) or not new_lens.is_contiguous():
+    bs, heads = ctx_lens.shape[0], weights.shape[1]
+    sums = _weights_args(weights, heads)
+    device = _device_of(weights, req_pool_indices, ctx_lens, keep_out, new_lens_out, workspace, err_flag)
+    keep = weights.new_empty((bs, budget), dtype=torch.int32) if keep_out is None else keep_out
+    new_lens = weights.new_empty(bs, dtype=torch.int64) if new_lens_out is None else new_lens_out
+    if keep.dtype is not torch.int32 or tuple(keep.shape) != (bs, budget) or not keep.is_contiguous() or \
+            new_lens.dtype is not torch.int64 or tuple(new_lens.shape) != (bs,) or not new_lens.is_contiguous():
         raise ValueError(f"keep_out must be contiguous int32 [{bs}, {budget}] and new_lens_out int64 [{bs}]")
-    need = mfd_hip.lib().mfd_evict_select_workspace_bytes(bs, weights.shape[2])
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
-        raise ValueError(f"a contiguous workspace of {need} bytes is needed")
+    need = mfd_hip.lib().mfd_evict_select_workspace_bytes(bs, sums[4])
+    workspace = _scratch(workspace, need, weights)
     rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
-    mfd_hip.call_on(device, "mfd_evict_select", *wargs, heads, rows.data_ptr(), lens.data_ptr(), bs, int(budget), int(sink),
-          int(recent), keep.data_ptr(), new_lens.data_ptr(), workspace.data_ptr() if need else None, need,
-          mfd_hip.ptr(err_flag))
+    mfd_hip.call_on(device, "mfd_evict_select", *sums, heads, rows.data_ptr(), lens.data_ptr(), bs, budget, sink, recent,
+                    keep.data_ptr(), new_lens.data_ptr(), workspace.data_ptr() if need else None, need, _err(err_flag))
     return keep, new_lens
 
 
@@ -342,23 +338,18 @@ def evict_compact_kv8(*, keep: torch.Tensor, new_lens: torch.Tensor, ctx_lens: t
     requests, but may be shared by nobody. Entries behind the last kept token keep their bits. ``weights``: the running sums
     move along in place, and those of positions new_lens[b] : ctx_lens[b] become 0. With several layers on the same tables,
     every layer's cache is compacted with the same ``keep`` and one call of them takes ``weights``."""
-    _check_page_size(page_size)
+    cache, heads = _cache_args(k_cache, v_cache, k_scale, v_scale, page_size)
     bs, budget = keep.shape
-    heads = k_cache.shape[1]
-    if keep.dtype != torch.int32 or not keep.is_contiguous():
+    if keep.dtype is not torch.int32 or not keep.is_contiguous():
         raise ValueError(f"keep must be contiguous int32 [bs, budget], got {keep.dtype}")
-    device = _same_device(keep, new_lens, ctx_lens, k_cache, v_cache, k_scale, v_scale, src_table, dst_table,
-                          req_pool_indices, weights, err_flag)
-    kp, kss, ksh, ksp = _cache_args(k_cache, k_scale, "k", page_size)
-    vp, vss, vsh, vsp = _cache_args(v_cache, v_scale, "v", page_size)
-    if k_scale.shape != v_scale.shape:
-        raise ValueError("the K and V caches have different sizes")
-    wargs = _weights_args(weights, heads) if weights is not None else (None, 0, 0, 0, 0)
+    device = _device_of(keep, new_lens, ctx_lens, k_cache, v_cache, k_scale, v_scale, src_table, dst_table,
+                        req_pool_indices, weights, err_flag)
+    sums = _weights_args(weights, heads) if weights is not None else (None, 0, 0, 0, 0)
     new, lens = _index(new_lens, bs, "new_lens"), _index(ctx_lens, bs, "ctx_lens")
     rows = _index(req_pool_indices, bs, "req_pool_indices")
-    mfd_hip.call_on(device, "mfd_evict_compact_kv8", keep.data_ptr(), budget, new.data_ptr(), lens.data_ptr(), kp, vp, kss, ksh, vss,
-          vsh, ksp, vsp, k_scale.shape[0], *_table_args(src_table), *_table_args(dst_table), page_size, rows.data_ptr(),
-          *wargs, bs, heads, HEAD_DIM, mfd_hip.ptr(err_flag))
+    mfd_hip.call_on(device, "mfd_evict_compact_kv8", keep.data_ptr(), budget, new.data_ptr(), lens.data_ptr(), *cache,
+                    *_table_args(src_table), *_table_args(dst_table), page_size, rows.data_ptr(), *sums, bs, heads, HEAD_DIM,
+                    _err(err_flag))
 
 
 # ------------------------------------------------------------------------------------------------------------ pool
@@ -370,7 +361,8 @@ class Kv8Pool:
     to whom is the caller's allocator's business."""
 
     def __init__(self, *, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, device="cuda"):
-        _check_page_size(page_size)
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size {page_size}: one of {PAGE_SIZES}")
         self.page_size, self.num_pages = int(page_size), int(num_pages)
         slots = self.num_pages * self.page_size
         codes = lambda: torch.zeros(slots, num_kv_heads, HEAD_DIM, dtype=torch.uint8, device=device).view(CODE_DTYPE)

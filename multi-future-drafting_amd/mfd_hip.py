@@ -159,14 +159,19 @@ def stream_of(t: torch.Tensor) -> int:
     return _raw_stream(index)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """call() with that GPU's current stream as the last argument, and the GPU as the current one (which it is in nearly
-    every program: a launch belongs to the current device, whatever its tensors')."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _raw_stream(device.index))
+_current_device = torch._C._cuda_getDevice
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """call() on GPU ``index`` (the tensors'), with its current stream as the last argument. A launch belongs to the current
+    device, whatever its tensors': where that is another one (in hardly any program), it is changed for the call."""
+    if index == _current_device():
+        status = _FN[name](*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args, _raw_stream(device.index))
+        with torch.cuda.device(index):
+            status = _FN[name](*args, _raw_stream(index))
+    if status != 0:
+        check(status, name)
 
 
 def as_dtype(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

@@ -38,9 +38,10 @@ class Mxfp4Weight(NamedTuple):
 
 def check_weight(codes: torch.Tensor, exps: torch.Tensor, values: bool = False) -> None:
     """The layout above, and with ``values`` (which waits for the device) the range of the scales; ValueError otherwise."""
-    if codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or codes.dim() != 2 or exps.dim() != 2 or \
-            not codes.is_contiguous() or not exps.is_contiguous() or codes.shape[1] % 64 or codes.shape[0] < 1 or \
-            tuple(exps.shape) != (codes.shape[0], codes.shape[1] * 2 // GROUP) or exps.device != codes.device or \
+    shape = codes.shape
+    if codes.dtype is not torch.uint8 or exps.dtype is not torch.uint8 or len(shape) != 2 or \
+            not codes.is_contiguous() or not exps.is_contiguous() or shape[1] % 64 or shape[0] < 1 or shape[1] < 1 or \
+            tuple(exps.shape) != (shape[0], shape[1] // 16) or exps.get_device() != codes.get_device() or \
             codes.data_ptr() % 16 or exps.data_ptr() % 4:
         raise ValueError(f"codes must be contiguous uint8 [vocab, hidden / 2] with hidden % 128 == 0 and exps contiguous "
                          f"uint8 [vocab, hidden / {GROUP}] on the same device, got {codes.dtype} {tuple(codes.shape)} and "
@@ -92,19 +93,26 @@ def draft_head_mxfp4(x: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor,
     rows, their stride a multiple of 4."""
     check_weight(codes, exps)
     vocab, hidden = codes.shape[0], codes.shape[1] * 2
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != hidden:
+    if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != hidden:
         raise ValueError(f"x must be bfloat16 [rows, {hidden}], got {x.dtype} {tuple(x.shape)}")
-    if not x.is_cuda or x.device != codes.device or (out is not None and out.device != x.device):
+    device = x.get_device()
+    if device < 0 or codes.get_device() != device or (out is not None and out.get_device() != device):
         raise ValueError(f"MFD kernels take GPU tensors of one device (x on {x.device}, codes on {codes.device})")
-    rows = x.shape[0]
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+    rows, stride = x.shape[0], x.stride()
+    if stride[1] != 1 or stride[0] % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
+        stride = x.stride()
     if out is None:
-        out = torch.empty((rows, (vocab + 7) // 8 * 8), dtype=torch.bfloat16, device=x.device)[:, :vocab]
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (rows, vocab) or (vocab > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be bfloat16 [{rows}, {vocab}] with contiguous rows")
-    mfd_hip.call_on(x.device, "mfd_draft_head_mxfp4", x.data_ptr(), x.stride(0), max(rows, 1), 0, codes.data_ptr(),
-                    exps.data_ptr(), rows, vocab, hidden, out.data_ptr(), out.stride(0))
+        out = x.new_empty((rows, (vocab + 7) // 8 * 8))
+        pitch = out.stride(0)
+        if out.shape[1] != vocab:
+            out = out[:, :vocab]
+    else:
+        pitch = out.stride(0)
+        if out.dtype is not torch.bfloat16 or tuple(out.shape) != (rows, vocab) or (vocab > 1 and out.stride(1) != 1):
+            raise ValueError(f"out must be bfloat16 [{rows}, {vocab}] with contiguous rows")
+    mfd_hip.call_on(device, "mfd_draft_head_mxfp4", x.data_ptr(), stride[0], rows or 1, 0, codes.data_ptr(),
+                    exps.data_ptr(), rows, vocab, hidden, out.data_ptr(), pitch)
     return out
