@@ -38,7 +38,6 @@ using kv8::u32x4;
 constexpr int TK = 64;         // keys per tile of the tile kernel
 constexpr int UROWS = 32;      // query rows per unit
 constexpr int SK = 32;         // keys per tile of the stream kernel
-constexpr int SNW = 4;         // its waves
 constexpr float LN2 = 0.6931471805599453f;
 
 typedef short v4i16 __attribute__((ext_vector_type(4)));
@@ -640,7 +639,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
 // ---------------------------------------------------------------------------------------------- stream kernel
 
+// SNW waves: four, and two workgroups on a CU; or eight, where the grid has no more workgroups than there are CUs
+template <int SNW>
 __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attn_stream_kernel(Args a) {
+  static_assert(SNW == 4 || SNW == 8, "a row's results are joined by 8 or 16 threads");
   constexpr int WLDS = SK * (KROW + VROW);  // bytes of a wave's widened K and V tile (17.5 KB)
   static_assert(UROWS * D * 4 <= WLDS, "a wave's result fits its tiles");
   __shared__ __attribute__((aligned(16))) uint8_t lds[SNW * WLDS];
@@ -831,8 +833,9 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
     l_run += psum;
   }
-  // ---- the waves' results: each brings its accumulators to the common reference and into its part of LDS as
-  //      [row][d] fp32 (16 KB); thread (row tid / 8, 16 d's tid % 8) adds them in wave order
+  // ---- the waves' results: each brings its accumulators to the common reference and into its part of LDS as [row][d] fp32
+  //      (16 KB); TPR threads per row add them in wave order
+  constexpr int TPR = SNW * 64 / UROWS, DPT = D / TPR;  // 8 or 16 threads, of 16 or 8 d's
   const float l_w = half_sum(l_run);
   if (half == 0) {
     lds_m[w][l32] = m_run;
@@ -845,7 +848,8 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const float fac = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_tot) * __uint_as_float(unit);
   float* const own = reinterpret_cast<float*>(lds + w * WLDS);
   // 16-byte piece c of row r at c ^ r, so that the lanes of a write or a read spread over the banks
-  if (w < ntiles || (with_block && w == SNW - 1)) {
+  auto has_keys = [&](int x) __attribute__((always_inline)) { return x < ntiles || (with_block && x == SNW - 1); };
+  if (has_keys(w)) {
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -857,58 +861,57 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
   }
   lds_barrier();
-  const int row = tid >> 3;
-  f32x4 o[4] = {};
+  const int row = tid / TPR, piece = tid % TPR, d0 = piece * DPT;
+  f32x4 o[DPT / 4] = {};
   float mt = -INFINITY, lt = 0.f;
 #pragma unroll
   for (int x = 0; x < SNW; ++x) mt = fmaxf(mt, lds_m[x][row]);
 #pragma unroll
   for (int x = 0; x < SNW; ++x) {
-    if (!(x < ntiles || (with_block && x == SNW - 1))) continue;  // a wave without keys
-    const float mw = lds_m[x][row];
-    lt += mw == -INFINITY ? (lds_l[x][row] == 0.f ? 0.f : lds_l[x][row]) : lds_l[x][row] * __builtin_amdgcn_exp2f(mw - mt);
+    if (!has_keys(x)) continue;
+    const float mw = lds_m[x][row], lw = lds_l[x][row];
+    lt += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - mt);  // (-inf: no key, 0, or NaN)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < DPT / 4; ++c)
       o[c] += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WLDS) + row * D +
-                                              (((4 * (tid & 7) + c) ^ row) & 31) * 4);
+                                              (((d0 / 4 + c) ^ row) & 31) * 4);
   }
-  if (row >= rows) return;  // (whole groups of eight threads)
+  if (row >= rows) return;  // (whole groups of threads)
   const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
   const float lse2 = lt > 0.f ? mt + __log2f(lt) : (lt == 0.f ? -INFINITY : lt);
-  const int d0 = (tid & 7) * 16;
   if (a.S == 1) {
     const int64_t token = (int64_t)b * KL + row % KL;
     const int head = kvh * a.G + row / KL;
     uint16_t* op = a.out + token * a.o_st + (int64_t)head * a.o_sh + d0;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < DPT / 8; ++c) {
       u16x8 v;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = f2bf_bits(o[2 * c + (e >> 2)][e & 3] * inv);
       *reinterpret_cast<u16x8*>(op + 8 * c) = v;
     }
-    if (a.lse && (tid & 7) == 0) a.lse[token * a.H + head] = lse2 * LN2;
+    if (a.lse && piece == 0) a.lse[token * a.H + head] = lse2 * LN2;
     return;
   }
   float mx = 0.f;
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int c = 0; c < DPT / 4; ++c)
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(o[c][e] * inv));
 #pragma unroll
-  for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+  for (int x = 1; x < TPR; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
   const int ex = mx > 0.f ? __builtin_amdgcn_frexp_expf(mx) : 0;
   const float down = __builtin_ldexpf(inv, -ex);
   const int64_t prow = partial_row(a, s, b, kvh, row);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < DPT / 8; ++c) {
     u32x4 hv;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       hv[e] = f2h2_bits(o[2 * c + (e >> 1)][2 * (e & 1)] * down, o[2 * c + (e >> 1)][2 * (e & 1) + 1] * down);
     *reinterpret_cast<u32x4*>(a.ws_o + prow * D + d0 + 8 * c) = hv;
   }
-  if ((tid & 7) == 0) {
+  if (piece == 0) {
     a.ws_lse[prow] = lse2;
     a.ws_exp[prow] = (float)ex;
   }
@@ -983,10 +986,10 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
 // units of 32 through a double buffer in LDS that the waves share. A lane then holds, for its query row, the 32 keys of its
 // half; p = exp2(s scale - lse) is added up per key over the units in registers, and once at the end over the 32 lanes.
 // Every sum has one owner and one order: no atomics. Bound by the exponentials (one per product of 256 flops).
-constexpr int WNW = 4;
-constexpr int WKEYS = WNW * TK;
-constexpr int WOCC = 3;  // waves per SIMD
-constexpr int QS = 2;    // units per stage of query rows
+//
+// RS: waves per 64 keys, each of which takes every RS-th pair of units; two where one would leave each CU a workgroup or none
+// (a single request), their sums joined in LDS in wave order. QS: units of a wave per stage; one where a KV head has one unit.
+constexpr int WKEYS = 4 * TK;
 
 struct WArgs {
   const uint16_t* q;
@@ -1005,13 +1008,18 @@ struct WArgs {
   int32_t* err_flag;
 };
 
-__global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, WOCC))) void kv8_weights_kernel(WArgs a) {
-  // 32 keys of each wave at a time first, then two stages of query rows
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[WNW * SK * KROW];
-  static_assert(2 * QS * UROWS * D * 2 <= WNW * SK * KROW, "two stages fit");
+template <int RS, int QS>
+__global__ __launch_bounds__(RS * 256) __attribute__((amdgpu_waves_per_eu(RS == 1 ? 3 : 2, RS == 1 ? 3 : 2)))
+void kv8_weights_kernel(WArgs a) {
+  static_assert(RS <= 2 && QS <= 2, "one or two");
+  constexpr int NWV = 4 * RS;
+  // widened keys first (32 of each wave at a time), then two stages of query rows
+  constexpr int KLDS = NWV * SK * KROW, STAGE = RS * QS * UROWS * D * 2;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[KLDS > 2 * STAGE ? KLDS : 2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
+  const int wk = w & 3, wr = w >> 2;  // the wave's 64 keys, and its share of the units
   // KV heads fastest, key ranges slowest: with eight heads each XCD (workgroup id modulo 8) has one, whose query rows stay in
   // its L2, and ranges that only the longest requests reach are spread over all of them
   const int kvh = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv % a.bs, range = blockIdx.x / a.Hkv / a.bs;
@@ -1025,98 +1033,117 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, 
   const int lo = range * WKEYS;
   if (lo >= ctx) return;
 
-  // Query rows come by direct-to-LDS loads, QS units (64 rows, 16 KB) at a time, double buffered. A load moves four whole
-  // rows: load i of wave w takes rows 16 i + 4 w + lane / 16 of the stage, and chunk c of row r lands at c ^ (r % 16) of
-  // the row (the lane at position p asks for chunk p ^ (r % 16)). Rows past the last repeat the first.
-  const int stages = (a.rows + QS * UROWS - 1) / (QS * UROWS);
+  // Query rows come by direct-to-LDS loads, a stage of RS QS units at a time, double buffered. A load moves four whole rows:
+  // load i of wave w takes rows 16 RS i + 4 w + lane / 16 of the stage, and chunk c of row r lands at c ^ (r % 16) of the row
+  // (the lane at position p asks for chunk p ^ (r % 16)). Rows past the last repeat the first.
+  const int stages = (a.rows + RS * QS * UROWS - 1) / (RS * QS * UROWS);
+  constexpr int QSTEP = 16 * RS;  // rows from one of a wave's loads to its next
   const int qr = 4 * w + (lane >> 4);
-  const int dg = 16 / a.KL, dq = 16 % a.KL;
-  const int64_t q_step = dg * a.q_sh + dq * a.q_st, q_wrap = a.q_sh - a.KL * a.q_st;
+  const int dg = QSTEP / a.KL, dq = QSTEP % a.KL;
+  const uint32_t q_st = (uint32_t)a.q_st, q_sh = (uint32_t)a.q_sh;  // (a request's queries span less than 2^30 elements)
+  const uint32_t q_step = dg * q_sh + dq * q_st, q_wrap = q_sh - a.KL * q_st;
+  const uint16_t* const q_b = a.q + (int64_t)b * a.KL * a.q_st + (int64_t)kvh * a.G * a.q_sh;
   int rr = qr, rq = qr % a.KL;  // the next load's row, and its query
-  const uint16_t* const q_first =
-      a.q + (int64_t)b * a.KL * a.q_st + (int64_t)kvh * a.G * a.q_sh + ((lane & 15) ^ (qr & 15)) * 8;
-  const uint16_t* qp = q_first + (qr / a.KL) * a.q_sh + rq * a.q_st;
+  const uint32_t q_first = ((lane & 15) ^ (qr & 15)) * 8;
+  uint32_t qo = q_first + (uint32_t)(qr / a.KL) * q_sh + (uint32_t)rq * q_st;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  auto load_q = [&](int j) __attribute__((always_inline)) {
+  auto load_q = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2 * QS; ++i) {
-      dma16(rr < a.rows ? qp : q_first, lds0 + (uint32_t)(j * QS * UROWS + 16 * i + 4 * w) * (D * 2));
-      rr += 16;
+      dma16(q_b + (rr < a.rows ? qo : q_first), lds0 + (uint32_t)((st & 1) * STAGE + (QSTEP * i + 4 * w) * (D * 2)));
+      rr += QSTEP;
       rq += dq;
       const bool wrap = rq >= a.KL;
       rq -= wrap ? a.KL : 0;
-      qp += q_step + (wrap ? q_wrap : 0);
+      qo += q_step + (wrap ? q_wrap : 0);
     }
   };
-  // lse of row l32 of the next unit; padding rows get +inf (probability 0), and so do rows whose lse is -inf (they saw no key)
-  const int lg = UROWS / a.KL, lq = UROWS % a.KL;
-  const int64_t l_step = lg + (int64_t)lq * a.H, l_wrap = 1 - (int64_t)a.KL * a.H;
-  int lr = l32, lrq = l32 % a.KL;
-  const float* lp = a.lse + ((int64_t)b * a.KL + lrq) * a.H + kvh * a.G + l32 / a.KL;
+  // lse of row l32 of the wave's units of the next stage; padding rows get +inf (probability 0), and so do rows whose lse is
+  // -inf (they saw no key)
+  constexpr int LSTEP = RS * QS * UROWS;
+  const int lg = LSTEP / a.KL, lq = LSTEP % a.KL;
+  const uint32_t l_step = lg + lq * a.H, l_wrap = 1 - a.KL * a.H;
+  const float* const lse_b = a.lse + (int64_t)b * a.KL * a.H + kvh * a.G;
+  int lr[QS], lrq[QS];
+  uint32_t lof[QS];
+#pragma unroll
+  for (int x = 0; x < QS; ++x) {
+    lr[x] = (wr * QS + x) * UROWS + l32;
+    lrq[x] = lr[x] % a.KL;
+    lof[x] = (uint32_t)lrq[x] * a.H + lr[x] / a.KL;
+  }
+  float l_nxt[QS];
   auto load_lse = [&]() __attribute__((always_inline)) {
-    float l = INFINITY;
-    if (lr < a.rows) l = *lp;
-    lr += UROWS;
-    lrq += lq;
-    const bool wrap = lrq >= a.KL;
-    lrq -= wrap ? a.KL : 0;
-    lp += l_step + (wrap ? l_wrap : 0);
-    return l;
+#pragma unroll
+    for (int x = 0; x < QS; ++x) {
+      l_nxt[x] = INFINITY;
+      if (lr[x] < a.rows) l_nxt[x] = lse_b[lof[x]];
+      lr[x] += LSTEP;
+      lrq[x] += lq;
+      const bool wrap = lrq[x] >= a.KL;
+      lrq[x] -= wrap ? a.KL : 0;
+      lof[x] += l_step + (wrap ? l_wrap : 0);
+    }
   };
 
   // keys of this wave: 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i, 32 rows through LDS at a time
   const int base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
   bf16x8 kf[2][D / 16];
+  const uint8_t* const kc_h = a.kc + (int64_t)kvh * a.kc_sh + (lane & 7) * 16;
+  int bad = 0;
+  auto load_key = [&](int key, u32x4& c, float& s) __attribute__((always_inline)) {
+    int e = trow[min(key, ctx - 1) >> shift];
+    if ((uint32_t)e >= (uint32_t)a.pages.num_pages) {
+      bad = 1;
+      e = 0;
+    }
+    c = *reinterpret_cast<const u32x4*>(slot_row(kc_h, (e << shift) + (min(key, ctx - 1) & pmask), (uint32_t)a.kc_ss));
+    s = a.ks[e * a.Hkv + kvh];
+  };
+  auto read_keys = [&](int ks, const uint8_t* tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) kf[ks][d] = as_bf16x8(*reinterpret_cast<const u16x8*>(tile + k_operand(lane) + 32 * d));
+  };
   {
-    const int r0 = lane >> 3, part = lane & 7;
-    const uint8_t* kc_h = a.kc + (int64_t)kvh * a.kc_sh + part * 16;
+    // 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i, 32 rows through the wave's part of LDS at a time
     uint8_t* tile = lds + w * (SK * KROW);
-    int bad = 0;
-    int e[8];
     u32x4 c[8];
     float sc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = min(lo + w * TK + r0 + 8 * i, ctx - 1);
-      e[i] = trow[key >> shift];
-      if ((uint32_t)e[i] >= (uint32_t)a.pages.num_pages) {
-        bad = 1;
-        e[i] = 0;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = min(lo + w * TK + r0 + 8 * i, ctx - 1);
-      c[i] = *reinterpret_cast<const u32x4*>(slot_row(kc_h, (e[i] << shift) + (key & pmask), (uint32_t)a.kc_ss));
-      sc[i] = a.ks[e[i] * a.Hkv + kvh];
-    }
-    if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+    for (int i = 0; i < 8; ++i) load_key(lo + wk * TK + (lane >> 3) + 8 * i, c[i], sc[i]);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) put_k_codes(tile + (r0 + 8 * i) * KROW, part, c[4 * ks + i], sc[4 * ks + i]);
+      for (int i = 0; i < 4; ++i) put_k_codes(tile + ((lane >> 3) + 8 * i) * KROW, lane & 7, c[4 * ks + i], sc[4 * ks + i]);
       asm volatile("" ::: "memory");  // (a wave's LDS operations complete in order)
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d)
-        kf[ks][d] = as_bf16x8(*reinterpret_cast<const u16x8*>(tile + k_operand(lane) + 32 * d));
+      read_keys(ks, tile);
       asm volatile("" ::: "memory");
     }
   }
+  if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   lds_barrier();
   float acc[32];
 #pragma unroll
   for (int x = 0; x < 32; ++x) acc[x] = 0.f;
   load_q(0);
-  float l_nxt = load_lse();
+  load_lse();
   wait_vmcnt0();
   lds_barrier();
   for (int st = 0; st < stages; ++st) {
-    if (st + 1 < stages) load_q((st + 1) & 1);  // (that buffer was last read in stage st - 1)
+    float l[QS];
+    // (opaque here: formed at the end of the last stage instead, l would wait there for the loads just issued)
+#pragma unroll
+    for (int x = 0; x < QS; ++x) asm volatile("" : "+v"(l_nxt[x]));
+#pragma unroll
+    for (int x = 0; x < QS; ++x) l[x] = l_nxt[x] == -INFINITY ? INFINITY : l_nxt[x] * 1.4426950408889634f;
+    if (st + 1 < stages) {  // (that buffer was last read in stage st - 1)
+      load_q(st + 1);
+      load_lse();
+    }
+    // (units past the last are computed with the rest: a test would part one unit's products from the other's exponentials)
 #pragma unroll
     for (int x = 0; x < QS; ++x) {
-      const uint16_t* qb = reinterpret_cast<const uint16_t*>(lds) + ((st & 1) * QS + x) * (UROWS * D);
-      const float l = l_nxt == -INFINITY ? INFINITY : l_nxt * 1.4426950408889634f;
-      l_nxt = load_lse();
+      const uint16_t* qb = reinterpret_cast<const uint16_t*>(lds + (st & 1) * STAGE) + (wr * QS + x) * (UROWS * D);
       f32x16 s0 = {}, s1 = {};
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
@@ -1126,8 +1153,8 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, 
       }
 #pragma unroll
       for (int y = 0; y < 16; ++y) {
-        acc[y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[y], a.scale_log2, -l));
-        acc[16 + y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[y], a.scale_log2, -l));
+        acc[y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[y], a.scale_log2, -l[x]));
+        acc[16 + y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[y], a.scale_log2, -l[x]));
       }
     }
     wait_vmcnt0();
@@ -1136,19 +1163,34 @@ __global__ __launch_bounds__(WNW * 64) __attribute__((amdgpu_waves_per_eu(WOCC, 
   // Sum over the 32 lanes of a half, halving the registers as the lanes are joined: in step m a lane keeps the half of its
   // registers that its bit m names and gives the other half to lane ^ m. Register x ends in the lane whose bits 4 .. 0
   // (m = 16, 8, 4, 2, 1) spell x.
-#pragma unroll
-  for (int n = 16; n >= 1; n >>= 1) {
+  auto join = [&](auto step) __attribute__((always_inline)) {
+    constexpr int n = decltype(step)::value;
     const bool up = (l32 & n) != 0;
 #pragma unroll
     for (int x = 0; x < n; ++x) {
       const float give = up ? acc[x] : acc[x + n], keep = up ? acc[x + n] : acc[x];
       acc[x] = keep + __shfl_xor(give, n);
     }
+  };
+  join(std::integral_constant<int, 16>{});
+  join(std::integral_constant<int, 8>{});
+  join(std::integral_constant<int, 4>{});
+  join(std::integral_constant<int, 2>{});
+  join(std::integral_constant<int, 1>{});
+  const int x = l32 & 15, in_tile = (l32 >> 4) * 32 + 8 * (x >> 2) + 4 * half + (x & 3);
+  float sum = acc[0];
+  if constexpr (RS == 2) {
+    // (behind the loop's last barrier: the query rows are read)
+    float* const part = reinterpret_cast<float*>(lds);
+    if (wr == 1) part[wk * TK + in_tile] = sum;
+    lds_barrier();
+    if (wr == 1) return;
+    sum += part[wk * TK + in_tile];
   }
-  const int x = l32 & 15, key = lo + w * TK + (l32 >> 4) * 32 + 8 * (x >> 2) + 4 * half + (x & 3);
+  const int key = lo + wk * TK + in_tile;
   if (key < ctx) {
     float* p = a.w + wrow * a.w_sr + (int64_t)kvh * a.w_sh + key;
-    *p = a.decay != 0.f ? a.decay * *p + acc[0] : acc[0];  // (a decay of 0 does not read the old sum)
+    *p = a.decay != 0.f ? a.decay * *p + sum : sum;  // (a decay of 0 does not read the old sum)
   }
 }
 
@@ -1236,8 +1278,10 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
   const int64_t grid = units == 1 ? programs : (programs + 7) / 8 * 8 * a.ngroups;
   if (grid > 0x7fffffff || (prows + 15) / 16 > 0x7fffffff)
     return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
-  if (units == 1)
-    hipLaunchKernelGGL(kv8_attn_stream_kernel, dim3((unsigned)grid), dim3(SNW * 64), 0, st, a);
+  if (units == 1 && grid <= mfd_num_cus())
+    hipLaunchKernelGGL(kv8_attn_stream_kernel<8>, dim3((unsigned)grid), dim3(512), 0, st, a);
+  else if (units == 1)
+    hipLaunchKernelGGL(kv8_attn_stream_kernel<4>, dim3((unsigned)grid), dim3(256), 0, st, a);
   else if (NW == 8 && page_size >= TK)
     hipLaunchKernelGGL((kv8_attn_tile_kernel<8, true>), dim3((unsigned)grid), dim3(512), 0, st, a);
   else if (NW == 8)
@@ -1266,6 +1310,9 @@ extern "C" int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, co
                             table_width, num_pages);
   if (rc == MFD_OK) rc = check_attn(who, bs, num_modes, block_size, H, Hkv, scale, q, q_st, q_sh);
   if (rc != MFD_OK) return rc;
+  if (q_st < 0 || q_sh < 0 || (int64_t)num_modes * block_size * q_st + (int64_t)H * q_sh >= (1 << 30) ||
+      (int64_t)num_modes * block_size * H >= (1 << 30))
+    return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: a request's queries must span less than 2^30 elements", who);
   if (w_rows < 0 || width < 0 || !(decay >= 0.f && decay <= 1.f))
     return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: bad weights rows=%d width=%d, or decay %g outside [0, 1]", who, w_rows,
                          width, (double)decay);
@@ -1285,7 +1332,10 @@ extern "C" int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, co
   const int64_t keys = std::min<int64_t>(width, (int64_t)table_width * page_size);
   const int64_t grid = (keys + WKEYS - 1) / WKEYS * Hkv * bs;
   if (grid > 0x7fffffff) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
-  hipLaunchKernelGGL(kv8_weights_kernel, dim3((unsigned)grid), dim3(WNW * 64), 0, static_cast<hipStream_t>(stream), a);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a.rows <= UROWS) hipLaunchKernelGGL((kv8_weights_kernel<1, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else if (grid > mfd_num_cus()) hipLaunchKernelGGL((kv8_weights_kernel<1, 2>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv8_weights_kernel<2, 2>), dim3((unsigned)grid), dim3(512), 0, st, a);
   MFD_CHECK_LAUNCH();
   return MFD_OK;
 }
