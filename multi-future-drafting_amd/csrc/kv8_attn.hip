@@ -1009,7 +1009,7 @@ struct WArgs {
 };
 
 template <int RS, int QS>
-__global__ __launch_bounds__(RS * 256) __attribute__((amdgpu_waves_per_eu(RS == 1 ? 3 : 2, RS == 1 ? 3 : 2)))
+__global__ __launch_bounds__(RS * 256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void kv8_weights_kernel(WArgs a) {
   static_assert(RS <= 2 && QS <= 2, "one or two");
   constexpr int NWV = 4 * RS;
@@ -1127,39 +1127,78 @@ void kv8_weights_kernel(WArgs a) {
   for (int x = 0; x < 32; ++x) acc[x] = 0.f;
   load_q(0);
   load_lse();
-  wait_vmcnt0();
-  lds_barrier();
-  for (int st = 0; st < stages; ++st) {
-    float l[QS];
-    // (opaque here: formed at the end of the last stage instead, l would wait there for the loads just issued)
+  float l_st[QS];  // of the stage that is read, base 2
+  // Stage st has landed in every wave and the one before is read: its buffer takes the one behind
+  auto next_stage = [&](int st) __attribute__((always_inline)) {
+    wait_vmcnt0();
+    lds_barrier();
 #pragma unroll
-    for (int x = 0; x < QS; ++x) asm volatile("" : "+v"(l_nxt[x]));
-#pragma unroll
-    for (int x = 0; x < QS; ++x) l[x] = l_nxt[x] == -INFINITY ? INFINITY : l_nxt[x] * 1.4426950408889634f;
-    if (st + 1 < stages) {  // (that buffer was last read in stage st - 1)
+    for (int x = 0; x < QS; ++x) {
+      asm volatile("" : "+v"(l_nxt[x]));  // (opaque: formed where it was asked for instead, l_st would wait for it there)
+      l_st[x] = l_nxt[x] == -INFINITY ? INFINITY : l_nxt[x] * 1.4426950408889634f;
+    }
+    if (st + 1 < stages) {
       load_q(st + 1);
       load_lse();
     }
-    // (units past the last are computed with the rest: a test would part one unit's products from the other's exponentials)
+  };
+  // S^T of the wave's unit n (n / QS: its stage), and meanwhile the probabilities of the one before: a wave's matrix and vector
+  // instructions overlap where they alternate (16 of v_mfma_f32_32x32x16, then 128 FMAs: 971 cycles, 776 with three waves per
+  // SIMD; each followed by 8 of them: 680 and 624). Slots 2 c and 2 c + 1 are the two 32-key subtiles against d chunk c, read FD
+  // chunks ahead; a scheduling barrier closes each slot. Units past the last are padding rows' (probability 0).
+  constexpr int FD = 2;
+  auto unit_step = [&](int n, bool first, bool more, float l, f32x16 (&cur)[2], f32x16 (&nxt)[2])
+                       __attribute__((always_inline)) {
+    const uint16_t* qb =
+        reinterpret_cast<const uint16_t*>(lds + (n / QS & 1) * STAGE) + (wr * QS + n % QS) * (UROWS * D);
+    bf16x8 qf[D / 16];
+    if (more) {
 #pragma unroll
-    for (int x = 0; x < QS; ++x) {
-      const uint16_t* qb = reinterpret_cast<const uint16_t*>(lds + (st & 1) * STAGE) + (wr * QS + x) * (UROWS * D);
-      f32x16 s0 = {}, s1 = {};
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        const bf16x8 qf = as_bf16x8(*reinterpret_cast<const u16x8*>(qb + (base ^ (c << 4))));
-        s0 = mfma32(kf[0][c], qf, s0);
-        s1 = mfma32(kf[1][c], qf, s1);
-      }
-#pragma unroll
-      for (int y = 0; y < 16; ++y) {
-        acc[y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[y], a.scale_log2, -l[x]));
-        acc[16 + y] += __builtin_amdgcn_exp2f(__builtin_fmaf(s1[y], a.scale_log2, -l[x]));
-      }
+      for (int c = 0; c < FD; ++c) qf[c] = as_bf16x8(*reinterpret_cast<const u16x8*>(qb + (base ^ (c << 4))));
+      nxt[0] = nxt[1] = (f32x16){};
     }
-    wait_vmcnt0();
-    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int sl = 0; sl < 16; ++sl) {
+      const int c = sl >> 1, ks = sl & 1;
+      if (more) {
+        if (ks == 0 && c + FD < D / 16)
+          qf[c + FD] = as_bf16x8(*reinterpret_cast<const u16x8*>(qb + (base ^ ((c + FD) << 4))));
+        nxt[ks] = mfma32(kf[ks][c], qf[c], nxt[ks]);
+      }
+      if (!first) {
+        asm volatile("" : "+v"(l));  // this and the one behind the sums keep the exponentials in this slot
+        acc[2 * sl] += __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 2][2 * (sl & 7)], a.scale_log2, -l));
+        acc[2 * sl + 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(cur[c >> 2][2 * (sl & 7) + 1], a.scale_log2, -l));
+        asm volatile("" : "+v"(acc[2 * sl]), "+v"(acc[2 * sl + 1]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  f32x16 s_a[2], s_b[2];
+  next_stage(0);
+  unit_step(0, true, true, 0.f, s_b, s_a);
+  const int n_units = stages * QS;
+  float l_cur = l_st[0];
+  // unit n - 1's probabilities are formed while unit n's products run
+  auto advance = [&](int n, f32x16 (&cur)[2], f32x16 (&nxt)[2]) __attribute__((always_inline)) {
+    const float l = l_cur;
+    if (QS == 1 || n % QS == 0) next_stage(n / QS);
+    l_cur = l_st[n % QS];
+    unit_step(n, false, true, l, cur, nxt);
+  };
+  int n = 1;
+  for (; n + 1 < n_units; n += 2) {
+    advance(n, s_a, s_b);
+    advance(n + 1, s_b, s_a);
   }
+  if (n < n_units) {
+    advance(n, s_a, s_b);
+    unit_step(0, false, false, l_cur, s_b, s_a);
+  } else {
+    unit_step(0, false, false, l_cur, s_a, s_b);
+  }
+  lds_barrier();
   // Sum over the 32 lanes of a half, halving the registers as the lanes are joined: in step m a lane keeps the half of its
   // registers that its bit m names and gives the other half to lane ^ m. Register x ends in the lane whose bits 4 .. 0
   // (m = 16, 8, 4, 2, 1) spell x.
