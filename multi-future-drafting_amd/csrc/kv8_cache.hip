@@ -8,10 +8,9 @@
 // rows behind the new ones. Bound by memory for prompts, by latency for the few tokens of a round.
 //
 // Selection. score[t] = the sum over KV heads of weights[h][t], formed in fp64 and rounded once to fp32, so that the
-// order of the sum cannot decide which token stays. One kernel turns scores into 32-bit keys whose unsigned order is the
-// scores' (always-kept tokens at the top, NaN at the bottom); a second, one workgroup per request, finds the budget-th
-// largest by three histogram passes over 11, 11 and 10 bits and writes the kept indices ascending by one prefix sum.
-// Ties at the border go to the lowest index.
+// order of the sum cannot decide which token stays. Scores become 32-bit keys whose unsigned order is the scores' (always-kept
+// tokens at the top, NaN at the bottom); one workgroup per request finds the budget-th largest by three histogram passes over
+// 11, 11 and 10 bits and writes the kept indices ascending by one prefix sum. Ties at the border go to the lowest index.
 //
 // Compaction. One workgroup per (destination page, KV head) of K or of V gathers its kept rows, finds their largest
 // magnitude, and writes them with a scale of their own; the same launch moves the running sums (a workgroup per request
@@ -152,27 +151,32 @@ __device__ __forceinline__ int select_len(const SelectArgs& a, int b) {
   return (int)max((int64_t)0, min(a.ctx_lens[b], (int64_t)a.width));
 }
 
-__global__ __launch_bounds__(256) void evict_score_kernel(SelectArgs a) {
-  const int b = blockIdx.y;
-  const int len = select_len(a, b);
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= len || len <= a.budget) return;  // (a request within the budget keeps everything)
-  const int64_t row = a.req_idx ? a.req_idx[b] : b;
-  const float* w = a.w + row * a.w_sr + t;
+// Key of token t of a request's row w: its score's, or the top one
+__device__ __forceinline__ uint32_t key_of(const SelectArgs& a, const float* w, int t, int len) {
   double sum = 0.;
   int h = 0;
   for (; h + 8 <= a.Hkv; h += 8) {
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = w[(h + j) * a.w_sh];
+    for (int j = 0; j < 8; ++j) x[j] = w[(h + j) * a.w_sh + t];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum += (double)x[j];
   }
-  for (; h < a.Hkv; ++h) sum += (double)w[h * a.w_sh];
+  for (; h < a.Hkv; ++h) sum += (double)w[h * a.w_sh + t];
   const float score = (float)sum + 0.f;  // -0 as +0
-  uint32_t key = score == score ? float_order_key(score) : 0u;
-  if (t < a.sink || t >= len - a.recent) key = ALWAYS;
-  a.keys[b * a.key_stride + t] = key;
+  const uint32_t key = score == score ? float_order_key(score) : 0u;
+  return t < a.sink || t >= len - a.recent ? ALWAYS : key;
+}
+__device__ __forceinline__ const float* weight_row(const SelectArgs& a, int b) {
+  return a.w + (a.req_idx ? a.req_idx[b] : b) * a.w_sr;
+}
+
+__global__ __launch_bounds__(256) void evict_score_kernel(SelectArgs a) {
+  const int b = blockIdx.y;
+  const int len = select_len(a, b);
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= len || len <= a.budget) return;  // (a request within the budget keeps everything)
+  a.keys[b * a.key_stride + t] = key_of(a, weight_row(a, b), t, len);
 }
 
 // Exclusive prefix sum of v over the workgroup's ST threads, and the total; buf: ST / 64 words. Two barriers.
@@ -198,10 +202,18 @@ __device__ __forceinline__ int group_scan(int v, int* buf, int& total) {
   return before + s - v;
 }
 
+// NK > 0: requests of at most NK ST tokens, whose keys are formed here and stay in registers (key i of a thread: token i ST +
+// thread). 0: longer ones, whose keys evict_score_kernel left in the workspace.
+template <int NK>
 __global__ __launch_bounds__(ST) void evict_select_kernel(SelectArgs a) {
-  __shared__ int hist[2048];
-  __shared__ int buf[ST / 64];
+  constexpr int NW = ST / 64;
+  // each bin COPIES times, one for every lane modulo COPIES: a wave's keys share few bins (the first digit is little more than
+  // the exponent), and adds to one word go one after the other
+  constexpr int COPIES = 8;
+  __shared__ __attribute__((aligned(16))) int hist[2048 * COPIES];
+  __shared__ int buf[NW];
   __shared__ uint32_t found[2];  // digit, and how many of its bin are still wanted
+  __shared__ int counts[NK > 0 ? 2 * NK * NW : 1];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int len = select_len(a, b);
   const int n = min(len, a.budget);
@@ -217,6 +229,15 @@ __global__ __launch_bounds__(ST) void evict_select_kernel(SelectArgs a) {
     for (int i = tid; i < n; i += ST) keep[i] = i;
     return;
   }
+  uint32_t key[NK > 0 ? NK : 1];
+  if constexpr (NK > 0) {
+    const float* w = weight_row(a, b);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int t = i * ST + tid;
+      key[i] = t < len ? key_of(a, w, t, len) : 0u;
+    }
+  }
   const uint32_t* keys = a.keys + b * a.key_stride;
   // the n-th largest key, digit by digit: `prefix` holds the digits found, `want` how many keys with them are kept
   uint32_t prefix = 0, mask = 0;
@@ -224,17 +245,31 @@ __global__ __launch_bounds__(ST) void evict_select_kernel(SelectArgs a) {
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < bins; i += ST) hist[i] = 0;
+    auto bin_of = [&](uint32_t digit) { return &hist[(digit & (bins - 1)) * COPIES + (tid & (COPIES - 1))]; };
+    auto count = [&](bool in, uint32_t k) {
+      if (in) atomicAdd(bin_of(k >> shift), 1);
+    };
+    auto bin_sum = [&](int d) {
+      const u32x4 x = reinterpret_cast<const u32x4*>(hist)[2 * d], y = reinterpret_cast<const u32x4*>(hist)[2 * d + 1];
+      return (int)(x[0] + x[1] + x[2] + x[3] + y[0] + y[1] + y[2] + y[3]);
+    };
+    for (int i = 4 * tid; i < bins * COPIES; i += 4 * ST) *reinterpret_cast<u32x4*>(hist + i) = (u32x4){};
     __syncthreads();
-    for (int i = 4 * tid; i < len; i += 4 * ST) {
-      const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);  // rows are padded to whole quads
+    if constexpr (NK > 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < len && (k[e] & mask) == prefix) atomicAdd(&hist[(k[e] >> shift) & (bins - 1)], 1);
+      for (int i = 0; i < NK; ++i)
+        count(i * ST + tid < len && (key[i] & mask) == prefix, key[i]);
+    } else {
+      for (int i = 4 * tid; i < len; i += 4 * ST) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);  // rows are padded to whole quads
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          count(i + e < len && (k[e] & mask) == prefix, k[e]);
+      }
     }
     __syncthreads();
     const int hi = bins - 1 - 2 * tid;  // this thread's bins hi, hi - 1: descending over the threads
-    const int h0 = hi >= 1 ? hist[hi] : 0, h1 = hi >= 1 ? hist[hi - 1] : 0;
+    const int h0 = hi >= 1 ? bin_sum(hi) : 0, h1 = hi >= 1 ? bin_sum(hi - 1) : 0;
     int total;
     const int before = group_scan(h0 + h1, buf, total);
     if (before < want && want <= before + h0) {
@@ -249,30 +284,63 @@ __global__ __launch_bounds__(ST) void evict_select_kernel(SelectArgs a) {
     mask |= (uint32_t)(bins - 1) << shift;
     want = (int)found[1];
   }
-  // kept: keys above the border `prefix`, and the first `want` of those equal to it. A thread takes a run of the row.
-  const int seg = ((len + ST - 1) / ST + 3) & ~3;
-  const int lo = tid * seg, hi = min(lo + seg, len);
-  int gt = 0, eq = 0;
-  for (int i = lo; i < hi; i += 4) {
-    const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+  // kept: keys above the border `prefix`, and the first `want` of those equal to it
+  if constexpr (NK > 0) {
+    // token order is (register, wave, lane): the wave's counts of each register meet in LDS, one prefix sum over them
+    const int lane = tid & 63, w = tid >> 6;
+    uint64_t above[NK], same[NK];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      gt += (i + e < hi && k[e] > prefix) ? 1 : 0;
-      eq += (i + e < hi && k[e] == prefix) ? 1 : 0;
+    for (int i = 0; i < NK; ++i) {
+      const bool in = i * ST + tid < len;
+      above[i] = __builtin_amdgcn_ballot_w64(in && key[i] > prefix);
+      same[i] = __builtin_amdgcn_ballot_w64(in && key[i] == prefix);
+      if (lane == 0) {
+        counts[i * NW + w] = __builtin_popcountll(above[i]);
+        counts[(NK + i) * NW + w] = __builtin_popcountll(same[i]);
+      }
     }
-  }
-  int total;
-  const int gt0 = group_scan(gt, buf, total);
-  int eq0 = group_scan(eq, buf, total);
-  int at = gt0 + min(eq0, want);
-  for (int i = lo; i < hi; i += 4) {
-    const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+    __syncthreads();
+    static_assert(2 * NK * NW <= ST, "a count per thread");
+    int total;
+    const int c = tid < 2 * NK * NW ? counts[tid] : 0;
+    const int before = group_scan(c, buf, total);
+    if (tid < 2 * NK * NW) counts[tid] = before;
+    __syncthreads();
+    const int gt_all = counts[NK * NW];  // (what lies before the first of the equal ones)
+    const uint64_t lower = ((uint64_t)1 << lane) - 1;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (i + e >= hi) break;
-      const bool same = k[e] == prefix;
-      if (k[e] > prefix || (same && eq0 < want)) keep[at++] = i + e;
-      eq0 += same ? 1 : 0;
+    for (int i = 0; i < NK; ++i) {
+      const int gt0 = counts[i * NW + w] + __builtin_popcountll(above[i] & lower);
+      const int eq0 = counts[(NK + i) * NW + w] - gt_all + __builtin_popcountll(same[i] & lower);
+      const bool is_above = above[i] >> lane & 1, is_same = same[i] >> lane & 1;
+      if (is_above || (is_same && eq0 < want)) keep[gt0 + min(eq0, want)] = i * ST + tid;
+    }
+  } else {
+    // a thread takes a run of the row
+    const int seg = ((len + ST - 1) / ST + 3) & ~3;
+    const int lo = tid * seg, hi = min(lo + seg, len);
+    int gt = 0, eq = 0;
+    for (int i = lo; i < hi; i += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        gt += (i + e < hi && k[e] > prefix) ? 1 : 0;
+        eq += (i + e < hi && k[e] == prefix) ? 1 : 0;
+      }
+    }
+    int total;
+    const int gt0 = group_scan(gt, buf, total);
+    int eq0 = group_scan(eq, buf, total);
+    int at = gt0 + min(eq0, want);
+    for (int i = lo; i < hi; i += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (i + e >= hi) break;
+        const bool same = k[e] == prefix;
+        if (k[e] > prefix || (same && eq0 < want)) keep[at++] = i + e;
+        eq0 += same ? 1 : 0;
+      }
     }
   }
 }
@@ -468,11 +536,18 @@ extern "C" int mfd_evict_select(const float* weights, int64_t w_row_stride, int6
   SelectArgs a{weights, w_row_stride, w_head_stride, w_rows, width, Hkv, req_idx, ctx_lens, budget, sink, recent, keep,
                new_lens, static_cast<uint32_t*>(workspace), key_stride_of(width), err_flag};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (width > budget) {  // (a shorter row holds no request above the budget: nothing to score)
-    hipLaunchKernelGGL(evict_score_kernel, dim3((unsigned)((width + 255) / 256), (unsigned)bs), dim3(256), 0, st, a);
-    MFD_CHECK_LAUNCH();
+  // keys in registers up to 16 per thread; beyond, a kernel of its own forms them (all CUs read the sums, not one per request)
+  if (width <= 8 * ST) {
+    hipLaunchKernelGGL(evict_select_kernel<8>, dim3((unsigned)bs), dim3(ST), 0, st, a);
+  } else if (width <= 16 * ST) {
+    hipLaunchKernelGGL(evict_select_kernel<16>, dim3((unsigned)bs), dim3(ST), 0, st, a);
+  } else {
+    if (width > budget) {  // (a shorter row holds no request above the budget: nothing to score)
+      hipLaunchKernelGGL(evict_score_kernel, dim3((unsigned)((width + 255) / 256), (unsigned)bs), dim3(256), 0, st, a);
+      MFD_CHECK_LAUNCH();
+    }
+    hipLaunchKernelGGL(evict_select_kernel<0>, dim3((unsigned)bs), dim3(ST), 0, st, a);
   }
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)bs), dim3(ST), 0, st, a);
   MFD_CHECK_LAUNCH();
   return MFD_OK;
 }

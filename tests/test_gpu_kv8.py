@@ -258,6 +258,8 @@ EVICT = [
     ([100, 7, 0, 64], 20, 4, 8, 2, 16, "normal"), ([1000, 300, 301], 300, 4, 32, 8, 64, "ties"),
     ([500], 64, 0, 0, 1, 16, "zero"), ([4100, 5000], 1025, 4, 32, 2, 32, "normal"), ([77], 1, 0, 0, 3, 16, "normal"),
     ([300, 5], 40, 40, 0, 2, 64, "ties"), ([300], 36, 4, 32, 2, 128, "normal"), ([900, 640], 200, 3, 5, 2, 256, "odd"),
+    ([8187, 9000], 3000, 4, 32, 9, 64, "ties"), ([9000, 16379], 2500, 4, 32, 2, 64, "odd"),  # keys in 8 and 16 registers
+    ([20000, 16385, 900], 1500, 4, 32, 3, 64, "odd"), ([17000], 16000, 0, 1, 1, 128, "ties"),  # .. and in the workspace
 ]
 
 
