@@ -16,6 +16,7 @@ from typing import Optional
 import torch
 
 import mfd_hip
+import mxfp4_head
 import tree_build_ext
 import tree_logits
 
@@ -211,15 +212,22 @@ class DDTreeDraftTopK:
     over the drafted rows, read in place (csrc/draft_head.hip: a hand-written weight-stream GEMM into a static
     bf16 logits buffer), then the logits step (csrc/logits_topk.hip): their top-k log-probabilities (bf16 value
     minus an fp32 log Z), token ids and log Z. With a reduced draft vocabulary, ``weight`` holds the LM head's
-    rows of ``vocab_ids`` (int32 [N]) and the winning columns are mapped back to full-vocabulary ids. Every buffer
-    is sized at construction for ``max_bs`` requests: a call allocates nothing (for bf16 hidden states with
-    16-byte aligned rows), so it can be captured in a graph."""
+    rows of ``vocab_ids`` (int32 [N]) and the winning columns are mapped back to full-vocabulary ids. ``weight`` is a bf16
+    matrix or an mxfp4_head.Mxfp4Weight (the head in 4 bits, csrc/mxfp4_head.hip: the same call, a quarter of the weight's
+    bytes). Every buffer is sized at construction for ``max_bs`` requests: a call allocates nothing (for bf16 hidden states
+    with 16-byte aligned rows), so it can be captured in a graph."""
 
     def __init__(self, *, weight: torch.Tensor, block_size: int, num_modes: int, budget: int, max_bs: int,
                  vocab_ids: Optional[torch.Tensor] = None):
-        mfd_hip.require_cuda(weight, vocab_ids)
+        self.mxfp4 = isinstance(weight, mxfp4_head.Mxfp4Weight)
         vocab, hidden = weight.shape
-        if weight.dtype != torch.bfloat16 or not weight.is_contiguous() or weight.data_ptr() % 16 or hidden % 64:
+        if self.mxfp4:
+            mxfp4_head.check_weight(weight.codes, weight.exps, values=True)
+            mfd_hip.require_cuda(weight.codes, weight.exps, vocab_ids)
+        else:
+            mfd_hip.require_cuda(weight, vocab_ids)
+        if not self.mxfp4 and (weight.dtype != torch.bfloat16 or not weight.is_contiguous() or weight.data_ptr() % 16 or
+                               hidden % 64):
             raise ValueError(f"weight must be a contiguous bf16 [vocab, hidden] matrix with hidden % 64 == 0, got "
                              f"{weight.dtype} {tuple(weight.shape)}")
         if vocab_ids is not None and (vocab_ids.dtype != torch.int32 or tuple(vocab_ids.shape) != (vocab,)):
@@ -258,8 +266,9 @@ class DDTreeDraftTopK:
         if n > self.logits.shape[0]:
             raise ValueError(f"{n} drafted rows exceed the {self.logits.shape[0]} of max_bs={self.max_bs}")
         rs = x.stride(0)
-        mfd_hip.call("mfd_draft_topk_head", x.data_ptr() + rs * 2, rs, L - 1, L * rs, self.weight.data_ptr(), n,
-                     self.vocab, H, self._logits.data_ptr(), self._logits.stride(0), self.topk,
+        weight = (self.weight.codes.data_ptr(), self.weight.exps.data_ptr()) if self.mxfp4 else (self.weight.data_ptr(),)
+        mfd_hip.call("mfd_draft_topk_head_mxfp4" if self.mxfp4 else "mfd_draft_topk_head", x.data_ptr() + rs * 2, rs, L - 1,
+                     L * rs, *weight, n, self.vocab, H, self._logits.data_ptr(), self._logits.stride(0), self.topk,
                      self.top_logp.data_ptr(), self.top_ids.data_ptr(), 0, self.log_z.data_ptr(),
                      mfd_hip.ptr(self.vocab_ids), self.workspace.data_ptr(), self.workspace.numel(),
                      mfd_hip.stream_of(x))

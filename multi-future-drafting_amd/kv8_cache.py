@@ -142,11 +142,12 @@ def kv8_store(*, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ks, vs = _rows(k, n, heads, "k"), _rows(v, n, heads, "v")
     if cu_tokens.dtype is not torch.int32 or cu_tokens.dim() != 1 or bs < 0 or not cu_tokens.is_contiguous():
         raise ValueError(f"cu_tokens must be contiguous int32 [bs + 1], got {cu_tokens.dtype} {tuple(cu_tokens.shape)}")
+    table = _table_args(page_table)
+    rows, starts = _index(req_pool_indices, bs, "req_pool_indices"), _index(start_lens, bs, "start_lens")
     device = _device_of(k, v, k_cache, v_cache, k_scale, v_scale, page_table, req_pool_indices, start_lens, cu_tokens,
                         err_flag)
-    rows, starts = _index(req_pool_indices, bs, "req_pool_indices"), _index(start_lens, bs, "start_lens")
     mfd_hip.call_on(device, "mfd_kv8_store", k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], *cache,
-                    *_table_args(page_table), page_size, rows.data_ptr(), starts.data_ptr(), cu_tokens.data_ptr(), n, bs,
+                    *table, page_size, rows.data_ptr(), starts.data_ptr(), cu_tokens.data_ptr(), n, bs,
                     max_tokens, heads, HEAD_DIM, _err(err_flag))
 
 
@@ -229,9 +230,10 @@ def paged_mode_block_attention_kv8(
         new = (k_new.data_ptr(), v_new.data_ptr(), ks[0], ks[1], vs[0], vs[1])
     else:
         new = (None, None, 0, 0, 0, 0)
+    table = _table_args(page_table)
+    rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
     device = _device_of(q, k_new, v_new, k_cache, v_cache, k_scale, v_scale, page_table, req_pool_indices, ctx_lens, out,
                         lse_out, workspace, err_flag)
-    table = _table_args(page_table)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, H, HEAD_DIM))
     os = _rows(out, T, H, "out")
@@ -251,7 +253,6 @@ def paged_mode_block_attention_kv8(
         if splits > 1:
             need = mfd_hip.lib().mfd_kv8_attn_workspace_bytes(bs, num_modes, block_size, H, heads, fresh, splits)
             workspace = _scratch(workspace, need, q)
-        rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
         mfd_hip.call_on(device, "mfd_kv8_attn", q.data_ptr(), qs[0], qs[1], *new, *cache, *table, page_size,
                         rows.data_ptr(), lens.data_ptr(), bs, num_modes, block_size, H, heads, HEAD_DIM, scaling,
                         1 if causal_in_block else 0, splits, keys, out.data_ptr(), os[0], os[1],
@@ -297,12 +298,12 @@ def attention_weights_kv8(*, q: torch.Tensor, lse: torch.Tensor, k_cache: torch.
     bs, H, qs = _query(q, heads, num_modes, block_size)
     if lse.dtype is not torch.float32 or tuple(lse.shape) != (q.shape[0], H) or not lse.is_contiguous():
         raise ValueError(f"lse must be contiguous float32 [{q.shape[0]}, {H}], got {lse.dtype} {tuple(lse.shape)}")
-    device = _device_of(q, lse, k_cache, k_scale, page_table, req_pool_indices, ctx_lens, weights, err_flag)
+    table, sums = _table_args(page_table), _weights_args(weights, heads)
     rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
+    device = _device_of(q, lse, k_cache, k_scale, page_table, req_pool_indices, ctx_lens, weights, err_flag)
     mfd_hip.call_on(device, "mfd_kv8_weights", q.data_ptr(), qs[0], qs[1], lse.data_ptr(), cache[0], cache[2], cache[3],
-                    cache[6], cache[8], *_table_args(page_table), page_size, rows.data_ptr(), lens.data_ptr(), bs,
-                    num_modes, block_size, H, heads, HEAD_DIM, scaling, decay, *_weights_args(weights, heads),
-                    _err(err_flag))
+                    cache[6], cache[8], *table, page_size, rows.data_ptr(), lens.data_ptr(), bs, num_modes, block_size, H,
+                    heads, HEAD_DIM, scaling, decay, *sums, _err(err_flag))
 
 
 def evict_select(*, weights: torch.Tensor, req_pool_indices: torch.Tensor, ctx_lens: torch.Tensor, budget: int,
@@ -315,15 +316,15 @@ def evict_select(*, weights: torch.Tensor, req_pool_indices: torch.Tensor, ctx_l
     behind them; new_lens [bs] int64). bs is ctx_lens' length."""
     bs, heads = ctx_lens.shape[0], weights.shape[1]
     sums = _weights_args(weights, heads)
-    device = _device_of(weights, req_pool_indices, ctx_lens, keep_out, new_lens_out, workspace, err_flag)
+    rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
     keep = weights.new_empty((bs, budget), dtype=torch.int32) if keep_out is None else keep_out
     new_lens = weights.new_empty(bs, dtype=torch.int64) if new_lens_out is None else new_lens_out
     if keep.dtype is not torch.int32 or tuple(keep.shape) != (bs, budget) or not keep.is_contiguous() or \
             new_lens.dtype is not torch.int64 or tuple(new_lens.shape) != (bs,) or not new_lens.is_contiguous():
         raise ValueError(f"keep_out must be contiguous int32 [{bs}, {budget}] and new_lens_out int64 [{bs}]")
+    device = _device_of(weights, req_pool_indices, ctx_lens, keep_out, new_lens_out, workspace, err_flag)
     need = mfd_hip.lib().mfd_evict_select_workspace_bytes(bs, sums[4])
     workspace = _scratch(workspace, need, weights)
-    rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
     mfd_hip.call_on(device, "mfd_evict_select", *sums, heads, rows.data_ptr(), lens.data_ptr(), bs, budget, sink, recent,
                     keep.data_ptr(), new_lens.data_ptr(), workspace.data_ptr() if need else None, need, _err(err_flag))
     return keep, new_lens
@@ -342,14 +343,14 @@ def evict_compact_kv8(*, keep: torch.Tensor, new_lens: torch.Tensor, ctx_lens: t
     bs, budget = keep.shape
     if keep.dtype is not torch.int32 or not keep.is_contiguous():
         raise ValueError(f"keep must be contiguous int32 [bs, budget], got {keep.dtype}")
-    device = _device_of(keep, new_lens, ctx_lens, k_cache, v_cache, k_scale, v_scale, src_table, dst_table,
-                        req_pool_indices, weights, err_flag)
+    src, dst = _table_args(src_table), _table_args(dst_table)
     sums = _weights_args(weights, heads) if weights is not None else (None, 0, 0, 0, 0)
     new, lens = _index(new_lens, bs, "new_lens"), _index(ctx_lens, bs, "ctx_lens")
     rows = _index(req_pool_indices, bs, "req_pool_indices")
+    device = _device_of(keep, new_lens, ctx_lens, k_cache, v_cache, k_scale, v_scale, src_table, dst_table,
+                        req_pool_indices, weights, err_flag)
     mfd_hip.call_on(device, "mfd_evict_compact_kv8", keep.data_ptr(), budget, new.data_ptr(), lens.data_ptr(), *cache,
-                    *_table_args(src_table), *_table_args(dst_table), page_size, rows.data_ptr(), *sums, bs, heads, HEAD_DIM,
-                    _err(err_flag))
+                    *src, *dst, page_size, rows.data_ptr(), *sums, bs, heads, HEAD_DIM, _err(err_flag))
 
 
 # ------------------------------------------------------------------------------------------------------------ pool

@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 
+import kv8_cache
 import mfd_hip
 import mode_attention
 
@@ -132,7 +133,11 @@ class PagedModeAttention:
     """The DFlashAttention hook (``mode_attention``, P:222-225; the reference class P:991-1026): q / k / v of
     the multi-mode draft forward arrive as [T, heads * D] slices of the fused qkv and leave as [T, H * D].
     ``impl``: "hip" (this library's kernel; "triton", the reference's name for its kernel, selects it too) or
-    "reference" (the float32 checking path)."""
+    "reference" (the float32 checking path).
+
+    A pool in 8 bits (kv8_cache.Kv8Pool, or any whose buffers are float8_e4m3fn and which has ``get_kv_scale(layer)``) is
+    read through kv8_cache.paged_mode_block_attention_kv8, ``req_to_token`` then being a page table of the pool's page
+    size (``forward_batch.seq_lens_cpu``, where there is one, tells it how far to split the contexts)."""
 
     _KERNELS = ("hip", "triton")
 
@@ -152,6 +157,8 @@ class PagedModeAttention:
         T = q.shape[0]
         bs = T // (K * L)
         k_cache, v_cache = self.kv_pool.get_kv_buffer(layer_id)
+        if k_cache.dtype == torch.float8_e4m3fn:
+            return self._kv8(q, k, v, k_cache, v_cache, forward_batch, layer_id)
         common = dict(q=q.view(T, H, D), k_new=k.view(T, Hkv, D), v_new=v.view(T, Hkv, D), k_cache=k_cache,
                       v_cache=v_cache, req_to_token=self.req_to_token,
                       req_pool_indices=forward_batch.req_pool_indices[:bs], ctx_lens=forward_batch.seq_lens[:bs],
@@ -160,4 +167,26 @@ class PagedModeAttention:
             o = paged_mode_block_attention_reference(**common).to(q.dtype)
         else:
             o = paged_mode_block_attention(**common, num_ctx_splits=self.num_ctx_splits)
+        return o.reshape(T, H * D)
+
+    def _kv8(self, q, k, v, k_cache, v_cache, forward_batch, layer_id: int) -> torch.Tensor:
+        H, Hkv, D = self.shape
+        K, L = self.blocks
+        T = q.shape[0]
+        bs = T // (K * L)
+        k_scale, v_scale = self.kv_pool.get_kv_scale(layer_id)
+        common = dict(q=q.view(T, H, D), k_new=k.view(T, Hkv, D), v_new=v.view(T, Hkv, D),
+                      req_pool_indices=forward_batch.req_pool_indices[:bs], ctx_lens=forward_batch.seq_lens[:bs],
+                      num_modes=K, block_size=L, scaling=self.scaling, page_size=self.page_size)
+        if self.exact:
+            o = paged_mode_block_attention_reference(
+                k_cache=kv8_cache.decode(k_cache, k_scale, self.page_size),
+                v_cache=kv8_cache.decode(v_cache, v_scale, self.page_size), req_to_token=self.req_to_token,
+                **common).to(q.dtype)
+        else:
+            lens = getattr(forward_batch, "seq_lens_cpu", None)  # only tunes the context splits
+            common["max_ctx"] = int(lens[:bs].max()) if lens is not None and bs else None
+            o = kv8_cache.paged_mode_block_attention_kv8(k_cache=k_cache, v_cache=v_cache, k_scale=k_scale,
+                                                         v_scale=v_scale, page_table=self.req_to_token,
+                                                         num_ctx_splits=self.num_ctx_splits, **common)
         return o.reshape(T, H * D)
