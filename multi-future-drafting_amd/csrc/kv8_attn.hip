@@ -225,8 +225,38 @@ __device__ __forceinline__ void split_range(const Args& a, int s, int ctx, int& 
   hi = ctx;
   if (a.SC > 1) {
     lo = (int)min((int64_t)s * a.split_keys, (int64_t)ctx);
-    if (s < a.SC - 1) hi = min(lo + a.split_keys, ctx);  // (the last split takes what a longer context has left)
+    if (s < a.SC - 1) hi = lo + min(a.split_keys, ctx - lo);  // (the last split takes what a longer context has left)
   }
+}
+
+// Infinities and NaN among the block's values: a product with them would be NaN in every row that shares the tile, also where
+// the key is masked (0 times infinity). They are staged as zeros, and the rows that see them take them by themselves.
+__device__ __forceinline__ bool has_nonfinite(const u32x4& x) {
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) any |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+  return any;
+}
+__device__ __forceinline__ void drop_nonfinite(u32x4& x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] &= (x[e] & 0x7f80u) == 0x7f80u ? 0xffff0000u : 0xffffffffu;
+    x[e] &= (x[e] & 0x7f800000u) == 0x7f800000u ? 0xffffu : 0xffffffffu;
+  }
+}
+// .. added to the accumulators of the rows (columns of O^T) that see the key; v: the key's values, from this half's d = 0
+__device__ __forceinline__ void add_nonfinite(const uint16_t* v, bool sees, f32x16 (&oacc)[D / 32]) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const u16x4 x = *reinterpret_cast<const u16x4*>(v + db * 32 + gq * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = bf2f(x[e]);
+        oacc[db][gq * 4 + e] += sees && !(fabsf(f) < INFINITY) ? f : 0.f;
+      }
+    }
 }
 
 // Index of a query row in the partials
@@ -245,6 +275,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   constexpr int RSTEP = NW * 8;
   __shared__ __attribute__((aligned(16))) uint8_t lds_k[2 * TK * KROW], lds_v[2 * TK * VROW];
   __shared__ uint32_t lds_vs[WHOLE ? 1 : 2 * TK];
+  __shared__ uint32_t lds_nf[2][TK / 32];  // block keys with infinities or NaN among their values, of this and the next tile
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
@@ -548,7 +579,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       bhi = ((g1 % KL) / Lb + 1) * Lb;
     }
     set_unit(0x3f800000u, unit, oacc);
-    for (int b0 = blo; b0 < bhi; b0 += TK) {
+    if (tid < TK / 32) lds_nf[0][tid] = 0;
+    int turn = 0;
+    for (int b0 = blo; b0 < bhi; b0 += TK, turn ^= 1) {
       lds_barrier();  // every wave is done with the buffers
 #pragma unroll
       for (int i = 0; i < NPT; ++i) {
@@ -556,11 +589,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const int64_t tk = (int64_t)b * KL + min(b0 + rr, bhi - 1);
         const u32x4* kp = reinterpret_cast<const u32x4*>(a.kn + tk * a.kn_st + (int64_t)kvh * a.kn_sh + part * 16);
         const u32x4* vp = reinterpret_cast<const u32x4*>(a.vn + tk * a.vn_st + (int64_t)kvh * a.vn_sh + part * 16);
-        const u32x4 kx = kp[0], ky = kp[1], vx = vp[0], vy = vp[1];
+        const u32x4 kx = kp[0], ky = kp[1];
+        u32x4 vx = vp[0], vy = vp[1];
+        if (has_nonfinite(vx) || has_nonfinite(vy)) {
+          drop_nonfinite(vx);
+          drop_nonfinite(vy);
+          atomicOr(&lds_nf[turn][rr >> 5], 1u << (rr & 31));
+        }
         put_row(lds_k + rr * KROW, part, kx, ky);
         put_row(lds_v + rr * VROW, part, vx, vy);
       }
       lds_barrier();
+      if (tid < TK / 32) lds_nf[turn ^ 1][tid] = 0;  // (read last in front of this tile's first barrier)
       const int klo = mode_lo - b0, khi = min(mode_lo + (causal ? qi - mode_lo + 1 : Lb), bhi) - b0;
       if (active && __builtin_amdgcn_ballot_w64(klo < TK && khi > 0) != 0) {
         f32x16 sv[2];
@@ -588,6 +628,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
           __builtin_amdgcn_sched_barrier(0);
         }
         l_run += psum;
+#pragma unroll 1
+        for (int x = 0; x < TK / 32; ++x) {
+          uint32_t nf = __builtin_amdgcn_readfirstlane(lds_nf[turn][x]);
+#pragma unroll 1
+          for (; nf; nf &= nf - 1) {
+            const int key = x * 32 + __builtin_ctz(nf);
+            const uint16_t* vp = a.vn + ((int64_t)b * KL + min(b0 + key, bhi - 1)) * a.vn_st + (int64_t)kvh * a.vn_sh;
+            add_nonfinite(vp + half * 4, key >= klo && key < khi, oacc);
+          }
+        }
       }
     }
   }
@@ -799,19 +849,28 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   // ---- the block keys (rows <= 32, so K L <= 32: one tile), in bf16 with P as a bf16 pair, by the last wave
   if (with_block && w == SNW - 1) {
     set_unit(0x3f800000u, unit, oacc);
+    uint32_t nf = 0;  // keys with infinities or NaN among their values
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int rr = r0 + 8 * i;
       const int64_t tk = (int64_t)b * KL + min(rr, KL - 1);
       const u32x4* kp = reinterpret_cast<const u32x4*>(a.kn + tk * a.kn_st + (int64_t)kvh * a.kn_sh + part * 16);
       const u32x4* vp = reinterpret_cast<const u32x4*>(a.vn + tk * a.vn_st + (int64_t)kvh * a.vn_sh + part * 16);
-      const u32x4 kx = kp[0], ky = kp[1], vx = vp[0], vy = vp[1];
+      const u32x4 kx = kp[0], ky = kp[1];
+      u32x4 vx = vp[0], vy = vp[1];
+      uint64_t lanes = __builtin_amdgcn_ballot_w64(has_nonfinite(vx) || has_nonfinite(vy));
+      if (lanes) {
+        drop_nonfinite(vx);
+        drop_nonfinite(vy);
+        for (; lanes; lanes &= lanes - 1) nf |= 1u << (8 * i + __builtin_ctzll(lanes) / 8);
+      }
       put_row(lds_k + rr * KROW, part, kx, ky);
       put_row(lds_v + rr * VROW, part, vx, vy);
     }
     asm volatile("" ::: "memory");
     f32x16 sv = scores();
-    const float msub = softmax_max(true, mode_lo, a.causal ? qi + 1 : mode_lo + Lb, sv);
+    const int khi = a.causal ? qi + 1 : mode_lo + Lb;
+    const float msub = softmax_max(true, mode_lo, khi, sv);
     float psum = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -832,6 +891,12 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
     }
     l_run += psum;
+#pragma unroll 1
+    for (; nf; nf &= nf - 1) {
+      const int key = __builtin_ctz(nf);
+      const uint16_t* vp = a.vn + ((int64_t)b * KL + min(key, KL - 1)) * a.vn_st + (int64_t)kvh * a.vn_sh;
+      add_nonfinite(vp + half * 4, key >= mode_lo && key < khi, oacc);
+    }
   }
   // ---- the waves' results: each brings its accumulators to the common reference and into its part of LDS as [row][d] fp32
   //      (16 KB); TPR threads per row add them in wave order
@@ -1149,6 +1214,11 @@ void kv8_weights_kernel(WArgs a) {
   constexpr int FD = 2;
   auto unit_step = [&](int n, bool first, bool more, float l, f32x16 (&cur)[2], f32x16 (&nxt)[2])
                        __attribute__((always_inline)) {
+    // rows that add nothing (lse -inf, padding): scores of infinities and NaN in their q must not make them NaN
+    if (!first && __builtin_amdgcn_ballot_w64(l == INFINITY) != 0) {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) cur[x >> 4][x & 15] = l == INFINITY ? 0.f : cur[x >> 4][x & 15];
+    }
     const uint16_t* qb =
         reinterpret_cast<const uint16_t*>(lds + (n / QS & 1) * STAGE) + (wr * QS + n % QS) * (UROWS * D);
     bf16x8 qf[D / 16];

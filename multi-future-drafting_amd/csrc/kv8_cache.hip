@@ -57,7 +57,8 @@ __global__ __launch_bounds__(NT) void kv8_store_kernel(StoreArgs a) {
   const int h = blockIdx.x % a.Hkv, pi = blockIdx.x / a.Hkv;
   const int shift = a.pages.page_shift, P = 1 << shift;
   const int c0 = max(0, min(a.cu_tokens[b], a.N)), c1 = max(c0, min(a.cu_tokens[b + 1], a.N));
-  const int64_t start = a.start_lens[b], end = start + (c1 - c0);
+  const int64_t start = max((int64_t)-1, min(a.start_lens[b], (int64_t)1 << 40));  // (beyond either: no table reaches there)
+  const int64_t end = start + (c1 - c0);
   if (c1 == c0) return;
   const int64_t p = (start >> shift) + pi;
   const int64_t p0 = p << shift;
@@ -142,7 +143,8 @@ struct SelectArgs {
   int32_t* err_flag;
 };
 
-constexpr int ST = 1024;  // threads of a selection workgroup
+constexpr int ST = 1024;      // threads of a selection workgroup
+constexpr int REG_KEYS = 16;  // keys of a thread that stay in registers, at most
 constexpr uint32_t ALWAYS = 0xFFFFFFFFu;
 
 __device__ __forceinline__ int select_len(const SelectArgs& a, int b) {
@@ -514,7 +516,7 @@ extern "C" int mfd_kv8_store(const uint16_t* k, const uint16_t* v, int64_t kn_st
 static int64_t key_stride_of(int width) { return ((int64_t)width + 3) & ~(int64_t)3; }
 
 extern "C" int64_t mfd_evict_select_workspace_bytes(int bs, int width) {
-  return bs > 0 && width > 0 ? (int64_t)bs * key_stride_of(width) * 4 : 0;
+  return bs > 0 && width > REG_KEYS * ST ? (int64_t)bs * key_stride_of(width) * 4 : 0;
 }
 
 extern "C" int mfd_evict_select(const float* weights, int64_t w_row_stride, int64_t w_head_stride, int w_rows,
@@ -539,8 +541,8 @@ extern "C" int mfd_evict_select(const float* weights, int64_t w_row_stride, int6
   // keys in registers up to 16 per thread; beyond, a kernel of its own forms them (all CUs read the sums, not one per request)
   if (width <= 8 * ST) {
     hipLaunchKernelGGL(evict_select_kernel<8>, dim3((unsigned)bs), dim3(ST), 0, st, a);
-  } else if (width <= 16 * ST) {
-    hipLaunchKernelGGL(evict_select_kernel<16>, dim3((unsigned)bs), dim3(ST), 0, st, a);
+  } else if (width <= REG_KEYS * ST) {
+    hipLaunchKernelGGL(evict_select_kernel<REG_KEYS>, dim3((unsigned)bs), dim3(ST), 0, st, a);
   } else {
     if (width > budget) {  // (a shorter row holds no request above the budget: nothing to score)
       hipLaunchKernelGGL(evict_score_kernel, dim3((unsigned)((width + 255) / 256), (unsigned)bs), dim3(256), 0, st, a);

@@ -96,7 +96,8 @@ def draft_head_mxfp4(x: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor,
     if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != hidden:
         raise ValueError(f"x must be bfloat16 [rows, {hidden}], got {x.dtype} {tuple(x.shape)}")
     device = x.get_device()
-    if device < 0 or codes.get_device() != device or (out is not None and out.get_device() != device):
+    if device < 0 or codes.get_device() != device or exps.get_device() != device or (
+            out is not None and out.get_device() != device):
         raise ValueError(f"MFD kernels take GPU tensors of one device (x on {x.device}, codes on {codes.device})")
     rows, stride = x.shape[0], x.stride()
     if stride[1] != 1 or stride[0] % 8 or x.data_ptr() % 16:

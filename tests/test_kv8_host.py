@@ -73,9 +73,9 @@ def _select(**kw):
     d = dict(w=P, ws=(800, 100), wrows=4, width=100, heads=8, idx=P, lens=P, bs=2, budget=40, sink=4, recent=32, keep=P, new=P,
              wsp=P, nws=1 << 20)
     d.update(kw)
-    return mfd_hip.lib().mfd_evict_select(d["w"], *d["ws"], d["wrows"], d["width"], d["heads"], d["idx"], d["lens"], d["bs"],
-                                          d["budget"], d["sink"], d["recent"], d["keep"], d["new"], d["wsp"], d["nws"], None,
-                                          None)
+    return mfd_hip.lib().mfd_evict_select(d["w"], *d["ws"], d["wrows"], d["width"], d["heads"], d["idx"], d["lens"],
+                                          d["bs"], d["budget"], d["sink"], d["recent"], d["keep"], d["new"], d["wsp"],
+                                          d["nws"], None, None)
 
 
 def _compact(**kw):
@@ -96,13 +96,16 @@ def _head(**kw):
 
 
 INVALID, UNSUPPORTED = -1, -2
-CACHE = [(dict(D=64), UNSUPPORTED, "head dim"), (dict(page=1), UNSUPPORTED, "page_size"), (dict(page=48), UNSUPPORTED, "page_size"),
-         (dict(page=512), UNSUPPORTED, "page_size"), (dict(heads=0), INVALID, "sizes"),
+CACHE = [(dict(D=64), UNSUPPORTED, "head dim"), (dict(page=1), UNSUPPORTED, "page_size"),
+         (dict(page=48), UNSUPPORTED, "page_size"), (dict(page=512), UNSUPPORTED, "page_size"), (dict(heads=0), INVALID, "sizes"),
          (dict(kc=P + 8), UNSUPPORTED, "alignment"), (dict(kcs=(1024, 100)), UNSUPPORTED, "alignment"),
          (dict(kcs=(1 << 26, 128)), UNSUPPORTED, "strides"), (dict(pages=1 << 27), UNSUPPORTED, "2^31")]
 
 
-@pytest.mark.parametrize("call,kw,code,word", [(f, kw, c, w) for f in (_store, _attn, _weigh, _compact) for kw, c, w in CACHE] + [
+EVERY = [(f, kw, c, w) for f in (_store, _attn, _weigh, _compact) for kw, c, w in CACHE]
+
+
+@pytest.mark.parametrize("call,kw,code,word", EVERY + [
     (_store, dict(table=None), INVALID, "table"), (_store, dict(k=None), INVALID, "null"),
     (_store, dict(kn=(1020, 128)), UNSUPPORTED, "16-byte"), (_store, dict(v=P + 2), UNSUPPORTED, "16-byte"),
     (_store, dict(bs=-1), INVALID, "sizes"), (_store, dict(most=-1), INVALID, "sizes"), (_store, dict(cu=None), INVALID, "null"),
@@ -118,10 +121,11 @@ CACHE = [(dict(D=64), UNSUPPORTED, "head dim"), (dict(page=1), UNSUPPORTED, "pag
     (_weigh, dict(lse=None), INVALID, "null"), (_weigh, dict(qs=(1 << 28, 128)), UNSUPPORTED, "2^30"),
     (_select, dict(budget=0), INVALID, "budget"), (_select, dict(sink=20, recent=21), INVALID, "budget"),
     (_select, dict(sink=-1), INVALID, "budget"), (_select, dict(keep=None), INVALID, "null"),
-    (_select, dict(nws=100), INVALID, "workspace"), (_select, dict(heads=0), INVALID, "sizes"),
+    (_select, dict(nws=100, width=20000), INVALID, "workspace"), (_select, dict(heads=0), INVALID, "sizes"),
     (_compact, dict(budget=0), INVALID, "sizes"), (_compact, dict(keep=None), INVALID, "null"),
     (_compact, dict(src=None), INVALID, "table"), (_compact, dict(dst=None), INVALID, "table"),
-    (_head, dict(K=2624), UNSUPPORTED, "128"), (_head, dict(c=P + 8), UNSUPPORTED, "alignment"), (_head, dict(e=P + 2), UNSUPPORTED, "alignment"),
+    (_head, dict(K=2624), UNSUPPORTED, "128"), (_head, dict(c=P + 8), UNSUPPORTED, "alignment"),
+    (_head, dict(e=P + 2), UNSUPPORTED, "alignment"),
     (_head, dict(x=None), INVALID, "null"), (_head, dict(os=999), UNSUPPORTED, "alignment"), (_head, dict(N=0), INVALID, "sizes"),
     (_head, dict(M=-1), INVALID, "sizes"), (_head, dict(rpg=0), INVALID, "sizes"),
 ])
@@ -138,7 +142,8 @@ def test_c_entries_with_nothing_to_do():
     # 4 splits and the block's partial, 2 x 32 x 128 rows: fp16 rows of 128, lse, scale exponent
     assert lib.mfd_kv8_attn_workspace_bytes(2, 8, 16, 32, 8, 1, 4) == 5 * 2 * 32 * 128 * (256 + 8)
     assert lib.mfd_kv8_attn_workspace_bytes(2, 1, 1, 32, 8, 1, 4) == 4 * 2 * 32 * (256 + 8)
-    assert lib.mfd_evict_select_workspace_bytes(3, 101) == 3 * 104 * 4
+    assert lib.mfd_evict_select_workspace_bytes(3, 16384) == 0  # (keys in registers)
+    assert lib.mfd_evict_select_workspace_bytes(3, 16385) == 3 * 16388 * 4
 
 
 # ------------------------------------------------------------------------------------------ refusals, Python entry points
@@ -186,10 +191,12 @@ BAD = [
     ("store", dict(page_table=TABLE.long())), ("store", dict(page_size=24)), ("store", dict(page_size=32)),
     ("store", dict(k_scale=torch.ones(4, 2, dtype=torch.float64))), ("store", dict(v_scale=torch.ones(2, 4).t())),
     ("store", dict(k_cache=torch.zeros(64, 2, 128))), ("store", dict(v_cache=torch.zeros(64, 1, 128).to(F8))),
-    ("attn", dict(q=torch.zeros(7, 4, 128, dtype=torch.bfloat16))), ("attn", dict(q=torch.zeros(8, 3, 128, dtype=torch.bfloat16))),
+    ("attn", dict(q=torch.zeros(7, 4, 128, dtype=torch.bfloat16))),
+    ("attn", dict(q=torch.zeros(8, 3, 128, dtype=torch.bfloat16))),
     ("attn", dict(q=torch.zeros(8, 4, 64, dtype=torch.bfloat16))), ("attn", dict(q=torch.zeros(8, 4, 128))),
     ("attn", dict(k_new=None)), ("attn", dict(v_new=torch.zeros(4, 2, 128, dtype=torch.bfloat16))),
-    ("attn", dict(num_modes=0)), ("attn", dict(ctx_lens=torch.tensor([5]))), ("attn", dict(req_pool_indices=torch.tensor([[0, 1]]))),
+    ("attn", dict(num_modes=0)), ("attn", dict(ctx_lens=torch.tensor([5]))),
+    ("attn", dict(req_pool_indices=torch.tensor([[0, 1]]))),
     ("weights", dict(lse=torch.zeros(4, 8))), ("weights", dict(lse=torch.zeros(8, 4).double())),
     ("weights", dict(weights=torch.zeros(3, 4, 32))), ("weights", dict(weights=torch.zeros(3, 2, 32).bfloat16())),
     ("select", dict(weights=torch.zeros(3, 32, 2).transpose(1, 2))), ("select", dict(keep_out=torch.zeros(2, 8))),
@@ -237,8 +244,8 @@ def test_quantize_takes_the_nearest_code():
 def test_head_refusals():
     codes, exps = torch.zeros(10, 64, dtype=torch.uint8), torch.full((10, 4), 120, dtype=torch.uint8)
     x = torch.zeros(3, 128, dtype=torch.bfloat16)
-    for bad in (dict(codes=codes.int()), dict(exps=exps[:, :3]), dict(codes=codes[:, :32]), dict(codes=codes.t()), dict(x=x.float()),
-                dict(x=x[:, :64])):
+    for bad in (dict(codes=codes.int()), dict(exps=exps[:, :3]), dict(codes=codes[:, :32]), dict(codes=codes.t()),
+                dict(x=x.float()), dict(x=x[:, :64])):
         with pytest.raises(ValueError) as e:
             mxfp4_head.draft_head_mxfp4(**{**dict(x=x, codes=codes, exps=exps), **bad})
         assert "GPU tensors" not in str(e.value)
@@ -266,8 +273,8 @@ def test_reference_path_over_an_8_bit_pool():
     table = torch.tensor([[0, 0, 0], [4, 1, 7], [3, 0, 0]], dtype=torch.int32)
     for x, cache, scale in zip("kv", pool.get_kv_buffer(1), pool.get_kv_scale(1)):
         values, s = cache.float().double().numpy(), scale.double().numpy()
-        kv8.store(torch.randn(53, heads, 128, generator=g).double().numpy(), values, s, table.numpy(), [1, 2], [0, 0], [0, 37, 53],
-                  page)
+        kv8.store(torch.randn(53, heads, 128, generator=g).double().numpy(), values, s, table.numpy(), [1, 2], [0, 0],
+                  [0, 37, 53], page)
         cache.copy_(torch.from_numpy(values).float().to(F8))
         scale.copy_(torch.from_numpy(s).float())
     T = 2 * K * L
