@@ -310,9 +310,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) qf[c] = as_bf16x8(*reinterpret_cast<const u16x8*>(qp + c * 16));
   }
+  const int64_t given_len = a.ctx_lens[b];
   const int32_t* trow = kv8::table_row(a.pages, b);
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
-  const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0);
+  const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, given_len) : 0);
   int lo, hi;
   split_range(a, s, ctx, lo, hi);
   bool with_block = a.kn != nullptr;
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   }
   const int ntiles = (hi - lo + TK - 1) / TK;
   const int last = ntiles - 1;
-  if (tid == 0 && s == 0 && ug == 0 && kvh == 0 && ctx != a.ctx_lens[b]) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  if (tid == 0 && s == 0 && ug == 0 && kvh == 0 && ctx != given_len) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   if (a.S > 1 && ntiles == 0 && !with_block) {  // an empty split
     if (row_ok && half == 0) a.ws_lse[partial_row(a, s, b, kvh, r)] = -INFINITY;
     return;
@@ -707,7 +708,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
   const int32_t* trow = kv8::table_row(a.pages, b);
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
-  const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0);
+  const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, a.ctx_lens[b]) : 0);
   int lo, hi;
   split_range(a, s, ctx, lo, hi);
   const bool with_block = a.kn != nullptr && s == 0;
@@ -985,7 +986,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
 // ------------------------------------------------------------------------------------------------------- merge
 
 // 16 threads per row, 8 d's each; the partials in batches of 8, all loads of a batch in flight together, joined with a
-// running log-sum-exp. An empty partial (lse -inf) wrote no row.
+// running log-sum-exp. An empty partial (lse -inf) wrote no row: what is read of it is not used.
 __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
   constexpr int SB = 8;
   const int64_t per = (int64_t)a.bs * a.Hkv * a.rows;
@@ -998,14 +999,15 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
     float l[SB], ex[SB];
     u32x4 oh[SB];
 #pragma unroll
-    for (int j = 0; j < SB; ++j) l[j] = s0 + j < a.S ? a.ws_lse[(s0 + j) * per + prow] : -INFINITY;
-#pragma unroll
     for (int j = 0; j < SB; ++j) {
+      l[j] = -INFINITY;
       ex[j] = 0.f;
       oh[j] = (u32x4){};
-      if (l[j] != -INFINITY) {
-        ex[j] = a.ws_exp[(s0 + j) * per + prow];
-        oh[j] = *reinterpret_cast<const u32x4*>(a.ws_o + ((s0 + j) * per + prow) * D + d0);
+      if (s0 + j < a.S) {
+        const int64_t at = (s0 + j) * per + prow;
+        l[j] = a.ws_lse[at];
+        ex[j] = a.ws_exp[at];
+        oh[j] = *reinterpret_cast<const u32x4*>(a.ws_o + at * D + d0);
       }
     }
     float mb = l[0];
@@ -1091,7 +1093,7 @@ void kv8_weights_kernel(WArgs a) {
   const int32_t* trow = kv8::table_row(a.pages, b);
   const int64_t wrow = a.pages.req_idx ? a.pages.req_idx[b] : b;
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1;
-  int ctx = trow && a.pages.num_pages > 0 && wrow < a.w_rows ? kv8::bounded_len(a.pages, a.ctx_lens, b) : 0;
+  int ctx = trow && a.pages.num_pages > 0 && wrow < a.w_rows ? kv8::bounded_len(a.pages, a.ctx_lens[b]) : 0;
   if (tid == 0 && range == 0 && kvh == 0 && (ctx > a.width || ctx != a.ctx_lens[b]))
     kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   ctx = __builtin_amdgcn_readfirstlane(min(ctx, a.width));

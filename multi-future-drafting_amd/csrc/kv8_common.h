@@ -31,9 +31,9 @@ __device__ __forceinline__ const int32_t* table_row(const Pages& p, int b) {
   return row >= 0 && row < p.table_rows ? p.table + row * p.table_stride : nullptr;
 }
 // A request's length, as far as its table row reaches.
-__device__ __forceinline__ int bounded_len(const Pages& p, const int64_t* lens, int b) {
+__device__ __forceinline__ int bounded_len(const Pages& p, int64_t len) {
   const int64_t cap = min((int64_t)p.table_width << p.page_shift, (int64_t)0x7fffff00);
-  return (int)max((int64_t)0, min(lens[b], cap));
+  return (int)max((int64_t)0, min(len, cap));
 }
 
 __device__ __forceinline__ void raise(int32_t* err_flag, int bit) {
