@@ -8,13 +8,14 @@
 // The weight (4.25 bits each: 207 MB at 151936 x 2560) streams once per 128 drafted rows, straight to registers: a lane takes
 // 16 bytes, 32 weights of one row under one scale, and the four lane groups of a 16-row tile take 128 k together. Which k a
 // lane holds is free as long as both operands agree, so the four MFMAs of such a step use k = 32 (lane / 16) + 8 j + 0 .. 7.
-//  * Wide form: a workgroup of eight waves takes an even share of the vocabulary, a wave up to VT 16-row tiles of it
-//    against all of the launch's drafted rows (MTL 16-row tiles), which come through LDS in blocks of 2048 / MTL k by
-//    direct loads, double buffered, one barrier per block. Bound by the weight's way from memory with few drafted rows, by
-//    the matrix pipes with 128.
-//  * K-split form, for vocabularies that leave a wave of the wide form without a tile: a workgroup takes VT tiles, each of
-//    its four waves every fourth step of k; the drafted rows come from L2 straight to registers, the partial sums meet in
-//    LDS and are added in wave order.
+//  * Wide form: a workgroup of eight waves takes a share of the vocabulary, a wave up to VT 16-row tiles of it against all
+//    of the launch's drafted rows (MTL 16-row tiles), which come through LDS in blocks of 32 to 64 KB by direct loads, double
+//    buffered, one barrier per block. Bound by the weight's way from memory with few drafted rows (151936 x 2560, 15 rows: 46
+//    us, 4.5 TB/s), by the matrix pipes with 128 (98304 x 2560, 120 rows: 61 us, 1.06 PFLOP/s with the padding to 128; a large
+//    library product reaches 1.24).
+//  * K-split form, for vocabularies that leave a wave of the wide form without a tile: a workgroup takes one tile, each of its
+//    four waves every fourth step of k; the drafted rows come from L2 straight to registers, the partial sums meet in LDS
+//    and are added in wave order. Bound by latency.
 #include <algorithm>
 #include <type_traits>
 
@@ -38,7 +39,9 @@ struct HeadArgs {
   const uint8_t* exps;   // [N][K / 32]
   uint16_t* out;      // [M][out_stride], row 0 = drafted row row0
   int64_t out_stride;
-  int M, N, K, nwg;
+  int M, N, K;
+  // wide form: workgroups; of more than one round also those of the whole ones and their vocabulary rows, and the others' rows
+  int nwg, full_wgs, full_rows, last_rows;
 };
 
 // One direct-to-LDS load: lane l's 16 bytes at g land at LDS byte address lds_byte + 16 l (lds_byte wave-uniform). Inline asm:
@@ -65,9 +68,14 @@ __device__ __forceinline__ const uint16_t* drafted_row(const HeadArgs& a, int r)
 }
 // An operand read takes chunk 4 g4 + j of 16 rows: four rows apart the low bits differ, within four the high ones
 __device__ __forceinline__ int swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
-// First vocabulary row of workgroup g: an even split, in multiples of 8 rows
-__host__ __device__ __forceinline__ int wg_row0(int g, int N, int nwg) {
-  return g >= nwg ? N : (int)(((int64_t)g * N / nwg) & ~(int64_t)7);
+// First vocabulary row of workgroup g. One round: an even split in multiples of 8 rows. More: full ranges for the whole rounds,
+// equal ones that are no larger for the last.
+template <bool ROUNDS>
+__host__ __device__ __forceinline__ int wg_row0(const HeadArgs& a, int g) {
+  if (!ROUNDS) return g >= a.nwg ? a.N : (int)(((int64_t)g * a.N / a.nwg) & ~(int64_t)7);
+  const int64_t row = (int64_t)(g < a.full_wgs ? g : a.full_wgs) * a.full_rows +
+                      (int64_t)(g < a.full_wgs ? 0 : g - a.full_wgs) * a.last_rows;
+  return (int)(row < a.N ? row : a.N);
 }
 
 // Eight codes times the scale as bf16: exact
@@ -95,14 +103,16 @@ __device__ __forceinline__ void store4(uint16_t* orow, int n, int rows, const f3
 // Sizes of the wide form by MTL
 template <int MTL>
 struct Wide {
-  static constexpr int BLOCK = (MTL <= 2 ? 32 : 64) * 1024;  // bytes of a drafted-row block
+  static constexpr int BLOCK = (MTL <= 2 ? 32 : MTL % 3 == 0 ? 48 : 64) * 1024;  // bytes of a drafted-row block
   static constexpr int WPC = MTL <= 2 ? 2 : 1;   // workgroups per CU
-  static constexpr int VT_MAX = MTL == 4 ? 5 : 3;
+  static constexpr int VT_MAX = MTL == 3 || MTL == 4 ? 5 : MTL == 6 ? 4 : 3;
 };
 
-template <int VT, int MTL>
+// ROUNDS: more than one round of workgroups; those of the last one have any number of tiles up to VT, else it is VT or VT - 1
+template <int VT, int MTL, bool ROUNDS>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2 * Wide<MTL>::WPC, 2 * Wide<MTL>::WPC)))
 void mxfp4_wide_kernel(HeadArgs a) {
+  constexpr int FEWEST = ROUNDS ? 0 : VT - 1;
   constexpr int BLOCK = Wide<MTL>::BLOCK, HPS = 2;  // 128-k halves per step
   constexpr int HB = BLOCK / (32 * MTL);  // k per drafted block
   constexpr int CPR = HB / 8;             // 16-byte chunks of a row's block
@@ -112,8 +122,8 @@ void mxfp4_wide_kernel(HeadArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int R0 = wg_row0(blockIdx.x, a.N, a.nwg);
-  const int rows = wg_row0(blockIdx.x + 1, a.N, a.nwg) - R0;
+  const int R0 = wg_row0<ROUNDS>(a, blockIdx.x);
+  const int rows = wg_row0<ROUNDS>(a, blockIdx.x + 1) - R0;
   if (rows <= 0) return;
   const int K = a.K, S = (K + KS * HPS - 1) / (KS * HPS);
   const int l16 = lane & 15, g4 = lane >> 4;
@@ -129,9 +139,8 @@ void mxfp4_wide_kernel(HeadArgs a) {
       dma16(drafted_row(a, r) + min(b * HB + 8 * c, K - 8), lds0 + (uint32_t)(b & 1) * BLOCK + (uint32_t)(i * NW + w) * 1024u);
     }
   };
-  // this wave's tiles: t0 .. t0 + VT - 1 or t0 + VT - 2 (an even split of at most 8 VT tiles, and more than 8 (VT - 1)
-  // rows' worth of them up to the range's rounding), the loop compiled for either: a test per product would cost more
-  // than the product. Rows past the range read as zero by the buffers' bounds.
+  // this wave's tiles: t0 .. t0 + vtv - 1 (an even split of at most 8 VT tiles), the loop compiled for each number of them: a
+  // test per product would cost more than the product. Rows past the range read as zero by the buffers' bounds.
   const int T = (rows + 15) / 16;
   const int t0 = __builtin_amdgcn_readfirstlane(w * T / NW);
   const int vtv = __builtin_amdgcn_readfirstlane((w + 1) * T / NW) - t0;
@@ -232,47 +241,39 @@ void mxfp4_wide_kernel(HeadArgs a) {
       for (int i = 0; i < V; ++i) store4(orow, 16 * (t0 + i) + 4 * g4, rows, acc[i][m]);
     }
   };
-  if (vtv == VT) walk(std::integral_constant<int, VT>{});
-  else walk(std::integral_constant<int, VT - 1>{});
+  auto pick = [&](auto self, auto tiles) __attribute__((always_inline)) {
+    constexpr int V = decltype(tiles)::value;
+    if (V == FEWEST || vtv == V) walk(tiles);
+    else if constexpr (V > FEWEST) self(self, std::integral_constant<int, V - 1>{});
+  };
+  pick(pick, std::integral_constant<int, VT>{});
 }
 
-template <int VT, int MTL>
+template <int MTL>
 __global__ __launch_bounds__(KNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void mxfp4_ksplit_kernel(HeadArgs a) {
-  constexpr int TT = VT * MTL;
-  __shared__ f32x4 part[KNW * TT * 64];
+  static_assert(MTL <= 2, "two steps' operands in registers");
+  __shared__ f32x4 part[KNW * MTL * 64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int R0 = blockIdx.x * (16 * VT);
-  const int rows = min(16 * VT, a.N - R0);
+  const int R0 = blockIdx.x * 16;
+  const int rows = min(16, a.N - R0);
   const int K = a.K, S = K / KS;
   const int l16 = lane & 15, g4 = lane >> 4;
-  const uint8_t* cp[VT];
-  const uint8_t* ep[VT];
-#pragma unroll
-  for (int i = 0; i < VT; ++i) {
-    const int64_t row = R0 + min(16 * i + l16, rows - 1);
-    cp[i] = a.codes + row * (K / 2) + 16 * g4;
-    ep[i] = a.exps + row * (K / 32);
-  }
+  const int64_t row = R0 + min(l16, rows - 1);
+  const uint8_t* cp = a.codes + row * (K / 2) + 16 * g4;
+  const uint8_t* ep = a.exps + row * (K / 32);
   const uint16_t* xp[MTL];
 #pragma unroll
   for (int m = 0; m < MTL; ++m) xp[m] = drafted_row(a, 16 * m + l16) + 32 * g4;
-  f32x4 acc[VT][MTL];
+  f32x4 acc[MTL];
 #pragma unroll
-  for (int i = 0; i < VT; ++i)
-#pragma unroll
-    for (int m = 0; m < MTL; ++m) acc[i][m] = (f32x4){};
-  // few drafted rows: two steps' operands in registers, else one
-  constexpr int NB = MTL <= 2 ? 2 : 1;
-  u32x4 wf[NB][VT];
-  uint32_t ef[NB][VT];
-  bf16x8 xf[NB][MTL][4];
+  for (int m = 0; m < MTL; ++m) acc[m] = (f32x4){};
+  u32x4 wf[2];
+  uint32_t ef[2];
+  bf16x8 xf[2][MTL][4];
   auto load = [&](int s, int v) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      wf[s][i] = *reinterpret_cast<const u32x4*>(cp[i] + 64 * v);
-      ef[s][i] = *reinterpret_cast<const uint32_t*>(ep[i] + 4 * v);
-    }
+    wf[s] = *reinterpret_cast<const u32x4*>(cp + 64 * v);
+    ef[s] = *reinterpret_cast<const uint32_t*>(ep + 4 * v);
 #pragma unroll
     for (int m = 0; m < MTL; ++m)
 #pragma unroll
@@ -280,71 +281,70 @@ __global__ __launch_bounds__(KNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
     __builtin_amdgcn_sched_barrier(0);
   };
   auto products = [&](int s) __attribute__((always_inline)) {
+    const float sc = scale_of(ef[s], g4);
 #pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      const float sc = scale_of(ef[s][i], g4);
+    for (int j = 0; j < 4; ++j) {
+      const bf16x8 f = widen(wf[s][j], sc);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bf16x8 f = widen(wf[s][i][j], sc);
-#pragma unroll
-        for (int m = 0; m < MTL; ++m) acc[i][m] = mfma16(f, xf[s][m][j], acc[i][m]);
-      }
+      for (int m = 0; m < MTL; ++m) acc[m] = mfma16(f, xf[s][m][j], acc[m]);
     }
   };
-  if constexpr (NB == 2) {
-    if (w < S) load(0, w);
-    for (int v = w; v < S; v += 2 * KNW) {
-      if (v + KNW < S) load(1, v + KNW);
-      products(0);
-      if (v + KNW < S) {
-        if (v + 2 * KNW < S) load(0, v + 2 * KNW);
-        products(1);
-      }
-    }
-  } else {
-    for (int v = w; v < S; v += KNW) {
-      load(0, v);
-      products(0);
+  if (w < S) load(0, w);
+  for (int v = w; v < S; v += 2 * KNW) {
+    if (v + KNW < S) load(1, v + KNW);
+    products(0);
+    if (v + KNW < S) {
+      if (v + 2 * KNW < S) load(0, v + 2 * KNW);
+      products(1);
     }
   }
 #pragma unroll
-  for (int i = 0; i < VT; ++i)
-#pragma unroll
-    for (int m = 0; m < MTL; ++m) part[(w * TT + i * MTL + m) * 64 + lane] = acc[i][m];
+  for (int m = 0; m < MTL; ++m) part[(w * MTL + m) * 64 + lane] = acc[m];
   __syncthreads();
-  for (int t = w; t < TT; t += KNW) {
-    const int i = t / MTL, m = 16 * (t % MTL) + l16;
-    f32x4 c = part[t * 64 + lane];
+  if (w < MTL) {
+    f32x4 c = part[w * 64 + lane];
 #pragma unroll
     for (int x = 1; x < KNW; ++x) {
-      const f32x4 d = part[(x * TT + t) * 64 + lane];
+      const f32x4 d = part[(x * MTL + w) * 64 + lane];
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[e] += d[e];
     }
-    if (m < a.M) store4(a.out + (int64_t)m * a.out_stride + R0, 16 * i + 4 * g4, rows, c);
+    const int mm = 16 * w + l16;
+    if (mm < a.M) store4(a.out + (int64_t)mm * a.out_stride + R0, 4 * g4, rows, c);
   }
 }
 
-template <int VT, int MTL>
+template <int VT, int MTL, bool ROUNDS = false>
 int launch_wide(const HeadArgs& a, hipStream_t st) {
   if constexpr (VT <= Wide<MTL>::VT_MAX) {
     constexpr int lds = 2 * Wide<MTL>::BLOCK;
-    const int rc = mfd_set_max_lds(reinterpret_cast<const void*>(&mxfp4_wide_kernel<VT, MTL>), lds);
+    const int rc = mfd_set_max_lds(reinterpret_cast<const void*>(&mxfp4_wide_kernel<VT, MTL, ROUNDS>), lds);
     if (rc != MFD_OK) return rc;
-    hipLaunchKernelGGL((mxfp4_wide_kernel<VT, MTL>), dim3((unsigned)a.nwg), dim3(NW * 64), lds, st, a);
+    hipLaunchKernelGGL((mxfp4_wide_kernel<VT, MTL, ROUNDS>), dim3((unsigned)a.nwg), dim3(NW * 64), lds, st, a);
   }
   return MFD_OK;
 }
 template <int MTL>
 int launch_rows(HeadArgs a, int cus, hipStream_t st) {
-  if ((int64_t)a.N <= (int64_t)NW * 16 * cus / 2) {
-    hipLaunchKernelGGL((mxfp4_ksplit_kernel<1, MTL>), dim3((unsigned)((a.N + 15) / 16)), dim3(KNW * 64), 0, st, a);
-    return MFD_OK;
-  }
-  // whole rounds of the workgroups that run together, as few as hold the vocabulary
-  const int slots = Wide<MTL>::WPC * cus;
+  // k-split: up to a tile per CU and 32 drafted rows (hidden 2560: 4000 x 32 rows 9.1 us against the wide form's 10.9, 4000 x 4
+  // 5.8 against 8.9; beyond either, 8000 x 16 rows 10.3 against 9.5, 4000 x 96 19.0 against 17.2, 16000 x 96 60.6 against 20.8)
+  if constexpr (MTL <= 2)
+    if (a.N <= 16 * cus) {
+      hipLaunchKernelGGL(mxfp4_ksplit_kernel<MTL>, dim3((unsigned)((a.N + 15) / 16)), dim3(KNW * 64), 0, st, a);
+      return MFD_OK;
+    }
+  const int slots = Wide<MTL>::WPC * cus;  // workgroups that run together
+  a.full_rows = NW * Wide<MTL>::VT_MAX * 16;
   a.nwg = slots;
-  while (a.N / a.nwg + 8 > NW * Wide<MTL>::VT_MAX * 16) a.nwg += slots;
+  if (a.N / slots + 8 > a.full_rows) {
+    // whole rounds of full workgroups, then one that shares the rest: a wave's tiles come whole, and an even split over the
+    // rounds leaves more waves with a part of one (98304 rows, 120 drafted ones: 61 us in one round, 73 in two even ones)
+    a.full_wgs = (int)(a.N / ((int64_t)slots * a.full_rows)) * slots;
+    const int64_t rest = a.N - (int64_t)a.full_wgs * a.full_rows;
+    a.last_rows = (int)((rest + 8 * slots - 1) / (8 * slots)) * 8;
+    a.nwg += a.full_wgs;
+    return launch_wide<Wide<MTL>::VT_MAX, MTL, true>(a, st);
+  }
   const int vt = (a.N / a.nwg + 8 + 16 * NW - 1) / (16 * NW);  // tiles of a wave
   switch (vt) {
     case 1: return launch_wide<1, MTL>(a, st);
@@ -373,9 +373,13 @@ int head_gemm(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t
   const hipStream_t st = static_cast<hipStream_t>(stream);
   for (int m0 = 0; m0 < M; m0 += MT) {
     const HeadArgs a{x, row_stride, group_stride, rows_per_group, m0, codes, exps, out + (int64_t)m0 * out_stride, out_stride,
-                     std::min(MT, M - m0), N, K, 0};
-    const int rc = a.M <= 16 ? launch_rows<1>(a, cus, st) : a.M <= 32 ? launch_rows<2>(a, cus, st)
-                   : a.M <= 64 ? launch_rows<4>(a, cus, st) : launch_rows<8>(a, cus, st);
+                     std::min(MT, M - m0), N, K, 0, 0, 0, 0};
+    const int rc = a.M <= 16   ? launch_rows<1>(a, cus, st)
+                   : a.M <= 32 ? launch_rows<2>(a, cus, st)
+                   : a.M <= 48 ? launch_rows<3>(a, cus, st)
+                   : a.M <= 64 ? launch_rows<4>(a, cus, st)
+                   : a.M <= 96 ? launch_rows<6>(a, cus, st)
+                               : launch_rows<8>(a, cus, st);
     if (rc != MFD_OK) return rc;
     MFD_CHECK_LAUNCH();
   }

@@ -32,6 +32,8 @@ def _check(got, x, codes, exps):
     (1, 1, 128), (3, 17, 128), (16, 250, 256), (17, 4001, 384), (33, 100, 2560), (128, 515, 1024), (200, 77, 640),  # k-split
     (1, 16500, 128), (15, 20001, 384), (32, 33000, 256), (50, 50003, 512), (65, 70001, 384), (128, 17000, 640),     # wide
     (130, 99999, 256), (7, 163841, 128), (120, 170003, 128),                                                        # rounds
+    (40, 18001, 256), (48, 100003, 128), (90, 20003, 384), (70, 140003, 128),                             # 48 and 96 rows
+    (128, 98301, 128), (20, 196605, 128), (64, 163839, 128),               # a round that is full but for a few rows
 ])
 def test_draft_head(rows, vocab, hidden):
     import mxfp4_head
