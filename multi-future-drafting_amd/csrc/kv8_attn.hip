@@ -1384,7 +1384,11 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t programs = (int64_t)bs * Hkv * a.S;
   const int units = (a.rows + UROWS - 1) / UROWS;
-  const int NW = units % 8 == 0 ? 8 : 4;
+  // Eight waves share a tile's widening where they all have a unit, and in a batch that half fills the chip even where some
+  // idle (16 requests of 4000 tokens: 12 units 134 us against 169 with four, 20 units 245 against 268; 4 requests, 12 units 65
+  // against 60). kv8_cache.py counts by the same rule.
+  const int64_t by8 = (int64_t)bs * Hkv * ((units + 7) / 8);
+  const int NW = units % 8 == 0 || (units > 4 && 2 * by8 >= mfd_num_cus()) ? 8 : 4;
   a.ngroups = (units + NW - 1) / NW;
   const int64_t grid = units == 1 ? programs : (programs + 7) / 8 * 8 * a.ngroups;
   if (grid > 0x7fffffff || (prows + 15) / 16 > 0x7fffffff)

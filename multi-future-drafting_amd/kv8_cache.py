@@ -164,8 +164,9 @@ def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int,
     76 in two parts). At least 128 keys per split there and 256 else, at most 32 and 64 splits (32768 tokens, one request:
     28 us in 32 parts, 34 in 64)."""
     units = -(-rows // UNIT)
-    waves = 8 if units % 8 == 0 else 4
-    slots = mfd_hip.cu_count(device) * (1 if waves == 8 else 2)
+    cus = mfd_hip.cu_count(device)
+    waves = 8 if units % 8 == 0 or units > 4 and 2 * bs * heads * -(-units // 8) >= cus else 4  # (as mfd_kv8_attn does)
+    slots = cus * (1 if waves == 8 else 2)
     programs = max(1, bs * heads * -(-units // waves))
     if units == 1:
         splits = 1 if programs >= slots else min((1 if bs == 1 else 3) * slots // programs, -(-max_ctx // 128), 32)
