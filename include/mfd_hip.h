@@ -437,8 +437,8 @@ int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* 
 /* Attention weight that each cached token received, added to its running sum:
  *   weights[row][h][t] = decay * weights[row][h][t] + sum over KV head h's query rows of exp(scale q.k_t - lse)
  * for t < ctx_lens[b]; other entries keep their values. lse [bs K L][H] as mfd_kv8_attn writes it (rows of -inf add
- * nothing). weights: [w_rows][Hkv][width] f32 with row and head strides, row = req_idx ? req_idx[b] : b; decay in [0, 1]
- * (0: the old sums are not read). Every sum is formed in one order: results repeat bit for bit. */
+ * nothing). weights: [w_rows][Hkv][width] f32 with row and head strides, row = req_idx ? req_idx[b] : b (of one request
+ * of the call each); decay in [0, 1] (0: the old sums are not read). Every sum is formed in one order: results repeat bit for bit. */
 int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, const float* lse, const uint8_t* k_cache,
                     int64_t kc_ss, int64_t kc_sh, const float* k_scale, int num_pages, const int32_t* page_table,
                     int64_t table_stride, int table_rows, int table_width, int page_size, const int64_t* req_idx,
@@ -450,7 +450,7 @@ int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, const float* 
  * once to fp32. Of a request longer than `budget`, the first `sink` and the last `recent` tokens stay, and of the rest
  * those with the largest scores (ties: the lowest position; NaN below everything); a shorter one keeps all.
  *   keep      [bs][budget] int32: the kept positions, ascending, -1 behind them;  new_lens [bs] int64: how many
- *   workspace mfd_evict_select_workspace_bytes(bs, width) bytes, 16-byte aligned
+ *   workspace mfd_evict_select_workspace_bytes(bs, width) bytes, 16-byte aligned (none up to a width of 16384)
  *   1 <= budget, sink + recent <= budget
  */
 int64_t mfd_evict_select_workspace_bytes(int bs, int width);

@@ -136,7 +136,7 @@ def kv8_store(*, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     A page's scale is the smallest power of two s with amax / s <= 448. A page whose first token is stored begins anew; in a
     page begun earlier the scale only grows, and the entries before the new ones are rounded again when it does. Entries
     behind the new ones keep their bits. Infinities become +-448 s, NaN stays NaN. Two requests must not store into one
-    page in the same call."""
+    page in the same call (nor two calls that may overlap)."""
     cache, heads = _cache_args(k_cache, v_cache, k_scale, v_scale, page_size)
     n, bs = k.shape[0], cu_tokens.numel() - 1
     ks, vs = _rows(k, n, heads, "k"), _rows(v, n, heads, "v")
@@ -294,7 +294,7 @@ def attention_weights_kv8(*, q: torch.Tensor, lse: torch.Tensor, k_cache: torch.
     with row = req_pool_indices[b]. q and ``lse`` [T, H] as paged_mode_block_attention_kv8 took and returned them (rows of
     lse -inf add nothing). weights: float32 [rows, KV heads, tokens], zero before a request's first call. With page tables
     that all layers share, one ``weights`` collects every layer's call: decay in the first, 1 in the others. decay 0 does not
-    read the old sums. Results repeat bit for bit."""
+    read the old sums. A row of ``weights`` belongs to one request of the call. Results repeat bit for bit."""
     cache, heads = _cache_args(k_cache, k_cache, k_scale, k_scale, page_size)
     bs, H, qs = _query(q, heads, num_modes, block_size)
     if lse.dtype is not torch.float32 or tuple(lse.shape) != (q.shape[0], H) or not lse.is_contiguous():
@@ -315,7 +315,7 @@ def evict_select(*, weights: torch.Tensor, req_pool_indices: torch.Tensor, ctx_l
     ``recent``, and of the rest those whose weights, summed over the KV heads (in float64, rounded once to float32), are
     largest (ties: the lowest position; NaN below everything). Returns (keep [bs, budget] int32: positions ascending, -1
     behind them; new_lens [bs] int64). bs is ctx_lens' length."""
-    bs, heads = ctx_lens.shape[0], weights.shape[1]
+    bs, heads = ctx_lens.numel(), weights.shape[1] if weights.dim() == 3 else -1
     sums = _weights_args(weights, heads)
     rows, lens = _index(req_pool_indices, bs, "req_pool_indices"), _index(ctx_lens, bs, "ctx_lens")
     keep = weights.new_empty((bs, budget), dtype=torch.int32) if keep_out is None else keep_out

@@ -199,7 +199,8 @@ BAD = [
     ("attn", dict(req_pool_indices=torch.tensor([[0, 1]]))),
     ("weights", dict(lse=torch.zeros(4, 8))), ("weights", dict(lse=torch.zeros(8, 4).double())),
     ("weights", dict(weights=torch.zeros(3, 4, 32))), ("weights", dict(weights=torch.zeros(3, 2, 32).bfloat16())),
-    ("select", dict(weights=torch.zeros(3, 32, 2).transpose(1, 2))), ("select", dict(keep_out=torch.zeros(2, 8))),
+    ("select", dict(weights=torch.zeros(3, 32, 2).transpose(1, 2))), ("select", dict(weights=torch.zeros(64))),
+    ("select", dict(ctx_lens=torch.tensor(5))), ("select", dict(keep_out=torch.zeros(2, 8))),
     ("compact", dict(keep=torch.zeros(2, 8))), ("compact", dict(dst_table=TABLE.t())),
     ("compact", dict(weights=torch.zeros(3, 3, 32))),
 ]
