@@ -158,20 +158,35 @@ def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int,
     """(num_ctx_splits, split_keys) for num_ctx_splits < 0, from what the kernels' workgroup slots hold (two workgroups per CU,
     one of eight waves) and the programs (request, KV head, group of units) that there are without a split.
 
-    A single request's splits fill one round of slots, less the block partial's; a batch's lengths differ and half a round
-    more evens them out, three rounds where a program is one unit (plain decoding: 16 requests of 4748 .. 32132 tokens, 40
-    heads: 173 us with one round, 146 with three, 152 with eight; 64 even ones, a workgroup per slot already: 66 us whole,
-    76 in two parts). At least 128 keys per split there and 256 else, at most 32 and 64 splits (32768 tokens, one request:
-    28 us in 32 parts, 34 in 64)."""
+    A single request's splits fill one round of slots, less the block partial's, and so do a small batch's (up to a third of
+    the slots whole: 2 requests of up to 8192 tokens, 32 heads, 8 x 16 queries, 36 to 45 us in 7 parts, 47 to 60 in 12); a
+    larger one's lengths differ and half a round more evens them out. At least 256 keys per split, at most 64 splits.
+
+    Where a program is one unit (plain decoding), a batch gets a workgroup per CU, or parts of 2048 tokens where those are
+    more, up to three rounds: 4 requests of up to 8192 tokens, 32 heads, 21 us in 8 parts, 28 in 32; 16 requests of 4748 ..
+    32132 tokens, 40 heads, 173 us with one round, 146 with three, 152 with eight; 64 even ones, a workgroup per slot already:
+    66 us whole, 76 in two parts. At least 128 keys per split, at most 32 splits (32768 tokens, one request: 28 us in 32
+    parts, 34 in 64)."""
     units = -(-rows // UNIT)
     cus = mfd_hip.cu_count(device)
     waves = 8 if units % 8 == 0 or units > 4 and 2 * bs * heads * -(-units // 8) >= cus else 4  # (as mfd_kv8_attn does)
     slots = cus * (1 if waves == 8 else 2)
     programs = max(1, bs * heads * -(-units // waves))
     if units == 1:
-        splits = 1 if programs >= slots else min((1 if bs == 1 else 3) * slots // programs, -(-max_ctx // 128), 32)
+        if programs >= slots:
+            splits = 1
+        elif bs == 1:
+            splits = slots // programs
+        else:
+            splits = min(3 * slots // programs, max(cus // programs, max_ctx // 2048))
+        splits = min(splits, -(-max_ctx // 128), 32)
     else:
-        splits = slots // programs - (1 if with_block else 0) if bs == 1 else 3 * slots // (2 * programs)
+        if bs == 1:
+            splits = slots // programs - (1 if with_block else 0)
+        elif 3 * programs <= slots:
+            splits = -(-slots // programs) - 1 if with_block else slots // programs
+        else:
+            splits = 3 * slots // (2 * programs)
         splits = min(splits, -(-max_ctx // 256), 64)
     return _splits_of(splits, max_ctx) if splits > 1 else (1, 0)
 
