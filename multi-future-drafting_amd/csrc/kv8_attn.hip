@@ -1088,9 +1088,11 @@ __global__ __launch_bounds__(RS * 256) __attribute__((amdgpu_waves_per_eu(2, 2))
 void kv8_weights_kernel(WArgs a) {
   static_assert(RS <= 2 && QS <= 2, "one or two");
   constexpr int NWV = 4 * RS;
-  // widened keys first (32 of each wave at a time), then two stages of query rows
+  // widened keys (32 of each wave at a time) and two stages of query rows, each with a place of its own: the first stage is
+  // on its way while the keys are looked up
   constexpr int KLDS = NWV * SK * KROW, STAGE = RS * QS * UROWS * D * 2;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[KLDS > 2 * STAGE ? KLDS : 2 * STAGE];
+  static_assert(KLDS % 1024 == 0, "the stages are aligned");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[KLDS + 2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
@@ -1121,7 +1123,7 @@ void kv8_weights_kernel(WArgs a) {
   int rr = qr, rq = qr % a.KL;  // the next load's row, and its query
   const uint32_t q_first = ((lane & 15) ^ (qr & 15)) * 8;
   uint32_t qo = q_first + (uint32_t)(qr / a.KL) * q_sh + (uint32_t)rq * q_st;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + KLDS);
   auto load_q = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2 * QS; ++i) {
@@ -1161,7 +1163,8 @@ void kv8_weights_kernel(WArgs a) {
     }
   };
 
-  // keys of this wave: 64 rows, a lane 16 codes (lane % 8) of rows lane / 8 + 8 i, 32 rows through LDS at a time
+  load_q(0);
+  load_lse();
   const int base = l32 * 128 + ((((half ^ l32) & 1) | (l32 & 14)) << 3);
   bf16x8 kf[2][D / 16];
   const uint8_t* const kc_h = a.kc + (int64_t)kvh * a.kc_sh + (lane & 7) * 16;
@@ -1196,12 +1199,9 @@ void kv8_weights_kernel(WArgs a) {
     }
   }
   if (bad) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
-  lds_barrier();
   float acc[32];
 #pragma unroll
   for (int x = 0; x < 32; ++x) acc[x] = 0.f;
-  load_q(0);
-  load_lse();
   float l_st[QS];  // of the stage that is read, base 2
   // Stage st has landed in every wave and the one before is read: its buffer takes the one behind
   auto next_stage = [&](int st) __attribute__((always_inline)) {
@@ -1230,7 +1230,7 @@ void kv8_weights_kernel(WArgs a) {
       for (int x = 0; x < 32; ++x) cur[x >> 4][x & 15] = l == INFINITY ? 0.f : cur[x >> 4][x & 15];
     }
     const uint16_t* qb =
-        reinterpret_cast<const uint16_t*>(lds + (n / QS & 1) * STAGE) + (wr * QS + n % QS) * (UROWS * D);
+        reinterpret_cast<const uint16_t*>(lds + KLDS + (n / QS & 1) * STAGE) + (wr * QS + n % QS) * (UROWS * D);
     bf16x8 qf[D / 16];
     if (more) {
 #pragma unroll
@@ -1299,7 +1299,6 @@ void kv8_weights_kernel(WArgs a) {
   const int x = l32 & 15, in_tile = (l32 >> 4) * 32 + 8 * (x >> 2) + 4 * half + (x & 3);
   float sum = acc[0];
   if constexpr (RS == 2) {
-    // (behind the loop's last barrier: the query rows are read)
     float* const part = reinterpret_cast<float*>(lds);
     if (wr == 1) part[wk * TK + in_tile] = sum;
     lds_barrier();
