@@ -1054,18 +1054,18 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
 
 // ----------------------------------------------------------------------------------------------------- weights
 
-// Attention weight per cached token. A workgroup takes 256 keys of one (request, KV head), 64 a wave: the wave's keys are
+// Attention weight per cached token. A workgroup takes 256 (or 128) keys of one (request, KV head), 64 a wave: the wave's keys are
 // widened once through LDS into MFMA operands (64 registers) and stay there, while the KV head's query rows stream by in
 // units of 32 through a double buffer in LDS that the waves share. A lane then holds, for its query row, the 32 keys of its
 // half; p = exp2(s scale - lse) is added up per key over the units in registers, and once at the end over the 32 lanes.
 // Every sum has one owner and one order: no atomics. Bound by issue, mostly the exponentials' (one per product of 256 flops):
-// 16 requests of 1187 .. 8033 tokens, 40 heads, 8 x 16 queries: 124 us, 0.76 PFLOP/s; one request of 4096, 32 heads: 12.9 us.
+// 16 requests of 1187 .. 8033 tokens, 40 heads, 8 x 16 queries: 124 us, 0.76 PFLOP/s; one request of 4096, 32 heads: 10 us of kernel.
 //
-// RS: waves per 64 keys, each of which takes every RS-th pair of units; two where one would leave each CU a workgroup or none
-// (one request of 4096 tokens 15.4 us against 16.5, 16 of them 183 against 131), their sums joined in LDS in wave order. QS:
-// units of a wave per stage; one where a KV head has one unit (3 requests of up to 12151 tokens, 4 rows: 14.3 us against 16.7).
-constexpr int WKEYS = 4 * TK;
-
+// KW: the workgroup's 64-key parts. RS: waves per part, each of which takes every RS-th share of the units, their sums joined in
+// LDS in wave order. One wave per part where that leaves each CU more than a workgroup; else two, and four on half as many keys
+// where that is still one round (one request of 4096 tokens 12.1 us against 14.9 with two, of 5000 20.3 against 15.1; 16 requests
+// 183 us with two against 131 with one). QS: units of a wave per stage; one where a KV head has one unit (3 requests of up
+// to 12151 tokens, 4 rows: 14.3 us against 16.7).
 struct WArgs {
   const uint16_t* q;
   int64_t q_st, q_sh;
@@ -1083,11 +1083,11 @@ struct WArgs {
   int32_t* err_flag;
 };
 
-template <int RS, int QS>
-__global__ __launch_bounds__(RS * 256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int KW, int RS, int QS>
+__global__ __launch_bounds__(KW * RS * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void kv8_weights_kernel(WArgs a) {
-  static_assert(RS <= 2 && QS <= 2, "one or two");
-  constexpr int NWV = 4 * RS;
+  static_assert((KW == 2 || KW == 4) && QS <= 2, "whole loads per stage");
+  constexpr int NWV = KW * RS, WKEYS = KW * TK;
   // widened keys (32 of each wave at a time) and two stages of query rows, each with a place of its own: the first stage is
   // on its way while the keys are looked up
   constexpr int KLDS = NWV * SK * KROW, STAGE = RS * QS * UROWS * D * 2;
@@ -1096,7 +1096,7 @@ void kv8_weights_kernel(WArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
-  const int wk = w & 3, wr = w >> 2;  // the wave's 64 keys, and its share of the units
+  const int wk = w % KW, wr = w / KW;  // the wave's 64 keys, and its share of the units
   // KV heads fastest, key ranges slowest: with eight heads each XCD (workgroup id modulo 8) has one, whose query rows stay in
   // its L2, and ranges that only the longest requests reach are spread over all of them
   const int kvh = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv % a.bs, range = blockIdx.x / a.Hkv / a.bs;
@@ -1111,10 +1111,10 @@ void kv8_weights_kernel(WArgs a) {
   if (lo >= ctx) return;
 
   // Query rows come by direct-to-LDS loads, a stage of RS QS units at a time, double buffered. A load moves four whole rows:
-  // load i of wave w takes rows 16 RS i + 4 w + lane / 16 of the stage, and chunk c of row r lands at c ^ (r % 16) of the row
+  // load i of wave w takes rows 4 NWV i + 4 w + lane / 16 of the stage, and chunk c of row r lands at c ^ (r % 16) of the row
   // (the lane at position p asks for chunk p ^ (r % 16)). Rows past the last repeat the first.
   const int stages = (a.rows + RS * QS * UROWS - 1) / (RS * QS * UROWS);
-  constexpr int QSTEP = 16 * RS;  // rows from one of a wave's loads to its next
+  constexpr int QSTEP = 4 * NWV;  // rows from one of a wave's loads to its next
   const int qr = 4 * w + (lane >> 4);
   const int dg = QSTEP / a.KL, dq = QSTEP % a.KL;
   const uint32_t q_st = (uint32_t)a.q_st, q_sh = (uint32_t)a.q_sh;  // (a request's queries span less than 2^30 elements)
@@ -1126,7 +1126,7 @@ void kv8_weights_kernel(WArgs a) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + KLDS);
   auto load_q = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2 * QS; ++i) {
+    for (int i = 0; i < RS * QS * UROWS / QSTEP; ++i) {
       dma16(q_b + (rr < a.rows ? qo : q_first), lds0 + (uint32_t)((st & 1) * STAGE + (QSTEP * i + 4 * w) * (D * 2)));
       rr += QSTEP;
       rq += dq;
@@ -1298,12 +1298,13 @@ void kv8_weights_kernel(WArgs a) {
   join(std::integral_constant<int, 1>{});
   const int x = l32 & 15, in_tile = (l32 >> 4) * 32 + 8 * (x >> 2) + 4 * half + (x & 3);
   float sum = acc[0];
-  if constexpr (RS == 2) {
-    float* const part = reinterpret_cast<float*>(lds);
-    if (wr == 1) part[wk * TK + in_tile] = sum;
+  if constexpr (RS > 1) {
+    float* const part = reinterpret_cast<float*>(lds) + wk * TK + in_tile;
+    if (wr > 0) part[(wr - 1) * WKEYS] = sum;
     lds_barrier();
-    if (wr == 1) return;
-    sum += part[wk * TK + in_tile];
+    if (wr > 0) return;
+#pragma unroll
+    for (int y = 0; y < RS - 1; ++y) sum += part[y * WKEYS];
   }
   const int key = lo + wk * TK + in_tile;
   if (key < ctx) {
@@ -1454,12 +1455,19 @@ extern "C" int mfd_kv8_weights(const uint16_t* q, int64_t q_st, int64_t q_sh, co
   a.decay = decay;
   a.err_flag = err_flag;
   const int64_t keys = std::min<int64_t>(width, (int64_t)table_width * page_size);
-  const int64_t grid = (keys + WKEYS - 1) / WKEYS * Hkv * bs;
-  if (grid > 0x7fffffff) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
+  auto grid_of = [&](int range) { return (keys + range - 1) / range * Hkv * bs; };
+  const int64_t grid = grid_of(4 * TK);
+  if (grid > 0x3fffffff) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a.rows <= UROWS) hipLaunchKernelGGL((kv8_weights_kernel<1, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
-  else if (grid > mfd_num_cus()) hipLaunchKernelGGL((kv8_weights_kernel<1, 2>), dim3((unsigned)grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((kv8_weights_kernel<2, 2>), dim3((unsigned)grid), dim3(512), 0, st, a);
+  const int cus = mfd_num_cus();
+  if (a.rows <= UROWS)
+    hipLaunchKernelGGL((kv8_weights_kernel<4, 1, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else if (grid > cus)
+    hipLaunchKernelGGL((kv8_weights_kernel<4, 1, 2>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else if (grid_of(2 * TK) > cus)
+    hipLaunchKernelGGL((kv8_weights_kernel<4, 2, 2>), dim3((unsigned)grid), dim3(512), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv8_weights_kernel<2, 4, 1>), dim3((unsigned)grid_of(2 * TK)), dim3(512), 0, st, a);
   MFD_CHECK_LAUNCH();
   return MFD_OK;
 }
