@@ -100,6 +100,10 @@ ATTN = [
     ([130], 2, 40, 4, 2, 256, True, False, 1),                        # blocks of 40: modes cross units and tiles
     ([90], 1, 150, 2, 1, 32, True, True, 2),                          # one long causal block over three tiles
     ([200, 1], 1, 5, 26, 2, 64, False, False, -1),                    # 65 rows without block keys
+    ([64 + 7 * i for i in range(16)], 2, 16, 40, 8, 64, True, False, -1),   # a batch with idle waves: five units
+    ([3 + 11 * i for i in range(16)], 1, 40, 40, 8, 32, True, True, 2),     # .. seven, small pages, splits
+    ([1 + 17 * i % 97 for i in range(40)], 1, 1, 32, 8, 16, True, False, 1),  # plain decoding, more workgroups than CUs
+    ([9 + 31 * i % 200 for i in range(40)], 1, 3, 32, 8, 64, False, False, -1),
 ]
 
 
@@ -132,6 +136,9 @@ WEIGHTS = [
     ([256, 257, 255], 1, 5, 26, 2, 64, 400, 0.9),
     ([700, 64], 8, 16, 32, 8, 64, 700, 0.0),
     ([77, 500], 3, 16, 40, 8, 32, 501, 1.0),
+    ([5003], 2, 16, 32, 8, 64, 5003, 0.5), ([4999], 1, 9, 32, 8, 16, 5100, 1.0),  # one request, more than one round of the smallest
+    ([8500, 1, 130], 4, 16, 40, 8, 64, 8500, 1.0), ([130, 9001], 1, 33, 8, 8, 128, 9100, 0.7),  # more workgroups than CUs
+    ([300], 1, 33, 2, 2, 64, 300, 0.3), ([100], 1, 161, 1, 1, 32, 200, 1.0),                   # two and six units
 ]
 
 
