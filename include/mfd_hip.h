@@ -419,7 +419,8 @@ int mfd_kv8_store(const uint16_t* k, const uint16_t* v, int64_t kn_st, int64_t k
  *                  block_size 1, after the token was stored). A row without any key gets output 0 and lse -inf
  *   num_ctx_splits, split_keys  1: one pass. > 1: split i takes the keys i * split_keys .. of every request (the last one
  *                  all that are left), so a request gets as many workgroups as its length asks for; split_keys a multiple
- *                  of 64
+ *                  of 64, or 0 (up to 64 requests): chosen on the device from the lengths, the shortest with which the splits
+ *                  of all requests fill the chip's workgroups in whole rounds and no request has more than num_ctx_splits
  *   lse            [bs K L][H] f32, natural log-sum-exp of a row's scaled scores, block keys included; or NULL
  *   workspace      mfd_kv8_attn_workspace_bytes(...) bytes, 16-byte aligned (NULL allowed when 0); with_block: k_new given
  */

@@ -72,6 +72,8 @@ struct Args {
   float* ws_exp;   // [S][bs][Hkv][rows] the row's power-of-two scale exponent
   int bs, K, L, H, Hkv, G, KL, rows;  // rows = G K L: query rows of a KV head
   int SC, S, split_keys;              // context splits; partials (tile kernel: one more for the block keys)
+  int pairs, min_tiles;               // split_keys 0: (request, partial) pairs of the grid, and a split's fewest 64-key tiles
+  int32_t* ws_n;                      // [bs] a request's context splits
   int causal, ngroups;
   float scale_log2;
   int32_t* err_flag;
@@ -214,23 +216,60 @@ __device__ __forceinline__ int request_of_rank(const int64_t* ctx_lens, int bs, 
   return rho;
 }
 
-// Program p of bs Hkv S: (split, KV head, rank of the request). KV heads fastest: with eight of them each XCD (workgroup id
-// modulo 8) has one, and with fewer the turn of the splits with the rank keeps a split from meeting the same XCDs in every
-// request (short requests have only the first splits: a fixed pairing of splits and XCDs measured 462 us against 276).
-__device__ __forceinline__ void program_of(const Args& a, int p, int& s, int& kvh, int& rho) {
+// Program p: (KV head, request b, split s of `parts` of `keys` keys); false where there is none. KV heads fastest: with eight of
+// them each XCD (workgroup id modulo 8) has one.
+//
+// split_keys given: every request SC splits; requests by rank, and with fewer heads the turn of the splits with the rank keeps
+// a split from meeting the same XCDs in every request (short requests have only the first splits: a fixed pairing of splits
+// and XCDs measured 462 us against 276).
+// Not given: the splits' length, the same for all requests, is the shortest for which the requests' partials together are no
+// more than the grid has pairs, so that a batch of mixed lengths fills it as well as one of equal ones; each workgroup finds it
+// from the lengths (a lane per request, a search by halves).
+__device__ __forceinline__ bool program_of(const Args& a, int p, int& s, int& kvh, int& b, int& parts, int& keys) {
   kvh = p % a.Hkv;
   const int q = p / a.Hkv;
-  rho = q / a.S;
-  s = (q + rho) % a.S;
+  if (a.split_keys > 0 || a.SC == 1) {
+    const int rho = q / a.S;
+    s = (q + rho) % a.S;
+    b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+    parts = a.SC;
+    keys = a.split_keys;
+    return true;
+  }
+  const int lane = threadIdx.x & 63;
+  const bool mine = lane < a.bs;
+  const int tiles = mine ? (kv8::bounded_len(a.pages, a.ctx_lens[lane]) + TK - 1) / TK : 0;
+  const int extra = a.S - a.SC, want = a.pairs - extra * a.bs;
+  const int total = kv8::wave_sum(tiles);
+  auto count = [&](int k) { return mine ? max(1, (tiles + k - 1) / k) : 0; };
+  // (at hi, total / hi + bs of them at most)
+  int lo = max(a.min_tiles, (total + want - 1) / want);
+  int hi = max(lo, max(total / (want - a.bs), total / a.SC) + 1);
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2, c = count(mid);
+    const bool fits = __builtin_amdgcn_ballot_w64(c > a.SC) == 0 && kv8::wave_sum(c) <= want;
+    hi = fits ? mid : hi;
+    lo = fits ? lo : mid + 1;
+  }
+  const int c = count(lo), n = mine ? c + extra : 0;
+  const int end = kv8::wave_scan(n);
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(q >= end - n && q < end);
+  if (hit == 0) return false;
+  b = __builtin_ctzll(hit);
+  parts = __builtin_amdgcn_readlane(c, b);
+  s = q - __builtin_amdgcn_readlane(end - n, b);
+  if (s == parts) s = a.SC;  // the block keys' partial
+  keys = lo * TK;
+  return true;
 }
 
-// The keys [lo, hi) of context split s
-__device__ __forceinline__ void split_range(const Args& a, int s, int ctx, int& lo, int& hi) {
+// The keys [lo, hi) of context split s of `parts`
+__device__ __forceinline__ void split_range(int s, int parts, int keys, int ctx, int& lo, int& hi) {
   lo = 0;
   hi = ctx;
-  if (a.SC > 1) {
-    lo = (int)min((int64_t)s * a.split_keys, (int64_t)ctx);
-    if (s < a.SC - 1) hi = lo + min(a.split_keys, ctx - lo);  // (the last split takes what a longer context has left)
+  if (parts > 1) {
+    lo = (int)min((int64_t)s * keys, (int64_t)ctx);
+    if (s < parts - 1) hi = lo + min(keys, ctx - lo);  // (the last split takes what a longer context has left)
   }
 }
 
@@ -290,14 +329,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
   // workgroup -> (program, unit group); the unit groups of a program read the same keys: consecutive on one XCD (workgroup
   // id modulo 8), they share its L2
-  const int P = a.bs * a.Hkv * a.S;
+  const int P = (a.pairs ? a.pairs : a.bs * a.S) * a.Hkv;
   const int jx = blockIdx.x >> 3;
   const int ug = jx % a.ngroups;
   const int pidx = (jx / a.ngroups) * 8 + (blockIdx.x & 7);
   if (pidx >= P) return;
-  int s, kvh, rho;
-  program_of(a, pidx, s, kvh, rho);
-  const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+  int s, kvh, b, parts, keys;
+  if (!program_of(a, pidx, s, kvh, b, parts, keys)) return;
 
   // this lane's query row; a padding row computes a copy of the last one and stores nothing
   const int u0 = (ug * NW + w) * UROWS;
@@ -320,7 +358,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
   const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, given_len) : 0);
   int lo, hi;
-  split_range(a, s, ctx, lo, hi);
+  split_range(s, parts, keys, ctx, lo, hi);
   bool with_block = a.kn != nullptr;
   if (a.S > a.SC) {  // split: the block keys are a partial of their own
     if (s == a.SC) lo = hi = ctx;
@@ -328,7 +366,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   }
   const int ntiles = (hi - lo + TK - 1) / TK;
   const int last = ntiles - 1;
-  if (tid == 0 && s == 0 && ug == 0 && kvh == 0 && ctx != given_len) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  if (tid == 0 && s == 0 && ug == 0 && kvh == 0) {
+    if (ctx != given_len) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+    if (a.S > 1) a.ws_n[b] = parts;
+  }
   if (a.S > 1 && ntiles == 0 && !with_block) {  // an empty split
     if (row_ok && half == 0) a.ws_lse[partial_row(a, s, b, kvh, r)] = -INFINITY;
     return;
@@ -727,16 +768,18 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int half = lane >> 5, l32 = lane & 31;
   const int KL = a.KL, Lb = a.L, rows = a.rows;
   const float scale = a.scale_log2;
-  int s, kvh, rho;
-  program_of(a, blockIdx.x, s, kvh, rho);
-  const int b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+  int s, kvh, b, parts, keys;
+  if (!program_of(a, blockIdx.x, s, kvh, b, parts, keys)) return;
   const int32_t* trow = kv8::table_row(a.pages, b);
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1, num_pages = a.pages.num_pages;
   const int ctx = __builtin_amdgcn_readfirstlane(trow && num_pages > 0 ? kv8::bounded_len(a.pages, a.ctx_lens[b]) : 0);
   int lo, hi;
-  split_range(a, s, ctx, lo, hi);
+  split_range(s, parts, keys, ctx, lo, hi);
   const bool with_block = a.kn != nullptr && s == 0;
-  if (tid == 0 && s == 0 && kvh == 0 && ctx != a.ctx_lens[b]) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+  if (tid == 0 && s == 0 && kvh == 0) {
+    if (ctx != a.ctx_lens[b]) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+    if (a.S > 1) a.ws_n[b] = parts;
+  }
   if (lo >= hi && !with_block && a.S > 1) {  // an empty split
     if (tid < rows) a.ws_lse[partial_row(a, s, b, kvh, tid)] = -INFINITY;
     return;
@@ -1018,9 +1061,10 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
   const int64_t prow = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   if (prow >= per) return;
   const int d0 = (threadIdx.x & 15) * 8;
+  const int parts = a.split_keys > 0 ? a.SC : a.ws_n[prow / a.rows / a.Hkv], S = parts + a.S - a.SC;
   float m = -INFINITY, tot = 0.f;
   float acc[8] = {};
-  for (int s0 = 0; s0 < a.S; s0 += SB) {
+  for (int s0 = 0; s0 < S; s0 += SB) {
     float l[SB], ex[SB];
     u32x4 oh[SB];
 #pragma unroll
@@ -1028,8 +1072,8 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
       l[j] = -INFINITY;
       ex[j] = 0.f;
       oh[j] = (u32x4){};
-      if (s0 + j < a.S) {
-        const int64_t at = (s0 + j) * per + prow;
+      if (s0 + j < S) {
+        const int64_t at = (s0 + j < parts ? s0 + j : a.SC) * per + prow;
         l[j] = a.ws_lse[at];
         ex[j] = a.ws_exp[at];
         oh[j] = *reinterpret_cast<const u32x4*>(a.ws_o + at * D + d0);
@@ -1343,7 +1387,8 @@ extern "C" int64_t mfd_kv8_attn_workspace_bytes(int bs, int num_modes, int block
                                                 int num_ctx_splits) {
   if (num_ctx_splits <= 1 || bs < 1 || num_modes < 1 || block_size < 1 || H < 1 || Hkv < 1) return 0;
   const int64_t rows = (int64_t)bs * H * num_modes * block_size;
-  return partials(with_block, num_ctx_splits, (int)(H / Hkv * (int64_t)num_modes * block_size)) * rows * (D * 2 + 4 + 4);
+  return partials(with_block, num_ctx_splits, (int)(H / Hkv * (int64_t)num_modes * block_size)) * rows * (D * 2 + 4 + 4) +
+         (int64_t)bs * 4;
 }
 
 static int check_attn(const char* who, int bs, int num_modes, int block_size, int H, int Hkv, float scale,
@@ -1375,8 +1420,9 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
   if (rc == MFD_OK) rc = check_attn(who, bs, num_modes, block_size, H, Hkv, scale, q, q_st, q_sh);
   if (rc != MFD_OK) return rc;
   if (num_ctx_splits < 1 || num_ctx_splits > 1024 ||
-      (num_ctx_splits > 1 && (split_keys < TK || split_keys % TK != 0)))
-    return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: num_ctx_splits %d (1..1024) of split_keys %d (a multiple of %d)", who,
+      (num_ctx_splits > 1 && (split_keys < 0 || split_keys % TK != 0 || (split_keys == 0 && bs > 64))))
+    return mfd_set_error(MFD_ERR_INVALID_ARG,
+                         "%s: num_ctx_splits %d (1..1024) of split_keys %d (a multiple of %d, 0 for up to 64 requests)", who,
                          num_ctx_splits, split_keys, TK);
   if (bs == 0) return MFD_OK;
   if (!q || !out || !ctx_lens || (!k_new) != (!v_new) ||
@@ -1399,7 +1445,7 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
   a.bs = bs; a.K = num_modes; a.L = block_size; a.H = H; a.Hkv = Hkv; a.G = H / Hkv;
   a.KL = num_modes * block_size;
   a.rows = a.G * a.KL;
-  a.SC = num_ctx_splits; a.split_keys = split_keys;
+  a.SC = num_ctx_splits; a.split_keys = num_ctx_splits > 1 ? split_keys : 0;
   a.S = (int)partials(k_new != nullptr, num_ctx_splits, a.rows);
   a.causal = causal_in_block ? 1 : 0;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -1408,8 +1454,8 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
   a.ws_o = static_cast<uint16_t*>(workspace);
   a.ws_lse = workspace ? reinterpret_cast<float*>(a.ws_o + a.S * prows * D) : nullptr;
   a.ws_exp = workspace ? a.ws_lse + a.S * prows : nullptr;
+  a.ws_n = workspace ? reinterpret_cast<int32_t*>(a.ws_exp + a.S * prows) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t programs = (int64_t)bs * Hkv * a.S;
   const int units = (a.rows + UROWS - 1) / UROWS;
   // Eight waves share a tile's widening where they all have a unit, and in a batch that half fills the chip even where some
   // idle (16 requests of 4000 tokens: 12 units 134 us against 169 with four, 20 units 245 against 268; 4 requests, 12 units 65
@@ -1417,6 +1463,14 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
   const int64_t by8 = (int64_t)bs * Hkv * ((units + 7) / 8);
   const int NW = units % 8 == 0 || (units > 4 && 2 * by8 >= mfd_num_cus()) ? 8 : 4;
   a.ngroups = (units + NW - 1) / NW;
+  if (num_ctx_splits > 1 && split_keys == 0) {
+    // whole rounds of the workgroups that run together, as few as leave a request two splits on average
+    const int64_t slots = (int64_t)mfd_num_cus() * (NW == 8 && units > 1 ? 1 : 2), per = (int64_t)Hkv * a.ngroups;
+    const int64_t need = (int64_t)bs * (2 + a.S - a.SC);
+    a.pairs = (int)std::max(need, (need * per + slots - 1) / slots * slots / per);
+    a.min_tiles = units == 1 ? 2 : 4;
+  }
+  const int64_t programs = (a.pairs ? a.pairs : (int64_t)bs * a.S) * Hkv;
   const int64_t grid = units == 1 ? programs : (programs + 7) / 8 * 8 * a.ngroups;
   if (grid > 0x7fffffff || (prows + 15) / 16 > 0x7fffffff)
     return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: %lld workgroups", who, (long long)grid);

@@ -187,21 +187,11 @@ __global__ __launch_bounds__(256) void evict_score_kernel(SelectArgs a) {
   a.keys[b * a.key_stride + t] = key_of(a, weight_row(a, b), t, len);
 }
 
-// Inclusive prefix sum over a wave's lanes, by DPP: within rows of 16, then a row's last lane to the rows behind it
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
-  return v;
-}
 // Exclusive prefix sum of v over the workgroup's ST threads; buf: ST / 64 words, other ones than the scan before took. One
 // barrier.
 __device__ __forceinline__ int group_scan(int v, int* buf) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int s = wave_scan(v);
+  const int s = kv8::wave_scan(v);
   if (lane == 63) buf[w] = s;
   __syncthreads();
   int before = 0;

@@ -40,6 +40,18 @@ __device__ __forceinline__ void raise(int32_t* err_flag, int bit) {
   if (err_flag) atomicOr(err_flag, bit);
 }
 
+// Inclusive prefix sum over a wave's lanes, by DPP: within rows of 16, then a row's last lane to the rows behind it
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
 // Smallest 2^e with amax / 2^e <= 448 = 0.875 * 2^9, e within the range (amax finite, not negative).
 __device__ __forceinline__ float page_scale(float amax) {
   const uint32_t bits = __float_as_uint(amax);

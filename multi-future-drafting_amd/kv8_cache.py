@@ -158,37 +158,33 @@ def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int,
     """(num_ctx_splits, split_keys) for num_ctx_splits < 0, from what the kernels' workgroup slots hold (two workgroups per CU,
     one of eight waves) and the programs (request, KV head, group of units) that there are without a split.
 
-    A single request's splits fill one round of slots, less the block partial's, and so do a small batch's (up to a third of
-    the slots whole: 2 requests of up to 8192 tokens, 32 heads, 8 x 16 queries, 36 to 45 us in 7 parts, 47 to 60 in 12); a
-    larger one's lengths differ and half a round more evens them out. At least 256 keys per split, at most 64 splits.
-
-    Where a program is one unit (plain decoding), a batch gets a workgroup per CU, or parts of 2048 tokens where those are
-    more, up to three rounds: 4 requests of up to 8192 tokens, 32 heads, 21 us in 8 parts, 28 in 32; 16 requests of 4748 ..
-    32132 tokens, 40 heads, 173 us with one round, 146 with three, 152 with eight; 64 even ones, a workgroup per slot already:
-    66 us whole, 76 in two parts. At least 128 keys per split, at most 32 splits (32768 tokens, one request: 28 us in 32
+    A single request's splits fill one round of slots, less the block partial's. A batch's (up to 64 requests) are measured out
+    on the device (keys 0), as long as makes all of them together fill the rounds whatever the lengths: 4 requests of 700 ..
+    8000 tokens, 32 heads, 8 x 16 queries, 62 us against 87 with a third of the longest each; 3 of 1024 .. 8192 45 against 60;
+    equal lengths as before. Plain decoding (a program is one unit) of few requests keeps a workgroup per CU, or parts of 2048
+    tokens where those are more: the device's search and one more load in the merge cost 2 us (4 requests of up to 8192 tokens 22.7
+    us against 25.3; 16 56.0 against 43.7). At least 128 keys per split there and 256 else (32768 tokens, one request: 28 us in 32
     parts, 34 in 64)."""
     units = -(-rows // UNIT)
     cus = mfd_hip.cu_count(device)
     waves = 8 if units % 8 == 0 or units > 4 and 2 * bs * heads * -(-units // 8) >= cus else 4  # (as mfd_kv8_attn does)
     slots = cus * (1 if waves == 8 else 2)
     programs = max(1, bs * heads * -(-units // waves))
-    if units == 1:
-        if programs >= slots:
-            splits = 1
-        elif bs == 1:
-            splits = slots // programs
-        else:
+    if programs >= slots:
+        return 1, 0
+    least = 128 if units == 1 else 256
+    if bs == 1 or bs > 64 or units == 1 and 8 * programs < slots:
+        splits = slots // programs - (1 if with_block and units > 1 else 0)
+        if units == 1 and bs > 1:
             splits = min(3 * slots // programs, max(cus // programs, max_ctx // 2048))
-        splits = min(splits, -(-max_ctx // 128), 32)
-    else:
-        if bs == 1:
-            splits = slots // programs - (1 if with_block else 0)
-        elif 3 * programs <= slots:
-            splits = -(-slots // programs) - 1 if with_block else slots // programs
-        else:
-            splits = 3 * slots // (2 * programs)
-        splits = min(splits, -(-max_ctx // 256), 64)
-    return _splits_of(splits, max_ctx) if splits > 1 else (1, 0)
+        splits = min(splits, -(-max_ctx // least), 32 if units == 1 else 64)
+        return _splits_of(splits, max_ctx) if splits > 1 else (1, 0)
+    # the pairs (request, partial) that mfd_kv8_attn deals out; one request's splits at most what the others leave
+    extra = 1 if with_block and units > 1 else 0
+    per, need = programs // bs, bs * (2 + extra)
+    pairs = max(need, -(-need * per // slots) * slots // per)
+    splits = min(pairs - extra * bs - bs + 1, -(-max_ctx // least), 32 if units == 1 else 16)
+    return (splits, 0) if splits > 1 else (1, 0)
 
 
 def _splits_of(splits: int, max_ctx: int) -> tuple[int, int]:

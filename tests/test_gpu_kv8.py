@@ -100,6 +100,11 @@ ATTN = [
     ([130], 2, 40, 4, 2, 256, True, False, 1),                        # blocks of 40: modes cross units and tiles
     ([90], 1, 150, 2, 1, 32, True, True, 2),                          # one long causal block over three tiles
     ([200, 1], 1, 5, 26, 2, 64, False, False, -1),                    # 65 rows without block keys
+    ([3000, 0, 700, 5000], 8, 16, 8, 2, 64, True, False, -1),               # splits measured out by the lengths
+    ([0, 0, 0], 4, 16, 8, 2, 64, True, True, -1), ([9000, 1], 3, 16, 4, 1, 32, False, False, -1),
+    ([i * 37 % 1500 for i in range(64)], 1, 40, 2, 1, 16, True, False, -1),  # .. of as many requests as a wave has lanes
+    ([2000 * (i % 7) + i for i in range(16)], 1, 1, 32, 8, 64, True, False, -1),
+    ([500 + i * 90 for i in range(65)], 1, 1, 8, 2, 64, False, False, -1),   # .. and one more than that
     ([64 + 7 * i for i in range(16)], 2, 16, 40, 8, 64, True, False, -1),   # a batch with idle waves: five units
     ([3 + 11 * i for i in range(16)], 1, 40, 40, 8, 32, True, True, 2),     # .. seven, small pages, splits
     ([1 + 17 * i % 97 for i in range(40)], 1, 1, 32, 8, 16, True, False, 1),  # plain decoding, more workgroups than CUs

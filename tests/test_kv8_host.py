@@ -114,7 +114,7 @@ EVERY = [(f, kw, c, w) for f in (_store, _attn, _weigh, _compact) for kw, c, w i
     (_attn, dict(q=P + 4), UNSUPPORTED, "16-byte"), (_attn, dict(os=(4096, 12)), UNSUPPORTED, "16-byte"),
     (_attn, dict(kn=None), INVALID, "null"), (_attn, dict(vn=None), INVALID, "null"), (_attn, dict(lens=None), INVALID, "null"),
     (_attn, dict(splits=0), INVALID, "num_ctx_splits"), (_attn, dict(splits=4, keys=100), INVALID, "split_keys"),
-    (_attn, dict(splits=4, keys=0), INVALID, "split_keys"), (_attn, dict(splits=4, keys=64), INVALID, "workspace"),
+    (_attn, dict(splits=4, keys=0, bs=65), INVALID, "split_keys"), (_attn, dict(splits=4, keys=64), INVALID, "workspace"),
     (_attn, dict(splits=4, keys=64, ws=P, nws=100), INVALID, "workspace"),
     (_attn, dict(splits=4, keys=64, ws=P + 8, nws=1 << 30), INVALID, "workspace"),
     (_weigh, dict(decay=-0.1), INVALID, "decay"), (_weigh, dict(decay=float("nan")), INVALID, "decay"),
@@ -140,8 +140,8 @@ def test_c_entries_with_nothing_to_do():
     lib = mfd_hip.lib()
     assert lib.mfd_kv8_attn_workspace_bytes(2, 8, 16, 32, 8, 1, 1) == 0
     # 4 splits and the block's partial, 2 x 32 x 128 rows: fp16 rows of 128, lse, scale exponent
-    assert lib.mfd_kv8_attn_workspace_bytes(2, 8, 16, 32, 8, 1, 4) == 5 * 2 * 32 * 128 * (256 + 8)
-    assert lib.mfd_kv8_attn_workspace_bytes(2, 1, 1, 32, 8, 1, 4) == 4 * 2 * 32 * (256 + 8)
+    assert lib.mfd_kv8_attn_workspace_bytes(2, 8, 16, 32, 8, 1, 4) == 5 * 2 * 32 * 128 * (256 + 8) + 2 * 4
+    assert lib.mfd_kv8_attn_workspace_bytes(2, 1, 1, 32, 8, 1, 4) == 4 * 2 * 32 * (256 + 8) + 2 * 4
     assert lib.mfd_evict_select_workspace_bytes(3, 16384) == 0  # (keys in registers)
     assert lib.mfd_evict_select_workspace_bytes(3, 16385) == 3 * 16388 * 4
 
@@ -300,12 +300,15 @@ def test_pool_refuses_page_sizes():
         kv8_cache.Kv8Pool(num_layers=1, num_pages=2, page_size=100, num_kv_heads=1, device="cpu")
 
 
-@pytest.mark.parametrize("bs,heads,rows", [(1, 8, 4), (16, 8, 5), (64, 8, 4), (1, 8, 512), (16, 8, 640), (4, 2, 64)])
+@pytest.mark.parametrize("bs,heads,rows", [(1, 8, 4), (16, 8, 5), (64, 8, 4), (1, 8, 512), (16, 8, 640), (4, 2, 64), (65, 1, 3)])
 def test_split_choice_covers_the_context(monkeypatch, bs, heads, rows):
     monkeypatch.setattr(mfd_hip, "cu_count", lambda device: 256)
     for ctx in (1, 63, 64, 65, 1000, 8192, 100001):
         splits, keys = kv8_cache._auto_splits(bs, heads, rows, True, ctx, None)
-        assert (splits, keys) == (1, 0) or (splits > 1 and keys % 64 == 0 and (splits - 1) * keys < ctx <= splits * keys)
+        if keys == 0:  # one pass, or measured out on the device
+            assert splits == 1 or 1 < bs <= 64 and 1 < splits <= 32
+        else:
+            assert splits > 1 and keys % 64 == 0 and (splits - 1) * keys < ctx <= splits * keys
         for want in (2, 3, 64):
             s, k = kv8_cache._splits_of(want, ctx)
             assert 1 <= s <= want and k % 64 == 0 and (s - 1) * k < ctx <= s * k
