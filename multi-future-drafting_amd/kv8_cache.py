@@ -162,8 +162,8 @@ def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int,
     on the device (keys 0), as long as makes all of them together fill the rounds whatever the lengths: 4 requests of 700 ..
     8000 tokens, 32 heads, 8 x 16 queries, 62 us against 87 with a third of the longest each; 3 of 1024 .. 8192 45 against 60;
     equal lengths as before. Plain decoding (a program is one unit) of few requests keeps a workgroup per CU, or parts of 2048
-    tokens where those are more: the device's search and one more load in the merge cost 2 us (4 requests of up to 8192 tokens 22.7
-    us against 25.3; 16 56.0 against 43.7). At least 128 keys per split there and 256 else (32768 tokens, one request: 28 us in 32
+    tokens where those are more: the device's search and one more load in the merge cost 2 us (4 requests of up to 8192 tokens
+    22.7 us against 25.3; 16 56.0 against 43.7). At least 128 keys per split there and 256 else (32768 tokens, one request: 28 us in 32
     parts, 34 in 64)."""
     units = -(-rows // UNIT)
     cus = mfd_hip.cu_count(device)
