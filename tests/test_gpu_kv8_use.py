@@ -374,6 +374,43 @@ def test_a_captured_round_replays():
             assert all(torch.equal(x, y) for x, y in zip(eager, s.state()))
 
 
+def test_a_captured_attention_follows_the_lengths():
+    """Captured with one batch's lengths and replayed with others, none among them: splits are measured out on the device."""
+    import kv8_cache
+
+    for K, L, H in ((4, 16, 8), (1, 2, 32)):
+        bs, page, Hkv = 9, 64, 8
+        most = [900 + 300 * b for b in range(bs)]
+        d = make_pool(most, page, Hkv, seed=795)
+        g = _gen(796)
+        T = bs * K * L
+        q, kn, vn = _bf(g, T, H, D).cuda(), _bf(g, T, Hkv, D).cuda(), _bf(g, T, Hkv, D).cuda()
+        args, table, lens = cache_args(d), d["table"].cuda(), d["lens"].cuda()
+        out, lse = torch.zeros_like(q), torch.zeros(T, H, device="cuda")
+        size = kv8_cache.workspace_bytes(bs=bs, num_modes=K, block_size=L, num_heads=H, num_kv_heads=Hkv, with_block=True,
+                                         max_ctx=max(most))
+        assert size > 0
+        ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+        run = lambda **kw: kv8_cache.paged_mode_block_attention_kv8(  # noqa: E731
+            q=q, k_new=kn, v_new=vn, page_table=table, ctx_lens=lens, num_modes=K, block_size=L, scaling=SCALE,
+            max_ctx=max(most), return_lse=True, **kw, **args)
+        run(out=out, lse_out=lse, workspace=ws)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(out=out, lse_out=lse, workspace=ws)
+        for turn in range(4):
+            now = [0] * bs if turn == 2 else [(n * (turn + 3) * (b + 2)) % (n + 1) for b, n in enumerate(most)]
+            lens.copy_(torch.tensor(now))
+            o, l = run()
+            torch.cuda.synchronize()
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert _same(o, out) and _same(l, lse)
+            check_attention(out, lse, oracle_attention(d, q.cpu(), kn.cpu(), vn.cpu(), now, K, L, SCALE, False))
+
+
 def test_on_another_stream():
     s = _Step(790)
     s.refill(791)
