@@ -1468,7 +1468,7 @@ extern "C" int mfd_kv8_attn(const uint16_t* q, int64_t q_st, int64_t q_sh, const
     const int64_t slots = (int64_t)mfd_num_cus() * (NW == 8 && units > 1 ? 1 : 2), per = (int64_t)Hkv * a.ngroups;
     const int64_t need = (int64_t)bs * (2 + a.S - a.SC);
     a.pairs = (int)std::max(need, (need * per + slots - 1) / slots * slots / per);
-    a.min_tiles = units == 1 ? 2 : 4;
+    a.min_tiles = units == 1 ? 2 : 3;  // (shorter splits cost more in partials than they save)
   }
   const int64_t programs = (a.pairs ? a.pairs : (int64_t)bs * a.S) * Hkv;
   const int64_t grid = units == 1 ? programs : (programs + 7) / 8 * 8 * a.ngroups;

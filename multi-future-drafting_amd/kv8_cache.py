@@ -163,16 +163,25 @@ def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int,
     8000 tokens, 32 heads, 8 x 16 queries, 62 us against 87 with a third of the longest each; 3 of 1024 .. 8192 45 against 60;
     equal lengths as before. Plain decoding (a program is one unit) of few requests keeps a workgroup per CU, or parts of 2048
     tokens where those are more: the device's search and one more load in the merge cost 2 us (4 requests of up to 8192 tokens
-    22.7 us against 25.3; 16 56.0 against 43.7). At least 128 keys per split there and 256 else (32768 tokens, one request: 28 us in 32
-    parts, 34 in 64)."""
+    22.7 us against 25.3; 16 56.0 against 43.7). At least 128 keys per split there and 192 else (32768 tokens, one request:
+    28 us in 32 parts, 34 in 64).
+
+    Short contexts stay whole: splits cost the block's own partial, the merge and its launch. Plain decoding up to 640 tokens
+    (600: 12.9 us against 12.0 on the device, but 16.3 against 21.2 with the call's host time); else the longer the more of the
+    slots the whole programs fill (8 x 16 queries, 32 heads: one request of 200 tokens 17.4 us split, 22.6 whole; 6 of 600 42.6
+    and 36.7, of 1500 52.5 and 60.7; 12 of 1500 93.5 and 66.7)."""
     units = -(-rows // UNIT)
     cus = mfd_hip.cu_count(device)
     waves = 8 if units % 8 == 0 or units > 4 and 2 * bs * heads * -(-units // 8) >= cus else 4  # (as mfd_kv8_attn does)
     slots = cus * (1 if waves == 8 else 2)
     programs = max(1, bs * heads * -(-units // waves))
-    if programs >= slots:
+    if units == 1:
+        short = 640
+    else:
+        short = 5120 * programs // slots - 1024 if 3 * programs > slots else 1536 * programs // slots
+    if programs >= slots or max_ctx <= short:
         return 1, 0
-    least = 128 if units == 1 else 256
+    least = 128 if units == 1 else 192
     if bs == 1 or bs > 64 or units == 1 and 8 * programs < slots:
         splits = slots // programs - (1 if with_block and units > 1 else 0)
         if units == 1 and bs > 1:
