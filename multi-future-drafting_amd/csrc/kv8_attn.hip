@@ -12,7 +12,8 @@
 // O^T += V^T P^T in fp16: V as bare codes (exact), P rounded to fp16 (2^-11 at most, an eighth of the bf16 output's own
 // rounding), times the quotient of the page's v_scale and the accumulators' unit: a power of two, which the exponential
 // takes along in its argument and the row sum leaves out again, both exactly. The accumulators are brought to another unit
-// only where that quotient leaves [2^-2, 2^6] (P stays below 2^14 and mostly above fp16's subnormals). Statistics are fp32.
+// only where that quotient leaves [2^-2, 2^6] (P stays below 2^14 and mostly above fp16's subnormals; a probability among
+// them is off by 2^-23 of the row's sum at most). Statistics are fp32.
 //
 // Two kernels, by the units of a KV head:
 //  * tile kernel: the waves of a workgroup (a unit each) share 64-key tiles. The codes come from memory to registers, two
@@ -725,7 +726,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (a.lse && row_ok && half == 0) a.lse[token * a.H + head] = lse2 * LN2;
     return;
   }
-  // partial row in fp16, scaled by a power of two into (-1, 1): half the bytes of fp32 for the merge to read back
+  // partial row in fp16, scaled by a power of two into (-1, 1): half the bytes of fp32 for the merge to read back, at 2^-11 of
+  // a component, or 2^-24 of the row's largest where that is more
   float mx = 0.f;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)

@@ -98,6 +98,37 @@ def test_a_nan_code_reaches_the_rows_that_see_it():
     assert _same(o0, o1)
 
 
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_value_scales_at_both_ends(form):
+    """Neighbouring pages whose values are a factor of 2^80 apart, the scales' whole range, in both orders and alone: the
+    accumulators change their unit with each.
+
+    Here probabilities far below the row's largest decide the result, and fp16 has fewer bits for those. A probability p enters
+    as fp16(p 2^q), q >= -2 the quotient of the page's scale and the unit, p relative to a maximum that the row has met, so that
+    the row's sum is at least 1. Below 2^-14 half a step is 2^-25: p / sum is off by 2^-25 2^-q <= 2^-23 at most, beside its
+    2^-11. Over the cached keys that is 2^-23 sum |v| on top of the bound elsewhere. A split's partial row is rounded to fp16
+    after a power of two has brought its largest component m into [1/2, 1): components below 2^-14 are off by 2^-25 there, 2^-24 m
+    in the row at most. (With one page deciding, single codes of very different size make up a row.)"""
+    K, L, H, Hkv, page, causal, splits = FORMS[form]
+    for ends in ((-40, 40), (40, -40), (-40, -40), (40, 40), (0, -40)):
+        lens = [5 * page + 3, page + 1]
+        d = make_pool(lens, page, Hkv, seed=780 + form)
+        for b, n in enumerate(lens):
+            for i in range(-(-n // page)):
+                d["v_scale"][int(d["table"][d["rows"][b]][i])] = 2.0 ** ends[i % 2]
+        g = _gen(790)
+        T = 2 * K * L
+        q, kn, vn = _bf(g, T, H, D), _bf(g, T, Hkv, D), _bf(g, T, Hkv, D)
+        o, l = _attend(d, cache_args(d), q.cuda(), kn.cuda(), vn.cuda(), K, L, num_ctx_splits=splits, causal_in_block=causal)
+        ref = oracle_attention(d, q, kn, vn, lens, K, L, SCALE, causal)
+        for b, n in enumerate(lens):
+            v = kv8.tokens(vals(d["v_cache"]), vals(d["v_scale"]), d["table"][d["rows"][b]].numpy(), n, page)
+            mass = ref[2][b * K * L:(b + 1) * K * L]
+            more = np.abs(v).sum(0).repeat(H // Hkv, 0) * 2.0 ** -23 + mass.max(-1, keepdims=True) * 2.0 ** -24
+            mass += more / (2 * 2.0 ** -11 + 2.0 ** -12)
+        check_attention(o, l, ref)
+
+
 def test_weights_of_rows_taken_out():
     """Rows whose lse is -inf add nothing, whatever their q holds."""
     import kv8_cache
