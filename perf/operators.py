@@ -18,7 +18,6 @@ The cache holds e4m3 codes [slots, KV heads, 128] and float32 scales [pages, KV 
 
 from __future__ import annotations
 
-import functools
 import math
 import os
 import random
@@ -40,9 +39,8 @@ _CTX16 = "7316,1903,5221,2874,6650,1187,4096,8033,3519,5902,1466,7704,2333,4777,
 _NEW16 = "5,1,9,3,16,2,7,1,4,12,1,6,3,8,2,10"
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
-    """The framework's modules (its directory on the path as a user puts it), imported once as a program does."""
+    """The framework's modules (its directory on the path as a user puts it)."""
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "multi-future-drafting_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
