@@ -726,14 +726,22 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (a.lse && row_ok && half == 0) a.lse[token * a.H + head] = lse2 * LN2;
     return;
   }
-  // partial row in fp16, scaled by a power of two into (-1, 1): half the bytes of fp32 for the merge to read back, at 2^-11 of
-  // a component, or 2^-24 of the row's largest where that is more
+  // partial row in fp16, its finite components scaled by a power of two into (-1, 1): half the bytes of fp32 for the merge to
+  // read back, at 2^-11 of a component, or 2^-24 of the row's largest where that is more
   float mx = 0.f;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int x = 0; x < 16; ++x) mx = fmaxf(mx, fabsf(oacc[db][x] * inv));
   mx = half_max(mx);
+  if (__builtin_amdgcn_ballot_w64(mx == INFINITY) != 0) {  // (hardly ever: the test per component would cost 1 us)
+    mx = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) mx = fmaxf(mx, kv8::finite_abs(oacc[db][x] * inv));
+    mx = half_max(mx);
+  }
   const int ex = mx > 0.f ? __builtin_amdgcn_frexp_expf(mx) : 0;
   const float down = __builtin_ldexpf(inv, -ex);
 #pragma unroll
@@ -1031,7 +1039,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
   for (int c = 0; c < DPT / 4; ++c)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(o[c][e] * inv));
+    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, kv8::finite_abs(o[c][e] * inv));
 #pragma unroll
   for (int x = 1; x < TPR; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
   const int ex = mx > 0.f ? __builtin_amdgcn_frexp_expf(mx) : 0;

@@ -62,7 +62,7 @@ __device__ __forceinline__ float page_scale(float amax) {
 // 1 / s of a power of two within the range
 __device__ __forceinline__ float inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// |x|, with infinities and NaN as 0: they do not set a page's scale
+// |x|, with infinities and NaN as 0: they set neither a page's scale nor a partial row's
 __device__ __forceinline__ float finite_abs(float x) {
   const float v = fabsf(x);
   return v < INFINITY ? v : 0.f;
