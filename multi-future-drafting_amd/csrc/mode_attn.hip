@@ -709,6 +709,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(oacc[db][r] * inv));
     mx = half_max(mx);
+    if (__builtin_amdgcn_ballot_w64(mx == INFINITY) != 0) {  // the finite components decide the scale
+      mx = 0.f;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = fabsf(oacc[db][r] * inv);
+          mx = fmaxf(mx, x < INFINITY ? x : 0.f);
+        }
+      mx = half_max(mx);
+    }
     const int ex = mx > 0.f ? __builtin_amdgcn_frexp_expf(mx) : 0;  // mx = f 2^ex, f in [0.5, 1)
     const float down = __builtin_ldexpf(inv, -ex);
     if (!row_ok) return;
