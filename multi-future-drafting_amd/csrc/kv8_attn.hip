@@ -196,24 +196,24 @@ __device__ __forceinline__ void set_unit(uint32_t to, uint32_t& unit, f32x16 (&o
 }
 
 // Request of scheduling rank rho: requests by context length, longest first (ties by index), so that the longest
-// workgroups start first and short ones fill in behind them.
+// workgroups start first and short ones fill in behind them. Up to MAX_RANKED of them, a lane each; larger batches go in their
+// own order: every workgroup compares all pairs, which soon takes longer than what it could save (plain decoding of up to 2048
+// tokens, 64 requests: 44.1 us ranked, 44.5 not; 128: 88 and 80, 512: 1241 and 254; 92 of 200 tokens and, behind them, four of
+// 8000: 94 and 94; thousands would hold the GPU for minutes).
+constexpr int MAX_RANKED = 64;
 __device__ __forceinline__ int request_of_rank(const int64_t* ctx_lens, int bs, int rho) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < bs; base += 64) {
-    const int b = base + lane;
-    int rank = -1;
-    if (b < bs) {
-      const int64_t cb = ctx_lens[b];
-      rank = 0;
-      for (int j = 0; j < bs; ++j) {
-        const int64_t cj = ctx_lens[j];
-        rank += (cj > cb || (cj == cb && j < b)) ? 1 : 0;
-      }
+  if (bs <= 1 || bs > MAX_RANKED) return rho;
+  const int b = threadIdx.x & 63;
+  int rank = -1;
+  if (b < bs) {
+    const int64_t cb = ctx_lens[b];
+    rank = 0;
+    for (int j = 0; j < bs; ++j) {
+      const int64_t cj = ctx_lens[j];
+      rank += (cj > cb || (cj == cb && j < b)) ? 1 : 0;
     }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(rank == rho);
-    if (hit) return base + __builtin_ctzll(hit);
   }
-  return rho;
+  return __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == rho));
 }
 
 // Program p: (KV head, request b, split s of `parts` of `keys` keys); false where there is none. KV heads fastest: with eight of
@@ -231,7 +231,7 @@ __device__ __forceinline__ bool program_of(const Args& a, int p, int& s, int& kv
   if (a.split_keys > 0 || a.SC == 1) {
     const int rho = q / a.S;
     s = (q + rho) % a.S;
-    b = __builtin_amdgcn_readfirstlane(a.bs > 1 ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+    b = __builtin_amdgcn_readfirstlane(request_of_rank(a.ctx_lens, a.bs, rho));
     parts = a.SC;
     keys = a.split_keys;
     return true;

@@ -170,24 +170,24 @@ __device__ __forceinline__ f32x16 mfma32_f16(f16x8 a, f16x8 b, f32x16 c) {
 enum { CTX_FLAT = 0, CTX_PAGED = 1, CTX_GATHER = 2 };
 
 // Request of scheduling rank rho: requests ordered by context length, longest first (ties by index),
-// so that the longest workgroups start first and the short ones fill in behind them.
+// so that the longest workgroups start first and the short ones fill in behind them. Up to MAX_RANKED of them, a lane
+// each; larger batches go in their own order: every workgroup compares all pairs, which soon takes longer than what it
+// could save (4 modes x 8, up to 2048 tokens, 32 requests: 42.4 us ranked, 44.5 not; 64: 57.4 and 53.7, 128: 86.4 and 86.4,
+// 512: 791 and 292; thousands would hold the GPU for minutes).
+constexpr int MAX_RANKED = 64;
 __device__ __forceinline__ int request_of_rank(const int64_t* ctx_lens, int bs, int rho) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < bs; base += 64) {
-    const int b = base + lane;
-    int rank = -1;
-    if (b < bs) {
-      const int64_t cb = ctx_lens[b];
-      rank = 0;
-      for (int j = 0; j < bs; ++j) {
-        const int64_t cj = ctx_lens[j];
-        rank += (cj > cb || (cj == cb && j < b)) ? 1 : 0;
-      }
+  if (bs <= 1 || bs > MAX_RANKED) return rho;
+  const int b = threadIdx.x & 63;
+  int rank = -1;
+  if (b < bs) {
+    const int64_t cb = ctx_lens[b];
+    rank = 0;
+    for (int j = 0; j < bs; ++j) {
+      const int64_t cj = ctx_lens[j];
+      rank += (cj > cb || (cj == cb && j < b)) ? 1 : 0;
     }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(rank == rho);
-    if (hit) return base + __builtin_ctzll(hit);
   }
-  return rho;
+  return __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == rho));
 }
 
 template <int CTX, int NW>
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int bk = pidx / a.S;
   const int kvh = bk % a.Hkv;
   const int rho = bk / a.Hkv;
-  const int b = __builtin_amdgcn_readfirstlane((a.ctx_lens && a.bs > 1) ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
+  const int b = __builtin_amdgcn_readfirstlane(a.ctx_lens ? request_of_rank(a.ctx_lens, a.bs, rho) : rho);
 
   const int upr = (KL + UROWS - 1) / UROWS;  // units per query head (the last one padded when KL % 32 != 0)
   const int U = a.G * upr;

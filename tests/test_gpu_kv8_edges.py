@@ -1,5 +1,5 @@
 """The 8-bit draft cache at the edges of what its calls allow: infinities beside very large and very small values in split
-contexts. Tolerances: those of test_gpu_kv8 and test_gpu_kv8_use, derived there."""
+contexts, batches of thousands. Tolerances: those of test_gpu_kv8, with what _bounded derives."""
 
 import numpy as np
 import pytest
@@ -12,13 +12,27 @@ from test_gpu_kv8_use import FORMS, SCALE, _attend, _bf
 pytestmark = pytest.mark.gpu
 
 
+def _bounded(ref, d, lens, KL, G):
+    """A reference whose ``mass`` covers fp16's subnormals too. Below 2^-14 half a step of fp16 is 2^-25. A probability p (of
+    a row whose sum is at least 1) enters as fp16(p 2^q), q >= -2: off by 2^-23 of the sum at most, 2^-23 sum |v| over the
+    cached keys. A split's partial row is rounded after a power of two has brought its largest finite component m into
+    [1/2, 1): off by 2^-24 m there, and its share of that in the result, at most 2^-24 of the row's largest mass for each of
+    up to four partials. check_attention takes (2 2^-11 + 2^-12) of ``mass``, so they are added divided by that."""
+    o, lse, mass, most = ref
+    for b, n in enumerate(lens):
+        v = kv8.tokens(vals(d["v_cache"]), vals(d["v_scale"]), d["table"][d["rows"][b]].numpy(), n, d["page"])
+        m = mass[b * KL:(b + 1) * KL]
+        more = np.abs(v).sum(0).repeat(G, 0) * 2.0 ** -23 + m.max(-1, keepdims=True) * 2.0 ** -22
+        m += more / (2 * 2.0 ** -11 + 2.0 ** -12)
+    return o, lse, mass, most
+
+
 @pytest.mark.parametrize("form", range(len(FORMS)))
 @pytest.mark.parametrize("size", [24, -30])
 def test_an_infinity_leaves_its_neighbours(form, size):
     """Infinities in single components of one mode's block values, the others about 2^24 (beyond fp16's largest) or 2^-30 (below
     its smallest): whatever the number of splits, the infinite components are infinite in the rows that see them, and all others
-    are what they are without it. The bound is test_value_scales_at_both_ends': a split's partial row is rounded to fp16 relative
-    to its largest finite component."""
+    are what they are without it."""
     K, L, H, Hkv, page, causal, _ = FORMS[form]
     print(f"case: kv8 infinity {FORMS[form]} 2^{size}", flush=True)
     lens, KL, G = [3 * page + 5, 0, 70], K * L, H // Hkv
@@ -30,12 +44,7 @@ def test_an_infinity_leaves_its_neighbours(form, size):
     spots = [(b * KL + L, 0, c, s) for b in range(3) for c, s in ((5, 1), (66, -1))]  # the first key of every request's mode 1
     for t, h, c, s in spots:
         vn[t, h, c] = 0  # (the oracle's: a masked infinity would be 0 times infinity there)
-    o, l, mass, most = oracle_attention(d, q, kn, vn, lens, K, L, SCALE, causal)
-    for b, n in enumerate(lens):
-        v = kv8.tokens(vals(d["v_cache"]), vals(d["v_scale"]), d["table"][d["rows"][b]].numpy(), n, page)
-        m = mass[b * KL:(b + 1) * KL]
-        more = np.abs(v).sum(0).repeat(G, 0) * 2.0 ** -23 + m.max(-1, keepdims=True) * 2.0 ** -24
-        m += more / (2 * 2.0 ** -11 + 2.0 ** -12)
+    ref = _bounded(oracle_attention(d, q, kn, vn, lens, K, L, SCALE, causal), d, lens, KL, G)
     bad = vn.clone()
     for t, h, c, s in spots:
         bad[t, h, c] = s * float("inf")
@@ -46,5 +55,28 @@ def test_an_infinity_leaves_its_neighbours(form, size):
         for t, h, c, s in spots:
             seen = out[t:t + L, h * G:(h + 1) * G, c]
             assert bool((seen == s * float("inf")).all()), (splits, t, c)
-            out[t:t + L, h * G:(h + 1) * G, c] = torch.from_numpy(o[t:t + L, h * G:(h + 1) * G, c]).to(torch.bfloat16)
-        check_attention(out, lse, (o, l, mass, most))
+            out[t:t + L, h * G:(h + 1) * G, c] = torch.from_numpy(ref[0][t:t + L, h * G:(h + 1) * G, c]).to(torch.bfloat16)
+        check_attention(out, lse, ref)
+
+
+@pytest.mark.parametrize("K,L,H,splits", [(1, 1, 4, 1), (1, 1, 4, 2), (2, 20, 2, 1), (2, 20, 2, 2)])
+def test_a_batch_of_thousands(K, L, H, splits):
+    """Thousands of requests in one call (every seventh compared)."""
+    import kv8_cache
+
+    bs, page, Hkv, KL = 3001, 16, 2, K * L
+    print(f"case: kv8 attention of {bs} requests {K} x {L} splits={splits}", flush=True)
+    g = _gen(830)
+    lens = torch.randint(0, 200, (bs,), generator=g)
+    pages = 200
+    d = make_pool([page * pages], page, Hkv, seed=831)
+    d.update(table=torch.randint(0, pages, (bs, -(-200 // page)), generator=g).int(), rows=torch.arange(bs))  # shared pages
+    q, kn, vn = _bf(g, bs * KL, H, D), _bf(g, bs * KL, Hkv, D), _bf(g, bs * KL, Hkv, D)
+    out, lse = kv8_cache.paged_mode_block_attention_kv8(
+        q=q.cuda(), k_new=kn.cuda(), v_new=vn.cuda(), page_table=d["table"].cuda(), ctx_lens=lens.cuda(), num_modes=K,
+        block_size=L, scaling=SCALE, num_ctx_splits=splits, max_ctx=200, return_lse=True, **cache_args(d))
+    some = torch.arange(0, bs, 7)
+    of = lambda t: t.cpu().view(bs, KL, -1, D)[some].reshape(len(some) * KL, -1, D)  # noqa: E731
+    d["rows"], n = some, lens[some].tolist()
+    ref = _bounded(oracle_attention(d, of(q), of(kn), of(vn), n, K, L, SCALE, False), d, n, KL, H // Hkv)
+    check_attention(of(out), lse.cpu().view(bs, KL, H)[some].reshape(-1, H), ref)

@@ -1,5 +1,5 @@
-"""Mode attention in bf16 with infinities among the block's values. A component that an infinity reaches is not finite (in the rows
-that see its key; what the masked ones get there is not looked at); every other component is what it is without it.
+"""Mode attention in bf16 in batches of thousands, and with infinities among the block's values: a component that one reaches is
+not finite (in the rows that see its key; what the masked ones get there is not looked at); every other is as without it.
 
 Tolerance: probabilities in fp16 (2^-11 of each), a split's partial row in fp16 (2^-11 of a component, or 2^-24 of the row's
 largest), scores and sums in fp32 (2^-12 at these sizes), the output in bf16 (2^-8):
@@ -41,3 +41,28 @@ def test_an_infinity_leaves_its_neighbours(K, L, H, Hkv, splits, ctx):
     others = np.ones((KL, H, D), bool)
     others[:, :G, [5, 66]] = False
     assert np.isfinite(got[others]).all() and (np.abs(got - o)[others] <= bound[others]).all()
+
+
+@pytest.mark.parametrize("page", [1, 64])
+def test_a_batch_of_thousands(page):
+    """Thousands of requests in one call: the bits of the same requests in calls of 60."""
+    import paged_mode_attention
+
+    bs, K, L, H, Hkv = 3001, 2, 10, 4, 2
+    print(f"case: mode attention of {bs} requests, page size {page}", flush=True)
+    g = torch.Generator().manual_seed(page)
+    KL, slots = K * L, 4096
+    lens = torch.randint(0, 200, (bs,), generator=g).cuda()
+    table = torch.randint(0, slots // page, (bs, -(-200 // page)), generator=g).int().cuda()
+    kc, vc = (torch.randn(slots, Hkv, D, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    q, kn, vn = (torch.randn(bs * KL, n, D, generator=g).to(torch.bfloat16).cuda() for n in (H, Hkv, Hkv))
+    rows = torch.arange(bs).cuda()
+    call = lambda a, b: paged_mode_attention.paged_mode_block_attention(  # noqa: E731
+        q=q[a * KL:b * KL], k_new=kn[a * KL:b * KL], v_new=vn[a * KL:b * KL], k_cache=kc, v_cache=vc, req_to_token=table,
+        req_pool_indices=rows[a:b], ctx_lens=lens[a:b], num_modes=K, block_size=L, scaling=D ** -0.5, num_ctx_splits=0,
+        page_size=page)
+    out = call(0, bs)
+    torch.cuda.synchronize()
+    for a in range(0, bs, 60):
+        b = min(a + 60, bs)
+        assert torch.equal(call(a, b).view(torch.int16), out[a * KL:b * KL].view(torch.int16))
