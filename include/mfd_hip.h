@@ -397,7 +397,8 @@ int mfd_mode_mask(const int64_t* prefix_lens, const int64_t* mask_offsets, uint8
  *                    int64). page_size 16, 32, 64, 128 or 256
  *   err_flag         optional; MFD_DEVERR_BAD_PAGE where a page id, row, length or count lies outside its bound. Nothing
  *                    out of bounds is read or written: a store skips such pages, reads take page 0 for such a page id and
- *                    no tokens for such a row, and lengths end where the table row ends.
+ *                    no tokens for such a row, lengths end where the table row ends, and counts are cut to what is there
+ *                    (also raised where `weights` has no row for a request, or a shorter one than its tokens need).
  *
  * mfd_kv8_store: new tokens of a batch. Request b's tokens are rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of k / v
  * (cu_tokens [bs + 1] int32 device, values up to N; row n, KV head g: k + n * kn_st + g * kn_sh, bf16) and go to the

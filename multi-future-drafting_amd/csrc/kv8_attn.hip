@@ -367,7 +367,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int ntiles = (hi - lo + TK - 1) / TK;
   const int last = ntiles - 1;
   if (tid == 0 && s == 0 && ug == 0 && kvh == 0) {
-    if (ctx != given_len) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+    if (ctx != given_len || !trow) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
     if (a.S > 1) a.ws_n[b] = parts;
   }
   if (a.S > 1 && ntiles == 0 && !with_block) {  // an empty split
@@ -786,7 +786,7 @@ __global__ __launch_bounds__(SNW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))
   split_range(s, parts, keys, ctx, lo, hi);
   const bool with_block = a.kn != nullptr && s == 0;
   if (tid == 0 && s == 0 && kvh == 0) {
-    if (ctx != a.ctx_lens[b]) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+    if (ctx != a.ctx_lens[b] || !trow) kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
     if (a.S > 1) a.ws_n[b] = parts;
   }
   if (lo >= hi && !with_block && a.S > 1) {  // an empty split
@@ -1177,7 +1177,7 @@ void kv8_weights_kernel(WArgs a) {
   const int64_t wrow = a.pages.req_idx ? a.pages.req_idx[b] : b;
   const int shift = a.pages.page_shift, pmask = (1 << shift) - 1;
   int ctx = trow && a.pages.num_pages > 0 && wrow < a.w_rows ? kv8::bounded_len(a.pages, a.ctx_lens[b]) : 0;
-  if (tid == 0 && range == 0 && kvh == 0 && (ctx > a.width || ctx != a.ctx_lens[b]))
+  if (tid == 0 && range == 0 && kvh == 0 && (ctx > a.width || ctx != a.ctx_lens[b] || !trow || wrow >= a.w_rows))
     kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   ctx = __builtin_amdgcn_readfirstlane(min(ctx, a.width));
   const int lo = range * WKEYS;

@@ -62,14 +62,17 @@ __global__ __launch_bounds__(NT) void kv8_store_kernel(StoreArgs a) {
   const int b = blockIdx.y, z = blockIdx.z;
   const int h = blockIdx.x % a.Hkv, pi = blockIdx.x / a.Hkv;
   const int shift = a.pages.page_shift, P = 1 << shift;
-  const int c0 = max(0, min(a.cu_tokens[b], a.N)), c1 = max(c0, min(a.cu_tokens[b + 1], a.N));
+  const int n0 = a.cu_tokens[b], n1 = a.cu_tokens[b + 1];
+  const int c0 = max(0, min(n0, a.N)), c1 = max(c0, min(n1, a.N));
   const int64_t start = max((int64_t)-1, min(a.start_lens[b], (int64_t)1 << 40));  // (beyond either: no table reaches there)
   const int64_t end = start + (c1 - c0);
+  const int32_t* row = kv8::table_row(a.pages, b);
+  if (blockIdx.x == 0 && z == 0 && threadIdx.x == 0 && (n0 < 0 || n1 < n0 || n1 > a.N || start < 0 || !row))
+    kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
   if (c1 == c0) return;
   const int64_t p = (start >> shift) + pi;
   const int64_t p0 = p << shift;
   if (p0 >= end) return;
-  const int32_t* row = kv8::table_row(a.pages, b);
   // tokens behind the last page of the grid (more of them than the call said) are not stored either
   const bool cut = pi == a.max_pages - 1 && p0 + P < end;
   int page = -1;
@@ -400,14 +403,20 @@ __global__ __launch_bounds__(NT) void evict_compact_kernel(CompactArgs a) {
   const int h = blockIdx.x % a.Hkv, p = blockIdx.x / a.Hkv;
   const int shift = a.dst.page_shift;
   const int n = (int)max((int64_t)0, min(a.new_lens[b], (int64_t)a.budget));
+  const int32_t *src_row = kv8::table_row(a.src, b), *dst_row = kv8::table_row(a.dst, b);
+  const int len = kv8::bounded_len(a.src, a.ctx_lens[b]);
   if (p == a.dst_pages) {
-    if (z == 0) move_weights(a, b, h, n);
+    if (z != 0) return;
+    if (h == 0 && threadIdx.x == 0) {  // what this request's workgroups cut, or leave out
+      const int64_t row = a.dst.req_idx ? a.dst.req_idx[b] : b;
+      if (n != a.new_lens[b] || len != a.ctx_lens[b] || !src_row || !dst_row || (a.w && (row >= a.w_rows || len > a.width)))
+        kv8::raise(a.err_flag, MFD_DEVERR_BAD_PAGE);
+    }
+    move_weights(a, b, h, n);
     return;
   }
   const int i0 = p << shift;
   if (i0 >= n) return;
-  const int32_t *src_row = kv8::table_row(a.src, b), *dst_row = kv8::table_row(a.dst, b);
-  const int len = kv8::bounded_len(a.src, a.ctx_lens[b]);
   int page = -1;
   if (src_row && dst_row && p < a.dst.table_width) page = dst_row[p];
   if (page < 0 || page >= a.dst.num_pages) {

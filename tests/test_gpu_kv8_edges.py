@@ -1,5 +1,6 @@
 """The 8-bit draft cache at the edges of what its calls allow: infinities beside very large and very small values in split
-contexts, batches of thousands. Tolerances: those of test_gpu_kv8, with what _bounded derives."""
+contexts, batches of thousands, counts and rows out of range. Tolerances: those of test_gpu_kv8, with what _bounded
+derives."""
 
 import numpy as np
 import pytest
@@ -7,7 +8,7 @@ import torch
 
 from oracle import kv8
 from test_gpu_kv8 import D, _gen, cache_args, check_attention, make_pool, oracle_attention, vals
-from test_gpu_kv8_use import FORMS, SCALE, _attend, _bf
+from test_gpu_kv8_use import FORMS, SCALE, _attend, _bf, _guarded
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +81,77 @@ def test_a_batch_of_thousands(K, L, H, splits):
     d["rows"], n = some, lens[some].tolist()
     ref = _bounded(oracle_attention(d, of(q), of(kn), of(vn), n, K, L, SCALE, False), d, n, KL, H // Hkv)
     check_attention(of(out), lse.cpu().view(bs, KL, H)[some].reshape(-1, H), ref)
+
+
+def test_counts_rows_and_lengths_out_of_range_are_reported():
+    """Whatever a call cuts to what its tensors hold, it says so in its error flag: the store's token counts and positions, the
+    compaction's counts, lengths and rows (of the table, and of the sums), and rows of requests that have nothing to do. The other
+    request's result keeps its bits, and nothing outside the tensors is written."""
+    import kv8_cache
+    import mfd_hip
+
+    page, Hkv, H, lens, budget = 64, 2, 4, [300, 200], 100
+    d = make_pool(lens, page, Hkv, seed=840, extra=2)
+    g = _gen(841)
+    k, v, q = _bf(g, 9, Hkv, D).cuda(), _bf(g, 9, Hkv, D).cuda(), _bf(g, 4, H, D).cuda()
+    table, dst = d["table"].cuda(), d["dst"].cuda()
+    keep = torch.stack([torch.arange(budget) * 2, torch.arange(budget)]).int().cuda()
+    i64 = lambda *x: torch.tensor(x).cuda()  # noqa: E731
+
+    def run(call, **kw):
+        """(the flag, request 0's pages, request 0's sums)"""
+        args, guards = {}, []
+        for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+            args[name], buf = _guarded(d[name])
+            guards.append(buf)
+        w, buf = _guarded(kw.pop("sums", torch.ones(3, Hkv, 300)))
+        guards.append(buf)
+        args.update(page_size=page, req_pool_indices=d["rows"].cuda(), err_flag=torch.zeros(1, dtype=torch.int32).cuda())
+        if call == "store":
+            args.update(k=k, v=v, page_table=table, start_lens=i64(290, 60), max_tokens=9,
+                        cu_tokens=torch.tensor([0, 3, 9], dtype=torch.int32).cuda())
+            kv8_cache.kv8_store(**{**args, **kw})
+        elif call == "compact":
+            args.update(keep=keep, new_lens=i64(budget, budget), ctx_lens=i64(*lens), src_table=table, dst_table=dst, weights=w)
+            kv8_cache.evict_compact_kv8(**{**args, **kw})
+        else:
+            args.update(q=q, page_table=table, ctx_lens=i64(*lens), num_modes=1, block_size=2, scaling=SCALE)
+            if call == "attn":
+                kv8_cache.paged_mode_block_attention_kv8(k_new=None, v_new=None, **{**args, **kw})
+            else:
+                del args["v_cache"], args["v_scale"]
+                kv8_cache.attention_weights_kv8(lse=torch.ones(4, H).cuda(), weights=w, **{**args, **kw})
+        torch.cuda.synchronize()
+        for buf in guards:
+            assert bool((buf[:4096] == 0x5A).all()) and bool((buf[-4096:] == 0x5A).all())
+        pages = torch.cat([t[d["rows"][0].item()].long() for t in (d["table"][:, :5], d["dst"])]).cuda()
+        caches = [args[x + "_cache"].view(torch.uint8).view(-1, page, Hkv, D)[pages] for x in "kv" if x + "_cache" in args]
+        return int(args["err_flag"]), caches, w[2].clone()
+
+    cu = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    r0 = int(d["rows"][0])
+    rows = [i64(r0, r) for r in (-1, 3, 2 ** 40)]
+    bad = {
+        "store": [dict(cu_tokens=cu(0, 3, 10)), dict(cu_tokens=cu(0, 3, 2 ** 31 - 1)), dict(cu_tokens=cu(0, 3, 2)),
+                  dict(cu_tokens=cu(0, 3, -5)), dict(start_lens=i64(290, -1), cu_tokens=cu(0, 3, 3)),
+                  *(dict(req_pool_indices=r, cu_tokens=cu(0, 3, 3)) for r in rows)],
+        "compact": [*(dict(new_lens=i64(budget, n)) for n in (-1, budget + 1, 2 ** 62, -2 ** 62)),
+                    *(dict(ctx_lens=i64(300, n)) for n in (-1, 10 ** 6, 2 ** 62, -2 ** 62)),
+                    *(dict(req_pool_indices=r, new_lens=i64(budget, 0)) for r in rows),
+                    *(dict(req_pool_indices=r, new_lens=i64(budget, 0), ctx_lens=i64(300, 0), weights=None) for r in rows)],
+        "attn": [dict(req_pool_indices=r, ctx_lens=i64(300, 0)) for r in rows],
+        "weights": [dict(req_pool_indices=r, ctx_lens=i64(300, 0)) for r in rows],
+    }
+    for call, changes in bad.items():
+        flag, caches, sums = run(call)
+        assert flag == 0
+        for change in changes:
+            print(f"case: kv8 {call} out of range", {x: t if t is None else t.tolist() for x, t in change.items()}, flush=True)
+            f, c, s = run(call, **change)
+            assert f == mfd_hip.DEVERR_BAD_PAGE
+            assert all(torch.equal(x, y) for x, y in zip(caches, c))
+            assert "weights" in change or torch.equal(s, sums)
+    # sums with fewer rows, or narrower ones, than the requests have
+    assert run("compact", sums=torch.ones(3, Hkv, 299))[0] == mfd_hip.DEVERR_BAD_PAGE
+    few = torch.ones(2, Hkv, 300).cuda()  # (request 0 is in row 2)
+    assert run("compact", weights=few)[0] == mfd_hip.DEVERR_BAD_PAGE
