@@ -154,9 +154,10 @@ def kv8_store(*, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
 # ------------------------------------------------------------------------------------------------------- attention
 
 
-def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int, device) -> tuple[int, int]:
-    """(num_ctx_splits, split_keys) for num_ctx_splits < 0, from what the kernels' workgroup slots hold (two workgroups per CU,
-    one of eight waves) and the programs (request, KV head, group of units) that there are without a split.
+def _auto_count(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int, device) -> tuple[int, bool]:
+    """For num_ctx_splits < 0: the most splits of a request, growing with max_ctx, and whether they are parts of max_ctx. From
+    what the kernels' workgroup slots hold (two workgroups per CU, one of eight waves) and the programs (request, KV head, group
+    of units) that there are without a split.
 
     A single request's splits fill one round of slots, less the block partial's. A batch's (up to 64 requests) are measured out
     on the device (keys 0), as long as makes all of them together fill the rounds whatever the lengths: 4 requests of 700 ..
@@ -180,20 +181,24 @@ def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int,
     else:
         short = 5120 * programs // slots - 1024 if 3 * programs > slots else 1536 * programs // slots
     if programs >= slots or max_ctx <= short:
-        return 1, 0
+        return 1, True
     least = 128 if units == 1 else 192
     if bs == 1 or bs > 64 or units == 1 and 8 * programs < slots:
         splits = slots // programs - (1 if with_block and units > 1 else 0)
         if units == 1 and bs > 1:
             splits = min(3 * slots // programs, max(cus // programs, max_ctx // 2048))
-        splits = min(splits, -(-max_ctx // least), 32 if units == 1 else 64)
-        return _splits_of(splits, max_ctx) if splits > 1 else (1, 0)
+        return max(1, min(splits, -(-max_ctx // least), 32 if units == 1 else 64)), True
     # the pairs (request, partial) that mfd_kv8_attn deals out; one request's splits at most what the others leave
     extra = 1 if with_block and units > 1 else 0
     per, need = programs // bs, bs * (2 + extra)
     pairs = max(need, -(-need * per // slots) * slots // per)
-    splits = min(pairs - extra * bs - bs + 1, -(-max_ctx // least), 32 if units == 1 else 16)
-    return (splits, 0) if splits > 1 else (1, 0)
+    return max(1, min(pairs - extra * bs - bs + 1, -(-max_ctx // least), 32 if units == 1 else 16)), False
+
+
+def _auto_splits(bs: int, heads: int, rows: int, with_block: bool, max_ctx: int, device) -> tuple[int, int]:
+    """(num_ctx_splits, split_keys) for num_ctx_splits < 0; split_keys 0: measured out on the device."""
+    splits, parts = _auto_count(bs, heads, rows, with_block, max_ctx, device)
+    return _splits_of(splits, max_ctx) if parts and splits > 1 else (splits, 0)
 
 
 def _splits_of(splits: int, max_ctx: int) -> tuple[int, int]:
@@ -284,15 +289,16 @@ def paged_mode_block_attention_kv8(
 
 def workspace_bytes(*, bs: int, num_modes: int, block_size: int, num_heads: int, num_kv_heads: int, with_block: bool,
                     max_ctx: int, num_ctx_splits: int = -1, device=None) -> int:
-    """Bytes of paged_mode_block_attention_kv8's workspace for these sizes (its ``max_ctx`` the same)."""
+    """Bytes of paged_mode_block_attention_kv8's workspace for these sizes, enough for every call whose ``max_ctx`` (or what its
+    page table's rows hold, where that is less or none is given) is at most this one. (Parts are whole tiles, so a longer context
+    can have fewer of them: what counts is how many were asked for, which only grows.)"""
+    max_ctx = max(1, max_ctx)
     if num_ctx_splits < 0:
         device = torch.device("cuda") if device is None else torch.device(device)
-        splits, _ = _auto_splits(bs, num_kv_heads, num_heads // num_kv_heads * num_modes * block_size, with_block,
-                                 max(1, max_ctx), device)
+        splits, _ = _auto_count(bs, num_kv_heads, num_heads // num_kv_heads * num_modes * block_size, with_block, max_ctx, device)
     else:
-        splits = _splits_of(num_ctx_splits, max(1, max_ctx))[0] if num_ctx_splits > 1 else 1
-    return mfd_hip.lib().mfd_kv8_attn_workspace_bytes(bs, num_modes, block_size, num_heads, num_kv_heads, with_block,
-                                                      splits)
+        splits = min(num_ctx_splits, -(-max_ctx // TILE_KEYS))
+    return mfd_hip.lib().mfd_kv8_attn_workspace_bytes(bs, num_modes, block_size, num_heads, num_kv_heads, with_block, splits)
 
 
 def decode(cache: torch.Tensor, scale: torch.Tensor, page_size: int) -> torch.Tensor:

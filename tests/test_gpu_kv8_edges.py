@@ -155,3 +155,27 @@ def test_counts_rows_and_lengths_out_of_range_are_reported():
     assert run("compact", sums=torch.ones(3, Hkv, 299))[0] == mfd_hip.DEVERR_BAD_PAGE
     few = torch.ones(2, Hkv, 300).cuda()  # (request 0 is in row 2)
     assert run("compact", weights=few)[0] == mfd_hip.DEVERR_BAD_PAGE
+
+
+@pytest.mark.parametrize("K,L,splits", [(1, 1, -1), (8, 16, -1), (8, 16, 32)])
+def test_one_workspace_for_many_lengths(K, L, splits):
+    """A buffer sized once, for one token more than the table's rows hold, serves calls without max_ctx and with smaller ones."""
+    import kv8_cache
+
+    page, Hkv, H = 64, 8, 32
+    table_reach = 2048 if K == 1 else 16128
+    print(f"case: kv8 workspace {K} x {L} splits={splits}", flush=True)
+    d = make_pool([table_reach], page, Hkv, seed=850)
+    g = _gen(851)
+    T = K * L
+    q, kn, vn = _bf(g, T, H, D).cuda(), _bf(g, T, Hkv, D).cuda(), _bf(g, T, Hkv, D).cuda()
+    size = kv8_cache.workspace_bytes(bs=1, num_modes=K, block_size=L, num_heads=H, num_kv_heads=Hkv, with_block=True,
+                                     max_ctx=table_reach + 1, num_ctx_splits=splits)
+    ws = torch.full((size + 64,), 0x5A, dtype=torch.uint8, device="cuda")
+    args = cache_args(d)
+    for n, most in ((table_reach, None), (table_reach, table_reach), (2047, 2048), (1000, 1900), (500, 2881), (0, 1)):
+        d["lens"][0] = n
+        o0, l0 = _attend(d, args, q, kn, vn, K, L, num_ctx_splits=splits, max_ctx=most)
+        o1, l1 = _attend(d, args, q, kn, vn, K, L, num_ctx_splits=splits, max_ctx=most, workspace=ws[:size])
+        assert torch.equal(o0.view(torch.int16), o1.view(torch.int16)) and torch.equal(l0, l1)
+    assert bool((ws[size:] == 0x5A).all())
