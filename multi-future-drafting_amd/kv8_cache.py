@@ -293,6 +293,8 @@ def workspace_bytes(*, bs: int, num_modes: int, block_size: int, num_heads: int,
     page table's rows hold, where that is less or none is given) is at most this one. (Parts are whole tiles, so a longer context
     can have fewer of them: what counts is how many were asked for, which only grows.)"""
     max_ctx = max(1, max_ctx)
+    if bs < 1:
+        return 0
     if num_ctx_splits < 0:
         device = torch.device("cuda") if device is None else torch.device(device)
         splits, _ = _auto_count(bs, num_kv_heads, num_heads // num_kv_heads * num_modes * block_size, with_block, max_ctx, device)

@@ -25,3 +25,11 @@ def test_a_workspace_serves_every_shorter_context(monkeypatch, bs, heads, group,
         need = mfd_hip.lib().mfd_kv8_attn_workspace_bytes(bs, modes, block, heads * group, heads, 1, count)
         largest = max(largest, need)
         assert kv8_cache.workspace_bytes(max_ctx=n, num_ctx_splits=splits, device="cuda:0", **sizes) >= largest, n
+
+
+def test_a_workspace_for_no_requests(monkeypatch):
+    monkeypatch.setattr(mfd_hip, "cu_count", lambda device: 256)
+    for modes, block in ((1, 1), (8, 16)):
+        for splits in (-1, 0, 4):
+            assert kv8_cache.workspace_bytes(bs=0, num_modes=modes, block_size=block, num_heads=32, num_kv_heads=8,
+                                             with_block=True, max_ctx=4096, num_ctx_splits=splits, device="cuda:0") == 0
