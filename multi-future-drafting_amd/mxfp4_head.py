@@ -99,21 +99,23 @@ def draft_head_mxfp4(x: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor,
     if device < 0 or codes.get_device() != device or exps.get_device() != device or (
             out is not None and out.get_device() != device):
         raise ValueError(f"MFD kernels take GPU tensors of one device (x on {x.device}, codes on {codes.device})")
+    # (one row has no stride: that of the tensor it was cut from says nothing)
     rows, stride = x.shape[0], x.stride()
-    if stride[1] != 1 or stride[0] % 8 or x.data_ptr() % 16:
+    step = stride[0] if rows > 1 else hidden
+    if stride[1] != 1 or step % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-        stride = x.stride()
+        step = hidden
     if out is None:
         out = x.new_empty((rows, (vocab + 7) // 8 * 8))
         pitch = out.stride(0)
         if out.shape[1] != vocab:
             out = out[:, :vocab]
     else:
-        pitch = out.stride(0)
+        pitch = out.stride(0) if rows > 1 else (vocab + 7) // 8 * 8
         if out.dtype is not torch.bfloat16 or tuple(out.shape) != (rows, vocab) or (vocab > 1 and out.stride(1) != 1):
             raise ValueError(f"out must be bfloat16 [{rows}, {vocab}] with contiguous rows")
-    mfd_hip.call_on(device, "mfd_draft_head_mxfp4", x.data_ptr(), stride[0], rows or 1, 0, codes.data_ptr(),
+    mfd_hip.call_on(device, "mfd_draft_head_mxfp4", x.data_ptr(), step, rows or 1, 0, codes.data_ptr(),
                     exps.data_ptr(), rows, vocab, hidden, out.data_ptr(), pitch)
     return out
