@@ -362,6 +362,8 @@ int head_gemm(const uint16_t* x, int64_t row_stride, int rows_per_group, int64_t
   if (M < 0 || N < 1 || K < 1 || rows_per_group < 1 || row_stride < 0 || group_stride < 0)
     return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: bad sizes M=%d N=%d K=%d rows_per_group=%d", who, M, N, K, rows_per_group);
   if (K % KS != 0) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: needs K %% %d == 0 (K=%d)", who, KS, K);
+  // a workgroup's share of the weight, up to 672 rows of K / 2 bytes with its last tile's padding, has 32-bit offsets
+  if (K > (1 << 23)) return mfd_set_error(MFD_ERR_UNSUPPORTED, "%s: hidden size %d above 2^23", who, K);
   if (M == 0) return MFD_OK;
   if (!x || !codes || !exps || !out) return mfd_set_error(MFD_ERR_INVALID_ARG, "%s: null pointer", who);
   if (row_stride % 8 != 0 || group_stride % 8 != 0 || out_stride < N || out_stride % 4 != 0 ||

@@ -33,3 +33,12 @@ def test_a_workspace_for_no_requests(monkeypatch):
         for splits in (-1, 0, 4):
             assert kv8_cache.workspace_bytes(bs=0, num_modes=modes, block_size=block, num_heads=32, num_kv_heads=8,
                                              with_block=True, max_ctx=4096, num_ctx_splits=splits, device="cuda:0") == 0
+
+
+def test_a_hidden_size_beyond_32_bit_offsets_is_refused():
+    """The wide form addresses a workgroup's share of the weight, up to 672 rows of hidden / 2 bytes, by 32-bit offsets."""
+    P, U8 = 1 << 20, 1 << 23  # (no pointer gets as far as being used)
+    call = lambda K: mfd_hip.lib().mfd_draft_head_mxfp4(P, K, 1, K, P, P, 1, 100000, K, P, 100000, None)  # noqa: E731
+    assert 672 * U8 // 2 < 2 ** 32 < 672 * 2 * U8 // 2
+    for K in (U8 + 128, 2 * U8, 2 ** 31 - 128):
+        assert call(K) == -2 and b"hidden" in mfd_hip.lib().mfd_last_error()
