@@ -184,8 +184,10 @@ class PagedModeAttention:
                 v_cache=kv8_cache.decode(v_cache, v_scale, self.page_size), req_to_token=self.req_to_token,
                 **common).to(q.dtype)
         else:
-            lens = getattr(forward_batch, "seq_lens_cpu", None)  # only tunes the context splits
-            common["max_ctx"] = int(lens[:bs].max()) if lens is not None and bs else None
+            # only tunes the context splits; a graph is replayed with other lengths than those it is captured with
+            lens = getattr(forward_batch, "seq_lens_cpu", None)
+            known = lens is not None and bs and not (q.is_cuda and torch.cuda.is_current_stream_capturing())
+            common["max_ctx"] = int(lens[:bs].max()) if known else None
             o = kv8_cache.paged_mode_block_attention_kv8(k_cache=k_cache, v_cache=v_cache, k_scale=k_scale,
                                                          v_scale=v_scale, page_table=self.req_to_token,
                                                          num_ctx_splits=self.num_ctx_splits, **common)

@@ -179,3 +179,42 @@ def test_one_workspace_for_many_lengths(K, L, splits):
         o1, l1 = _attend(d, args, q, kn, vn, K, L, num_ctx_splits=splits, max_ctx=most, workspace=ws[:size])
         assert torch.equal(o0.view(torch.int16), o1.view(torch.int16)) and torch.equal(l0, l1)
     assert bool((ws[size:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("K,L,H", [(1, 1, 8), (4, 16, 8)])
+def test_a_captured_hook_splits_for_the_table(monkeypatch, K, L, H):
+    """PagedModeAttention captured with the lengths of an empty batch (as engines capture it), replayed with others: the splits
+    are those of what the table holds, not of the lengths at capture, and the results an eager call's."""
+    import kv8_cache
+    import paged_mode_attention
+
+    page, Hkv, bs = 64, 2, 3
+    d = make_pool([1500, 700, 1100], page, Hkv, seed=860)
+    g = _gen(861)
+    T, args = bs * K * L, cache_args(d)
+    q, k, v = (_bf(g, T, n * D).cuda() for n in (H, Hkv, Hkv))
+    pool = kv8_cache.Kv8Pool(num_layers=1, num_pages=d["k_scale"].shape[0], page_size=page, num_kv_heads=Hkv)
+    pool.caches, pool.scales = [(args["k_cache"], args["v_cache"])], [(args["k_scale"], args["v_scale"])]
+    lens = torch.ones(bs, dtype=torch.int64).cuda()
+    batch = type("Batch", (), dict(req_pool_indices=d["rows"].cuda(), seq_lens=lens,
+                                   seq_lens_cpu=torch.ones(bs, dtype=torch.int64)))
+    hook = paged_mode_attention.PagedModeAttention(
+        kv_pool=pool, req_to_token=d["table"].cuda(), num_modes=K, block_size=L, num_heads=H, num_kv_heads=Hkv, head_dim=D,
+        scaling=SCALE, num_ctx_splits=-1, impl="hip", page_size=page)
+    given, attention = [], kv8_cache.paged_mode_block_attention_kv8
+    monkeypatch.setattr(kv8_cache, "paged_mode_block_attention_kv8",
+                        lambda **kw: given.append(kw["max_ctx"]) or attention(**kw))
+    hook(q, k, v, batch, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hook(q, k, v, batch, 0)
+    assert given == [1, None]
+    for now in ([1500, 700, 1100], [0, 64, 1], [1499, 0, 1100], [3, 3, 3]):
+        lens.copy_(torch.tensor(now))
+        batch.seq_lens_cpu = None
+        eager = hook(q, k, v, batch, 0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
