@@ -1,14 +1,14 @@
 """The 8-bit draft cache at the edges of what its calls allow: infinities beside very large and very small values in split
-contexts, batches of thousands, counts and rows out of range. Tolerances: those of test_gpu_kv8, with what _bounded
-derives."""
+contexts, batches of thousands, counts and rows out of range, one workspace for many lengths, captured hooks, side streams.
+Tolerances: those of test_gpu_kv8, with what _bounded derives."""
 
 import numpy as np
 import pytest
 import torch
 
 from oracle import kv8
-from test_gpu_kv8 import D, _gen, cache_args, check_attention, make_pool, oracle_attention, vals
-from test_gpu_kv8_use import FORMS, SCALE, _attend, _bf, _guarded
+from test_gpu_kv8 import D, F8, _gen, cache_args, check_attention, make_pool, oracle_attention, vals
+from test_gpu_kv8_use import FORMS, SCALE, _attend, _bf, _guarded, _Step
 
 pytestmark = pytest.mark.gpu
 
@@ -218,3 +218,105 @@ def test_a_captured_hook_splits_for_the_table(monkeypatch, K, L, H):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+
+
+def _operators():
+    """{name: (inputs by name, what the call changes or returns, the call)} on one round's static buffers. Every input is one that
+    is in range under both of its values below."""
+    import ddtree_sglang_ops
+    import kv8_cache
+    import mxfp4_head
+    import paged_mode_attention
+
+    s = _Step(870)
+    a = s.args
+    cache = {x: a[x] for x in ("k_cache", "v_cache", "k_scale", "v_scale")}
+    index = dict(page_size=s.page, req_pool_indices=a["req_pool_indices"])
+    sizes = dict(num_modes=s.K, block_size=s.L, scaling=SCALE, page_table=s.table, ctx_lens=s.ctx)
+    rows = s.out.view(-1, s.H * D)
+    s.out.copy_(s.q)
+    s.lse.fill_(6.0)
+    s.w.copy_(torch.rand(s.w.shape, generator=_gen(871)))
+    s.keep.copy_(torch.arange(100) * 3 % 300)
+    s.keep.copy_(s.keep.sort(1).values.clamp(max=128))
+    s.new.fill_(100)
+    pool = kv8_cache.Kv8Pool(num_layers=1, num_pages=a["k_scale"].shape[0], page_size=s.page, num_kv_heads=s.Hkv)
+    pool.caches, pool.scales = [(a["k_cache"], a["v_cache"])], [(a["k_scale"], a["v_scale"])]
+    batch = type("Batch", (), dict(req_pool_indices=a["req_pool_indices"].int(), seq_lens=s.ctx.int()))
+    hook = paged_mode_attention.PagedModeAttention(
+        kv_pool=pool, req_to_token=s.table, num_modes=s.K, block_size=s.L, num_heads=s.H, num_kv_heads=s.Hkv, head_dim=D,
+        scaling=SCALE, num_ctx_splits=3, impl="hip", page_size=s.page)
+    head = ddtree_sglang_ops.DDTreeDraftTopK(weight=mxfp4_head.Mxfp4Weight(s.codes, s.exps), block_size=s.L, num_modes=s.K,
+                                             budget=17, max_bs=2)
+    flat = lambda t: t.view(t.shape[0], -1)  # noqa: E731
+    qkv = dict(q=s.q, kn=s.kn, vn=s.vn)
+    return {
+        "attention": (dict(qkv, **cache), (s.out, s.lse), lambda: kv8_cache.paged_mode_block_attention_kv8(
+            q=s.q, k_new=s.kn, v_new=s.vn, out=s.out, lse_out=s.lse, num_ctx_splits=3, **cache, **index, **sizes)),
+        "hook": (dict(qkv, **cache), (), lambda: hook(flat(s.q), flat(s.kn), flat(s.vn), batch, 0)),
+        "weights": (dict(q=s.q, lse=s.lse, w=s.w, k_cache=a["k_cache"], k_scale=a["k_scale"]), (s.w,),
+                    lambda: kv8_cache.attention_weights_kv8(q=s.q, lse=s.lse, weights=s.w, decay=0.9, k_cache=a["k_cache"],
+                                                            k_scale=a["k_scale"], **index, **sizes)),
+        "store": (dict(kn=s.kn, vn=s.vn, **cache), tuple(cache.values()), lambda: kv8_cache.kv8_store(
+            k=s.kn[:9], v=s.vn[:9], page_table=s.table, start_lens=s.ctx.int(), cu_tokens=s.cu, max_tokens=5, **cache, **index)),
+        "select": (dict(w=s.w), (), lambda: torch.cat([t.flatten().long() for t in kv8_cache.evict_select(
+            weights=s.w, req_pool_indices=a["req_pool_indices"], ctx_lens=s.ctx, budget=100)])),
+        "select, narrow rows": (dict(w=s.w), (), lambda: kv8_cache.evict_select(
+            weights=s.w[:, :, :300], req_pool_indices=a["req_pool_indices"].int(), ctx_lens=s.ctx, budget=100)[0]),
+        "compact": (dict(keep=s.keep, w=s.w, **cache), (s.w, *cache.values()), lambda: kv8_cache.evict_compact_kv8(
+            keep=s.keep, new_lens=s.new, ctx_lens=s.ctx, src_table=s.table, dst_table=s.dst, weights=s.w, **cache, **index)),
+        "evict": (dict(w=s.w, **cache), (s.w, *cache.values()), lambda: pool.evict(
+            weights=s.w, page_table=s.table, dst_table=s.dst, req_pool_indices=a["req_pool_indices"], ctx_lens=s.ctx,
+            budget=100)[0]),
+        "head": (dict(x=s.out), (), lambda: mxfp4_head.draft_head_mxfp4(rows, s.codes, s.exps)),
+        "head of an unaligned view": (dict(x=s.out), (), lambda: mxfp4_head.draft_head_mxfp4(
+            rows.view(-1)[1:-(s.H * D) + 1].view(-1, s.H * D), s.codes, s.exps)),
+        "candidates": (dict(x=s.out), (head.top_logp, head.top_ids, head.log_z), lambda: head(rows)),
+    }
+
+
+NAMES = ["attention", "hook", "weights", "store", "select", "select, narrow rows", "compact", "evict", "head",
+         "head of an unaligned view", "candidates"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_each_operator_runs_on_the_current_stream(name):
+    """An operator on a side stream behind a long wait and the copies that bring its inputs: a launch on any other stream would
+    read what the inputs held before, which gives another result (the first assertion)."""
+    print(f"case: side stream, {name}", flush=True)
+    inputs, changed, call = _operators()[name]
+    true = {k: t.clone() for k, t in inputs.items()}
+
+    def other(k, t):
+        if k == "keep":
+            return (t + 1).clamp(max=128)
+        return t.view(torch.uint8).flip(0).view(t.dtype) if t.dtype == F8 else t.flip(0)
+
+    false = {k: other(k, t) for k, t in true.items()}
+
+    def run():
+        res = call()
+        return [t.clone().view(torch.uint8) for t in (*changed, *([res] if torch.is_tensor(res) else []))]
+
+    def put(values):
+        for k, t in inputs.items():
+            t.view(torch.uint8).copy_(values[k].view(torch.uint8))
+
+    put(false)
+    wrong = run()
+    put(true)
+    right = run()
+    put(false)
+    for t in changed:
+        if not any(t is x for x in inputs.values()):
+            t.zero_()
+    torch.cuda.synchronize()
+    assert any(not torch.equal(x, y) for x, y in zip(wrong, right))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        put(true)
+        got = run()
+    assert not side.query()  # (it still waits: nothing above has begun)
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(right, got))
