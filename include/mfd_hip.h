@@ -476,7 +476,7 @@ int mfd_evict_compact_kv8(const int32_t* keep, int budget, const int64_t* new_le
 /* ---------------------------------------------------------------- draft head with a 4-bit weight
  * mfd_draft_head_gemm / mfd_draft_topk_head with the weight in the OCP microscaling format MXFP4:
  *   W[n][k] = e2m1(half k % 2 (low first) of codes[n][k / 2]) * 2^(exps[n][k / 32] - 127)
- *   codes [N][K / 2] uint8, 16-byte aligned;  exps [N][K / 32] uint8, 4-byte aligned, values 1 .. 252;
+ *   codes [N][K / 2] uint8, 16-byte aligned;  exps [N][K / 32] uint8, 4-byte aligned, values 0 .. 252;
  *   K % 128 == 0, up to 2^23
  * The other arguments are as there (drafted row m at x + (m / rows_per_group) * group_stride + (m % rows_per_group) *
  * row_stride; out_stride a multiple of 4). Products are exact, sums fp32, logits rounded once to bf16. */

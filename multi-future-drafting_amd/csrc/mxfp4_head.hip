@@ -84,7 +84,7 @@ __device__ __forceinline__ bf16x8 widen(uint32_t c, float s) {
                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3)};
   return __builtin_bit_cast(bf16x8, v);
 }
-// The scale of lane group g4 among a step's four
+// The scale of lane group g4 among a step's four (the conversion reads the float's exponent alone: 0 is 2^-127, as in the format)
 __device__ __forceinline__ float scale_of(uint32_t e4, int g4) { return __uint_as_float(((e4 >> (8 * g4)) & 0xffu) << 23); }
 
 // C registers of a tile pair to bf16 and out: weight rows n .. n + 3 of the range, the drafted row's output at orow

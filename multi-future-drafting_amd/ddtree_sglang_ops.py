@@ -222,7 +222,7 @@ class DDTreeDraftTopK:
         self.mxfp4 = isinstance(weight, mxfp4_head.Mxfp4Weight)
         vocab, hidden = weight.shape
         if self.mxfp4:
-            mxfp4_head.check_weight(weight.codes, weight.exps, values=True)
+            mxfp4_head.check_weight(weight.codes, weight.exps, values=True, ready_made=True)
             mfd_hip.require_cuda(weight.codes, weight.exps, vocab_ids)
         else:
             mfd_hip.require_cuda(weight, vocab_ids)

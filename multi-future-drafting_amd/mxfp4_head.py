@@ -3,8 +3,9 @@
 The weight is in the OCP microscaling format MXFP4: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a
 byte, low half first, and a power-of-two scale 2^(e - 127) for 32 weights of a row:
   codes  uint8 [vocab, hidden / 2],  exps  uint8 [vocab, hidden / 32],  hidden a multiple of 128.
-e is 1 .. 252: from 253 on 6 * 2^(e - 127) is infinite in bf16, and 0 (in the format 2^-127) and 255 (NaN) are no scales
-of a weight here. check_weight(values=True) refuses them; a call does not look at the values.
+quantize writes e of 1 .. 252: from 253 on 6 * 2^(e - 127) is infinite in bf16, and 255 is NaN. check_weight(values=True)
+holds a weight to that, with ``ready_made`` also allowing 0, the format's 2^-127, which ready-made weights give their groups of
+zeros (products with it are exact too). A call does not look at the values.
 The product is exact in float32 (bf16 hidden states times such weights) and summed there; a logit is rounded once to bf16.
 """
 
@@ -36,7 +37,7 @@ class Mxfp4Weight(NamedTuple):
         return self.codes.shape[0], self.codes.shape[1] * 2
 
 
-def check_weight(codes: torch.Tensor, exps: torch.Tensor, values: bool = False) -> None:
+def check_weight(codes: torch.Tensor, exps: torch.Tensor, values: bool = False, ready_made: bool = False) -> None:
     """The layout above, and with ``values`` (which waits for the device) the range of the scales; ValueError otherwise."""
     shape = codes.shape
     if codes.dtype is not torch.uint8 or exps.dtype is not torch.uint8 or len(shape) != 2 or \
@@ -46,8 +47,9 @@ def check_weight(codes: torch.Tensor, exps: torch.Tensor, values: bool = False) 
         raise ValueError(f"codes must be contiguous uint8 [vocab, hidden / 2] with hidden % 128 == 0 and exps contiguous "
                          f"uint8 [vocab, hidden / {GROUP}] on the same device, got {codes.dtype} {tuple(codes.shape)} and "
                          f"{exps.dtype} {tuple(exps.shape)}")
-    if values and bool(((exps < 1) | (exps > MAX_EXP)).any()):
-        raise ValueError(f"scale exponents must be 1 .. {MAX_EXP}")
+    least = 0 if ready_made else 1
+    if values and bool(((exps < least) | (exps > MAX_EXP)).any()):
+        raise ValueError(f"scale exponents must be {least} .. {MAX_EXP}")
 
 
 def quantize(weight: torch.Tensor, rows_at_once: int = 16384) -> Mxfp4Weight:

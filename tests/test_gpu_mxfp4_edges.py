@@ -1,5 +1,5 @@
-"""The 4-bit draft head at the edges of what its call allows: one row of a tensor with odd strides, and hidden sizes of several
-blocks of drafted rows. Tolerance: test_gpu_mxfp4's."""
+"""The 4-bit draft head at the edges of what its call allows: one row of a tensor with odd strides, hidden sizes of several
+blocks of drafted rows, exponent 0. Tolerance: test_gpu_mxfp4's."""
 
 import pytest
 import torch
@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 
 
 def test_one_row_has_no_stride():
-    """Slices of one row, whose stride is that of the tensor they come from and means nothing: as x, and as the result's buffer."""
+    """Slices of one row, whose stride is that of the tensor they come from and means nothing: as x, and as the
+    result's buffer."""
     import mxfp4_head
 
     codes, exps = _weight(3001, 128, seed=7)
@@ -55,3 +56,51 @@ def test_blocks_of_drafted_rows(rows, vocab, hidden):
         ref, mass = xd @ w.t(), xd.abs() @ w.abs().t()
         bound = (2.0 ** -8 * ref.abs() + hidden * 2.0 ** -24 * mass) * (1 + 2.0 ** -8)
         assert bool(((got[:, part].double() - ref).abs() <= bound).all()), lo
+
+
+def _ready_made():
+    """A weight as ready-made files have it: groups of zeros under exponent 0 (2^-127), and one group of codes under it."""
+    codes, exps = _weight(20001, 256, seed=11)
+    codes[5:500:7, 16:32] = 0
+    exps[5:500:7, 1] = 0
+    codes[9, 32:48], exps[9, 2] = torch.arange(16, 32, dtype=torch.uint8), 0
+    return codes, exps
+
+
+def test_exponent_zero():
+    """2^-127 under each code, met by a single one and by 2^100: exact, the subnormal values too; and a weight with
+    such groups."""
+    import mxfp4_head
+
+    for vocab in (252, 20000):  # k-split and wide form
+        codes = torch.arange(256, dtype=torch.uint8)[torch.arange(vocab * 64) % 256].view(vocab, 64).contiguous()
+        exps = torch.zeros(vocab, 4, dtype=torch.uint8)
+        pair = torch.stack([codes & 15, codes >> 4], dim=-1).view(vocab, 128).int()
+        ref = torch.tensor(mxfp4_head.E2M1 + tuple(-v for v in mxfp4_head.E2M1), dtype=torch.float64)[pair].t() * 2.0 ** -127
+        assert torch.equal(mxfp4_head.dequantize(mxfp4_head.Mxfp4Weight(codes, exps)).double().t(), ref)
+        for size in (1.0, 2.0 ** 100):
+            x = (torch.eye(128) * size).to(torch.bfloat16)
+            got = mxfp4_head.draft_head_mxfp4(x.cuda(), codes.cuda(), exps.cuda())
+            assert torch.equal(got.cpu().double(), ref * size)
+    codes, exps = _ready_made()
+    x = torch.randn(20, 256, generator=torch.Generator().manual_seed(12)).to(torch.bfloat16)
+    _check(mxfp4_head.draft_head_mxfp4(x.cuda(), codes.cuda(), exps.cuda()), x, codes, exps)
+
+
+def test_candidates_from_a_ready_made_weight():
+    """DDTreeDraftTopK takes such a weight as it is."""
+    import ddtree_sglang_ops
+    import mxfp4_head
+
+    codes, exps = (t.cuda() for t in _ready_made())
+    head = ddtree_sglang_ops.DDTreeDraftTopK(weight=mxfp4_head.Mxfp4Weight(codes, exps), block_size=8, num_modes=2, budget=17,
+                                             max_bs=1)
+    x = torch.randn(16, 256, generator=torch.Generator().manual_seed(13)).to(torch.bfloat16).cuda()
+    head(x)
+    logits = mxfp4_head.draft_head_mxfp4(x.view(2, 8, 256)[:, 1:].reshape(14, 256), codes, exps)
+    assert torch.equal(head.logits[:14].view(torch.int16), logits.view(torch.int16))
+    for e in (253, 255):
+        exps[3, 1] = e
+        with pytest.raises(ValueError, match="exponents"):
+            ddtree_sglang_ops.DDTreeDraftTopK(weight=mxfp4_head.Mxfp4Weight(codes, exps), block_size=8, num_modes=2, budget=17,
+                                              max_bs=1)
