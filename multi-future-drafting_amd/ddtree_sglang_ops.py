@@ -259,7 +259,9 @@ class DDTreeDraftTopK:
         if H != self.weight.shape[1] or hidden_states.shape[0] % L:
             raise ValueError(f"hidden_states must be [blocks * {L}, {self.weight.shape[1]}], got "
                              f"{tuple(hidden_states.shape)}")
-        x = hidden_states
+        x, device = hidden_states, hidden_states.get_device()
+        if device < 0 or device != self._logits.get_device():
+            raise ValueError(f"hidden_states on {x.device}, the head on {self._logits.device}: not the same GPU device")
         if x.dtype != torch.bfloat16 or x.stride(-1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
             x = x.to(torch.bfloat16).contiguous()
         n = (x.shape[0] // L) * (L - 1)
@@ -267,11 +269,10 @@ class DDTreeDraftTopK:
             raise ValueError(f"{n} drafted rows exceed the {self.logits.shape[0]} of max_bs={self.max_bs}")
         rs = x.stride(0)
         weight = (self.weight.codes.data_ptr(), self.weight.exps.data_ptr()) if self.mxfp4 else (self.weight.data_ptr(),)
-        mfd_hip.call("mfd_draft_topk_head_mxfp4" if self.mxfp4 else "mfd_draft_topk_head", x.data_ptr() + rs * 2, rs, L - 1,
-                     L * rs, *weight, n, self.vocab, H, self._logits.data_ptr(), self._logits.stride(0), self.topk,
-                     self.top_logp.data_ptr(), self.top_ids.data_ptr(), 0, self.log_z.data_ptr(),
-                     mfd_hip.ptr(self.vocab_ids), self.workspace.data_ptr(), self.workspace.numel(),
-                     mfd_hip.stream_of(x))
+        mfd_hip.call_on(device, "mfd_draft_topk_head_mxfp4" if self.mxfp4 else "mfd_draft_topk_head", x.data_ptr() + rs * 2, rs,
+                        L - 1, L * rs, *weight, n, self.vocab, H, self._logits.data_ptr(), self._logits.stride(0), self.topk,
+                        self.top_logp.data_ptr(), self.top_ids.data_ptr(), 0, self.log_z.data_ptr(),
+                        mfd_hip.ptr(self.vocab_ids), self.workspace.data_ptr(), self.workspace.numel())
 
     def outputs(self, bs: int):
         """(top_logp [bs, K, L - 1, k] float32, top_ids [bs, K, L - 1, k] int32), views of the static buffers."""

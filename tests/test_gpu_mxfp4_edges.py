@@ -104,3 +104,30 @@ def test_candidates_from_a_ready_made_weight():
         with pytest.raises(ValueError, match="exponents"):
             ddtree_sglang_ops.DDTreeDraftTopK(weight=mxfp4_head.Mxfp4Weight(codes, exps), block_size=8, num_modes=2, budget=17,
                                               max_bs=1)
+
+
+@pytest.mark.parametrize("mxfp4", [True, False])
+def test_candidates_belong_to_the_tensors_device(monkeypatch, mxfp4):
+    """DDTreeDraftTopK launches on its tensors' GPU, whichever is current, and refuses hidden states of another device than the
+    weight's. (One GPU: the current device is said to be another, and the change to the tensors' own is looked for.)"""
+    import ddtree_sglang_ops
+    import mfd_hip
+    import mxfp4_head
+
+    codes, exps = (t.cuda() for t in _weight(20001, 256, seed=14))
+    weight = mxfp4_head.Mxfp4Weight(codes, exps)
+    if not mxfp4:
+        weight = mxfp4_head.dequantize(weight).to(torch.bfloat16)
+    head = ddtree_sglang_ops.DDTreeDraftTopK(weight=weight, block_size=8, num_modes=2, budget=17, max_bs=1)
+    x = torch.randn(16, 256, generator=torch.Generator().manual_seed(15)).to(torch.bfloat16).cuda()
+    head(x)
+    logp, ids = (t.clone() for t in head.outputs(1))
+    monkeypatch.setattr(mfd_hip, "_current_device", lambda: 1)
+    entered, device = [], torch.cuda.device
+    monkeypatch.setattr(torch.cuda, "device", lambda index: entered.append(index) or device(index))
+    head.top_logp.zero_()
+    head(x)
+    assert entered == [0]
+    assert torch.equal(head.outputs(1)[0], logp) and torch.equal(head.outputs(1)[1], ids)
+    with pytest.raises(ValueError, match="device"):
+        head(x.cpu())
