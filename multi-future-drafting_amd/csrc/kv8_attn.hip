@@ -20,13 +20,15 @@
 //    tiles ahead, and are widened on their way into LDS (K to bf16 with its scale folded in by the conversion, V to
 //    fp16), so that each code is widened once per workgroup and the products find plain MFMA operands: two buffers each
 //    of K and V, one barrier per tile. Scores of tile t + 1 and the products of tile t run interleaved in 32 slots.
-//    Bound by the issue of vector and matrix instructions (33 % and 37 % of the cycles, with two waves per SIMD to overlap
-//    them): 16 requests of 1187 .. 8033 tokens, 40 heads, 8 x 16 queries: 229 to 236 us, 0.82 PFLOP/s. One request of 4096
-//    tokens, 32 heads: 24 us and 5.4 of merge; a workgroup's 5 tiles take 11 of them, the look-ups and first loads in front 3.4.
+//    Bound by the issue of matrix and vector instructions (32 % and 37 % of the cycles) and by how the grid fills (1.5 waves
+//    per SIMD on average of the two that fit: 384 workgroups on 256 places, waves without rows, the longest request's outlast
+//    the others): 16 requests of 1187 .. 8033 tokens, 40 heads, 8 x 16 queries: 236 us, 0.80 PFLOP/s; over pages of 16 or 32
+//    tokens, with a look-up per thread, 246. One request of 4096 tokens, 32 heads: 22 us and 5.3 of merge; a workgroup's 5 tiles
+//    take 11 of them, the look-ups and first loads in front 3.4.
 //  * stream kernel, for one unit per KV head (plain decoding): nothing is shared, so each wave walks 32-key tiles of its
 //    own through its own LDS, without barriers, and the waves' results meet at the end. Bound by the cache's way from
-//    memory: 16 requests of 4748 .. 32132 tokens 137 us with the merge, 4.3 TB/s of the 4.9 that a large copy reaches. One
-//    request of 1187 tokens: 8.6 us and 3.9 of merge, latency.
+//    memory: 16 requests of 4748 .. 32132 tokens 137 us with the merge, 4.3 TB/s (a plain read of as much 6.7, a copy 4.9). One
+//    request of 1187 tokens: 8.7 us and 4.0 of merge, latency.
 // Both split a context over workgroups (a fixed number of keys each, so that a batch's long contexts become more
 // workgroups, not longer ones) and merge by log-sum-exp.
 #include <algorithm>
@@ -1131,8 +1133,9 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Args a) {
 // units of 32 through a double buffer in LDS that the waves share. A lane then holds, for its query row, the 32 keys of its
 // half; p = exp2(s scale - lse) is added up per key over the units in registers, and once at the end over the 32 lanes.
 // Every sum has one owner and one order: no atomics. Bound by issue, mostly the exponentials' (one per product of 256 flops):
-// 16 requests of 1187 .. 8033 tokens, 40 heads, 8 x 16 queries: 124 to 129 us, 0.75 PFLOP/s; one request of 4096, 32 heads:
-// 10 us in a row of calls, look-ups and latency.
+// 16 requests of 1187 .. 8033 tokens, 40 heads, 8 x 16 queries: 125 us, 0.76 PFLOP/s; one request of 4096, 32 heads: 10.9 us,
+// look-ups and latency. Plain decoding reads the keys and little else, by 1.2 waves per SIMD: the 16 requests 31.5 us (2.5 TB/s),
+// one of 4096 tokens 5.9.
 //
 // KW: the workgroup's 64-key parts. RS: waves per part, each of which takes every RS-th share of the units, their sums joined in
 // LDS in wave order. One wave per part where that leaves each CU more than a workgroup; else two, and four on half as many keys

@@ -6,21 +6,23 @@
 // takes one (page, KV head) of K or of V: it holds the page's new rows in registers while the largest magnitude is found (one
 // pass over the input), rounds the page's older rows again only if the scale grew (a shift of the exponent: exact except where
 // a code becomes subnormal), and never touches the rows behind the new ones. Prompts (16476 tokens of four requests, 8 heads)
-// are bound by memory: 22 us, 4.6 TB/s of the 4.9 that a large copy reaches. The tokens of a round (16 requests, 81 tokens)
-// take 5 us, a launch and one chain of dependent loads, and their host call 10.
+// are bound by memory: 22 us, 4.6 TB/s of the 4.9 that a large copy reaches. The tokens of a round (16 requests, 90 tokens)
+// take 5 us, a launch and one chain of dependent loads, and their eager call 12.
 //
 // Selection. score[t] = the sum over KV heads of weights[h][t], formed in fp64 and rounded once to fp32, so that the order of
 // the sum cannot decide which token stays. Scores become 32-bit keys whose unsigned order is the scores' (always-kept tokens at
 // the top, NaN at the bottom); one workgroup per request finds the budget-th largest by three histogram passes over 11, 11 and
 // 10 bits and writes the kept indices ascending by one prefix sum. Ties at the border go to the lowest index. 2048 of 8192
 // tokens, 8 heads: 12.8 us, of which 4 are the sums' way into one CU, 1.1 each pass's chain of counts, prefix sum and barriers,
-// 2 the indices; 32 requests at once 13.6.
+// 2 the indices; 32 requests at once the same. Rows wider than 16384 tokens take a kernel for the keys and one that reads them from
+// memory, whatever the lengths: 2000 tokens in rows of 32768 17.6 us in a graph, in rows of 8192 17.2; 32768 tokens 3 + 23.
 //
 // Compaction. One workgroup per (destination page, KV head) of K or of V gathers its kept rows, finds their largest magnitude,
 // and writes them with a scale of their own; the same launch moves the running sums (a workgroup per request and head, in
-// place) and clears those of the freed tail. Bound by memory: 32 requests to 1024 tokens each 37.8 us, 3.5 TB/s of gathered
-// reads and writes (as much with the kept tokens side by side; four heads to a workgroup, with the look-ups made once: no
-// gain). One request to 2048: 6.2 us, launch and latency.
+// place) and clears those of the freed tail. 32 requests to 1024 tokens each 36.3 us, 3.7 TB/s of gathered reads and writes (as
+// much with the kept tokens side by side; four heads to a workgroup, with the look-ups made once: no gain). Vector instructions
+// take 63 % of the cycles, two decodes, the maximum and an encode for each code, with 5.6 waves per SIMD under way. One request
+// to 2048: 6.0 us, launch and latency.
 #include <algorithm>
 
 #include "kv8_common.h"

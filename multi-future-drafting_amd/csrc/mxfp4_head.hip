@@ -10,9 +10,9 @@
 // lane holds is free as long as both operands agree, so the four MFMAs of such a step use k = 32 (lane / 16) + 8 j + 0 .. 7.
 //  * Wide form: a workgroup of eight waves takes a share of the vocabulary, a wave up to VT 16-row tiles of it against all
 //    of the launch's drafted rows (MTL 16-row tiles), which come through LDS in blocks of 32 to 64 KB by direct loads, double
-//    buffered, one barrier per block. Bound by the weight's way from memory with few drafted rows (151936 x 2560, 15 rows: 46
-//    us, 4.5 TB/s), by the matrix pipes with 128 (98304 x 2560, 120 rows: 61 us, 1.06 PFLOP/s with the padding to 128; a large
-//    library product reaches 1.24).
+//    buffered, one barrier per block. Bound by the weight's way from memory with few drafted rows (151936 x 2560, 15 rows: 47
+//    us, 4.5 TB/s; a plain read of the weight alone 32), by the matrix pipes with 128 (98304 x 2560, 120 rows: 61 us, 1.06
+//    PFLOP/s with the padding to 128; a large library product reaches 1.24).
 //  * K-split form, for vocabularies that leave a wave of the wide form without a tile: a workgroup takes one tile, each of its
 //    four waves every fourth step of k; the drafted rows come from L2 straight to registers, the partial sums meet in LDS
 //    and are added in wave order. Bound by latency.
