@@ -187,7 +187,8 @@ __device__ __forceinline__ int request_of_rank(const int64_t* ctx_lens, int bs, 
       rank += (cj > cb || (cj == cb && j < b)) ? 1 : 0;
     }
   }
-  return __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == rho));
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(rank == rho);
+  return hit ? __builtin_ctzll(hit) : rho;  // (none: lengths written while they were read; the index stays in range)
 }
 
 template <int CTX, int NW>

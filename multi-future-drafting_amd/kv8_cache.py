@@ -243,7 +243,7 @@ def paged_mode_block_attention_kv8(
 
     num_ctx_splits: > 1 splits contexts of ``max_ctx`` tokens in that many parts (a shorter context has fewer, a longer one
     a longer last part), joined by log-sum-exp; 0 or 1: one pass; < 0: by the batch's sizes. ``max_ctx`` (default: what the
-    page table's rows hold) changes no result, only the splits. With num_ctx_splits < 0 those of 2 to 64 requests are measured
+    page table's rows hold) only tunes the splits. With num_ctx_splits < 0 those of 2 to 64 requests are measured
     out from the lengths on the device; those of one request, of more than 64 and of a few in plain decoding are equal parts of
     max_ctx, which should be near the longest length then (one request of 4096 tokens, 32 heads, bound 131072: 8 x 16 queries
     120 us against 29, plain decoding 42 against 19). ``workspace``: a uint8 buffer of workspace_bytes(...), for capture without
