@@ -71,12 +71,14 @@ def _index(t, n: int, name: str):
 
 
 def _rows(t, count: int, heads: int, name: str):
-    """Strides of bf16 rows [count, heads, 128]."""
+    """Strides of bf16 rows [count, heads, 128] (of an axis with one entry: 0, what it has there says nothing)."""
     shape, stride = t.shape, t.stride()
     if t.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1 or shape[0] != count or \
             shape[1] != heads:
         raise ValueError(f"{name} must be bfloat16 [{count}, {heads}, {HEAD_DIM}] with contiguous rows, got {t.dtype} "
                          f"{tuple(shape)}")
+    if count == 1 or heads == 1:
+        return stride[0] if count > 1 else 0, stride[1] if heads > 1 else 0, 1
     return stride
 
 

@@ -320,3 +320,34 @@ def test_each_operator_runs_on_the_current_stream(name):
     assert not side.query()  # (it still waits: nothing above has begun)
     side.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(right, got))
+
+
+def test_one_token_and_one_head_have_no_stride():
+    """Slices of one token out of a projection of odd width, and of one head: the strides of axes with one entry mean nothing. The
+    bits are those of contiguous tensors."""
+    import kv8_cache
+
+    page = 64
+    print("case: kv8 one token, one head", flush=True)
+    d = make_pool([300], page, 1, seed=880)
+    g = _gen(881)
+    index = dict(page_table=d["table"].cuda(), req_pool_indices=d["rows"].cuda())
+    wide = _bf(g, 1, 3 * D + 1).cuda()
+    one = lambda i: wide[:, i * D:(i + 1) * D].as_strided((1, 1, D), (3 * D + 1, 3 * D + 1, 1), i * D)  # noqa: E731
+    results = []
+    for q, k, v in ((one(0), one(1), one(2)), tuple(one(i).clone(memory_format=torch.contiguous_format) for i in range(3))):
+        args = cache_args(d)
+        buf = torch.full((2, 3 * D + 1), 3.0, dtype=torch.bfloat16, device="cuda")
+        out = buf.as_strided((1, 1, D), (3 * D + 1, 3 * D + 1, 1))
+        _, lse = _attend(d, args, q, k, v, 1, 1, out=out)
+        assert bool((buf[0, D:] == 3).all()) and bool((buf[1] == 3).all())
+        w = torch.zeros(2, 1, 300, device="cuda")
+        wargs = {x: args[x] for x in ("k_cache", "k_scale", "page_size")}
+        kv8_cache.attention_weights_kv8(q=q, lse=lse, ctx_lens=d["lens"].cuda(), num_modes=1, block_size=1, scaling=SCALE,
+                                        weights=w, **wargs, **index)
+        kv8_cache.kv8_store(k=k, v=v, start_lens=torch.tensor([290]).cuda(), max_tokens=1, **index,
+                            cu_tokens=torch.tensor([0, 1], dtype=torch.int32).cuda(),
+                            **{x: y for x, y in args.items() if x != "req_pool_indices"})
+        results.append([t.clone().contiguous().view(torch.uint8) for t in (
+            out, lse, w, args["k_cache"], args["v_cache"], args["k_scale"], args["v_scale"])])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
